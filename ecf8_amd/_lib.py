@@ -107,6 +107,15 @@ _SIGNATURES = {
                                   _i32, _vp, _vp], _i32),
     "ecf8_embed_rows": ([_vp, _i64, _vp, _i64, _i64, _vp, _vp], _i32),
     "ecf8_embed_rows_checked": ([_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp], _i32),
+    # include/ecf8_paged.h: ragged batches over a paged KV cache
+    "ecf8_paged_work_bytes": ([_i64, _i64, _i32, _i32], _i64),
+    "ecf8_paged_plan": ([_vp, _vp, _vp, _vp, _vp], _i32),
+    "ecf8_paged_qk_norm_rope": ([_vp, _i64, _vp, _vp, _vp, _f32, _vp, _vp, _i64, _vp, _vp, _vp,
+                                 _i32, _vp, _vp, _vp], _i32),
+    "ecf8_paged_attention": ([_vp, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i64,
+                              _vp], _i32),
+    "ecf8_ragged_attention": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _vp,
+                               _i64, _vp], _i32),
 }
 
 EXPORTED = tuple(_SIGNATURES)

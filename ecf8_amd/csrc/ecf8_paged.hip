@@ -1,0 +1,470 @@
+// The bookkeeping of a paged KV cache on gfx950: block tables, slot maps and
+// the attention's schedule from request lengths, and the cache write of a
+// step's rows (head norms, rotary embedding, optional e4m3 codes).
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ecf8.h"
+#include "ecf8_dev.h"
+#include "ecf8_paged.h"
+#include "ecf8_paged_layout.h"
+
+namespace {
+
+using namespace ecf8::paged;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+constexpr float kFp8Max = 448.f;
+
+// --------------------------------------------------------------- the plan
+
+struct Plan {
+  int *table, *owned, *free_pages, *n_free, *starts, *lengths, *slots, *positions;
+  const int *cached, *new_tokens, *release;
+  int *refused;
+  Counts *counts;
+  Item *few, *tiles;
+  Join *few_joins, *tile_joins;
+  int seqs, rows, pages, shift, width, group;  // page size 1 << shift
+  int few_target, tile_target, tile_parts, fill_rows;
+};
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPer = kMaxSeqs / kPlanThreads;  // most sequences per thread
+
+// The i-th sequence of this thread: seqs / kPlanThreads consecutive ones
+// each, rounded up; -1 past its last.
+__device__ __forceinline__ int seq_of(int i, int seqs) {
+  const int step = (seqs + kPlanThreads - 1) / kPlanThreads;
+  const int s = step * (int)threadIdx.x + i;
+  return i < step && s < seqs ? s : -1;
+}
+
+// The exclusive prefix sums of v over the workgroup, and the total.
+__device__ __forceinline__ int block_scan(int v, int *waves, int &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int inc = ecf8::dev::wave_inclusive_scan(v);
+  __syncthreads();  // waves may still be read from the last scan
+  if (lane == 63) waves[wave] = inc;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    const int t = waves[w];
+    if (w < wave) before += t;
+    all += t;
+  }
+  total = all;
+  return before + inc - v;
+}
+
+// Exclusive prefix sums of the threads' sequences' values, into LDS (and the
+// total at out[seqs]).
+__device__ __forceinline__ int scan_seqs(const int (&v)[kPer], int seqs, int *out, int *waves) {
+  int sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += v[i];
+  int at = block_scan(sum, waves, total);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = seq_of(i, seqs);
+    if (s >= 0) out[s] = at;
+    at += v[i];
+  }
+  if (threadIdx.x == 0) out[seqs] = total;
+  __syncthreads();
+  return total;
+}
+
+// The last s < seqs with first[s] <= i: the sequence that element i of a
+// flattened ragged list belongs to (first: exclusive prefix sums).
+__device__ __forceinline__ int find_seq(const int *first, int seqs, int i) {
+  int lo = 0, hi = seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void fill_row(const Plan &a, const int *first, int i) {
+  int slot = -1, pos = -1;
+  if (i < first[a.seqs]) {
+    const int s = find_seq(first, a.seqs, i);
+    pos = a.lengths[s] - (first[s + 1] - first[s]) + (i - first[s]);
+    slot = (a.table[(size_t)s * a.width + (pos >> a.shift)] << a.shift) |
+           (pos & ((1 << a.shift) - 1));
+  }
+  a.slots[i] = slot;
+  a.positions[i] = pos;
+}
+
+// One workgroup plans the step: three prefix sums over the sequences (rows,
+// pages to take, pages to give back) say where everything goes, then pages,
+// items and rows are written element by element, each finding its sequence by
+// bisection in LDS.  All of it is latency: ~15 dependent rounds.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
+  __shared__ int s_start[kMaxSeqs + 1], s_take[kMaxSeqs + 1], s_back[kMaxSeqs + 1];
+  __shared__ int s_waves[kPlanThreads / 64];
+  __shared__ int s_bad;
+  const int tid = threadIdx.x, S = a.seqs;
+  const int page = 1 << a.shift;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  const int n_free = a.n_free[0];
+  int c[kPer], n[kPer], own[kPer], take[kPer], back[kPer];
+  bool bad = n_free < 0 || n_free > a.pages;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = seq_of(i, S);
+    c[i] = n[i] = own[i] = take[i] = back[i] = 0;
+    if (s < 0) continue;
+    c[i] = a.cached[s];
+    n[i] = a.new_tokens[s];
+    own[i] = a.owned[s];
+    if (own[i] < 0 || own[i] > a.width) bad = true, own[i] = 0;
+    if (a.release && a.release[s]) back[i] = own[i], own[i] = 0;
+    const int most = a.width << a.shift;
+    if (c[i] < 0 || n[i] < 0 || n[i] > a.rows || c[i] > most - n[i]) bad = true, c[i] = n[i] = 0;
+    take[i] = max(0, ((c[i] + n[i] + page - 1) >> a.shift) - own[i]);
+  }
+  if (bad) s_bad = 1;
+  const int rows = scan_seqs(n, S, s_start, s_waves);
+  const int taken = scan_seqs(take, S, s_take, s_waves);
+  const int given = scan_seqs(back, S, s_back, s_waves);
+  if (s_bad || rows > a.rows || taken > n_free + given || given > a.pages - n_free) {
+    for (int s = tid; s <= S; s += kPlanThreads) {
+      s_start[s] = 0;
+      a.starts[s] = 0;
+      if (s < S) a.lengths[s] = 0;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      *a.counts = Counts{0, 0, 0, 0};
+      if (a.refused) *a.refused = 1;
+    }
+    if (a.fill_rows)
+      for (int i = tid; i < a.rows; i += kPlanThreads) fill_row(a, s_start, i);
+    return;
+  }
+  // pages given back, then pages taken
+  for (int i = tid; i < given; i += kPlanThreads) {
+    const int s = find_seq(s_back, S, i);
+    int *e = a.table + (size_t)s * a.width + (i - s_back[s]);
+    a.free_pages[n_free + i] = *e;
+    *e = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = seq_of(i, S);
+    if (s < 0) continue;
+    a.owned[s] = own[i] + take[i];
+    a.starts[s] = s_start[s];
+    a.lengths[s] = c[i] + n[i];
+  }
+  if (tid == 0) {
+    a.n_free[0] = n_free + given - taken;
+    a.starts[S] = rows;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int i = tid; i < taken; i += kPlanThreads) {
+    const int s = find_seq(s_take, S, i), j = i - s_take[s];
+    const int held = a.owned[s] - (s_take[s + 1] - s_take[s]);
+    a.table[(size_t)s * a.width + held + j] = a.free_pages[n_free + given - 1 - i];
+  }
+  // The attention's schedule.  Sequences of few rows: split into parts of
+  // `per` steps of kFewKeys keys, so that about few_target parts make up
+  // the whole.
+  int units[kPer], items[kPer], parts[kPer], joins[kPer], total;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool few = n[i] > 0 && n[i] * a.group <= kFewRows;
+    units[i] = few ? (c[i] + n[i] + kFewKeys - 1) / kFewKeys : 0;
+    sum += units[i];
+  }
+  block_scan(sum, s_waves, total);
+  const int per = max(1, (total + a.few_target - 1) / a.few_target);
+  int sums[3] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    items[i] = (units[i] + per - 1) / per;
+    parts[i] = items[i] > 1 ? items[i] : 0;
+    joins[i] = items[i] > 1;
+    sums[0] += items[i], sums[1] += parts[i], sums[2] += joins[i];
+  }
+  int n_items, n_parts, n_joins;
+  int at = block_scan(sums[0], s_waves, n_items), part = block_scan(sums[1], s_waves, n_parts),
+      join = block_scan(sums[2], s_waves, n_joins);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = seq_of(i, S);
+    // equal parts, in steps
+    for (int j = 0; j < items[i]; ++j) {
+      const int k0 = (int)((int64_t)units[i] * j / items[i]) * kFewKeys;
+      const int k1 = (int)((int64_t)units[i] * (j + 1) / items[i]) * kFewKeys;
+      a.few[at + j] =
+          Item{s, 0, k0, min(k1, c[i] + n[i]), parts[i] ? part + j : -1, {0, 0, 0}};
+    }
+    if (joins[i]) a.few_joins[join] = Join{s, 0, part, parts[i]};
+    at += items[i], part += parts[i], join += joins[i];
+  }
+  // Tiles of the others.  The target's estimate takes a tile's keys as those
+  // of the middle of its sequence.
+  int tiles[kPer];
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool many = n[i] * a.group > kFewRows;
+    tiles[i] = many ? (n[i] * a.group + kTileRows - 1) / kTileRows : 0;
+    const int mid = (c[i] + (n[i] + 1) / 2 + kTileKeys - 1) / kTileKeys;
+    sum += (int)min((int64_t)tiles[i] * mid, (int64_t)(1 << 18));
+  }
+  block_scan(sum, s_waves, total);
+  const int n_tiles = scan_seqs(tiles, S, s_back, s_waves);
+  const int tper = max(kTileMinSteps, (total + a.tile_target - 1) / a.tile_target);
+  int t_items = 0, t_parts = 0, t_joins = 0;
+  for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {  // uniform
+    int k = 0, s = 0, row0 = 0, ext = 0, u = 0;
+    // the last tiles of a sequence, which read the most keys, first
+    const int i = n_tiles - 1 - (i0 + tid);
+    if (i >= 0) {
+      s = find_seq(s_back, S, i);
+      row0 = (i - s_back[s]) * kTileRows;
+      const int ns = s_start[s + 1] - s_start[s];
+      ext = a.cached[s] + min(ns, (row0 + kTileRows - 1) / a.group + 1);
+      u = (ext + kTileKeys - 1) / kTileKeys;
+      k = (u + tper - 1) / tper;
+    }
+    int all;
+    int p = block_scan(k > 1 ? k : 0, s_waves, all);
+    const bool room = t_parts + p + k <= a.tile_parts;
+    if (!room) k = k > 0;  // beyond the estimate: unsplit
+    int n_p, n_i, n_j;
+    p = t_parts + block_scan(k > 1 ? k : 0, s_waves, n_p);
+    const int q = t_items + block_scan(k, s_waves, n_i), jn = t_joins + block_scan(k > 1, s_waves, n_j);
+    for (int j = 0; j < k; ++j) {
+      const int k0 = (int)((int64_t)u * j / k) * kTileKeys;
+      const int k1 = (int)((int64_t)u * (j + 1) / k) * kTileKeys;
+      a.tiles[q + j] = Item{s, row0, k0, min(k1, ext), k > 1 ? p + j : -1, {0, 0, 0}};
+    }
+    if (k > 1) a.tile_joins[jn] = Join{s, row0, p, k};
+    t_items += n_i, t_parts += n_p, t_joins += n_j;
+  }
+  if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins};
+  if (a.fill_rows) {
+    __threadfence_block();
+    __syncthreads();
+    for (int i = tid; i < a.rows; i += kPlanThreads) fill_row(a, s_start, i);
+  }
+}
+
+// The rows of a large step, on workgroups of their own.
+constexpr int kFillThreads = 256;
+__global__ __launch_bounds__(kFillThreads) void fill_kernel(Plan a) {
+  __shared__ int s_start[kMaxSeqs + 1];
+  for (int s = threadIdx.x; s <= a.seqs; s += kFillThreads) s_start[s] = a.starts[s];
+  __syncthreads();
+  const int i = blockIdx.x * kFillThreads + threadIdx.x;
+  if (i < a.rows) fill_row(a, s_start, i);
+}
+
+// -------------------------------------------------------- the cache write
+
+__device__ __forceinline__ float bf16_f32(uint32_t h16) { return __uint_as_float(h16 << 16); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const v2bf v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[2 * j] = bf16_f32(v[j] & 0xffffu);
+    f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8f(const float *p, float (&f)[8]) {
+  const float4 a = *reinterpret_cast<const float4 *>(p);
+  const float4 b = *reinterpret_cast<const float4 *>(p + 4);
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+  f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl,
+                                                               0xF, 0xF, true));
+}
+
+// Four values / scale, clamped to +-448, as e4m3fn codes.  NaN stays NaN.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float scale) {
+  auto clamped = [scale](float x) {
+    const float y = x / scale;
+    return y != y ? y : fminf(fmaxf(y, -kFp8Max), kFp8Max);
+  };
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clamped(a), clamped(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped(c), clamped(d), lo, true);
+}
+
+struct Write {
+  const uint16_t *qkv, *qn, *kn;
+  const float *cosv, *sinv;
+  const int *slots, *positions, *step_rows;
+  int *refused;
+  uint16_t *q_out;
+  void *kp, *vp;
+  const float *ks, *vs;
+  float eps;
+  int Hq, Hkv, shift, table_len, rows, parts;  // parts: workgroups a row
+  uint32_t slots_end;                    // pages * page size
+};
+
+// 16 lanes a head, 8 dims a lane (16-byte loads); dims d and d +- 64 lie 8
+// lanes apart, the norm's sum and the rotary partner are row rotations.
+// Workgroup: one row, 16 kU heads, all loads before the arithmetic.
+template <int kU, bool kFp8>
+__global__ __launch_bounds__(256) void write_kernel(Write a) {
+  const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x % a.parts;
+  const int H = a.Hq + 2 * a.Hkv;
+  const int l = threadIdx.x & 15;
+  const int h0 = part * 16 * kU + (int)(threadIdx.x >> 4);
+  const int slot = a.slots[row], pos = a.positions[row];
+  if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused && *a.step_rows > a.rows) *a.refused = 1;
+  u32x4 x[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+    x[u] = *reinterpret_cast<const u32x4 *>(
+        a.qkv + ((size_t)row * H + min(h0 + 16 * u, H - 1)) * kD + 8 * l);
+  const u32x4 qw = *reinterpret_cast<const u32x4 *>(a.qn + 8 * l);
+  const u32x4 kw = *reinterpret_cast<const u32x4 *>(a.kn + 8 * l);
+  if ((uint32_t)slot >= a.slots_end || (uint32_t)pos >= (uint32_t)a.table_len) return;
+  float c[8], s[8];
+  load8f(a.cosv + (size_t)pos * 64 + 8 * (l & 7), c);
+  load8f(a.sinv + (size_t)pos * 64 + 8 * (l & 7), s);
+  if (l < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = -s[j];
+  }
+  const uint32_t page = (uint32_t)slot >> a.shift, off = (uint32_t)slot & ((1u << a.shift) - 1);
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int h = h0 + 16 * u;
+    if (h >= H) break;
+    float v[8];
+    unpack8(x[u], v);
+    if (h < a.Hq + a.Hkv) {
+      float w[8];
+      unpack8(h < a.Hq ? qw : kw, w);
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+      ss += dpp<0x128>(ss);  // row_ror:8
+      ss += dpp<0x124>(ss);  // row_ror:4
+      ss += dpp<0x4E>(ss);   // quad_perm 2, 3, 0, 1
+      ss += dpp<0xB1>(ss);   // quad_perm 1, 0, 3, 2
+      const float rs = rsqrtf(ss / (float)kD + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * w[j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], c[j], dpp<0x128>(v[j]) * s[j]);
+    }
+    if (h < a.Hq) {
+      *reinterpret_cast<u32x4 *>(a.q_out + ((size_t)row * a.Hq + h) * kD + 8 * l) =
+          u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                pack_bf16(v[6], v[7])};
+      continue;
+    }
+    const bool key = h < a.Hq + a.Hkv;
+    const int kh = h - a.Hq - (key ? 0 : a.Hkv);
+    const size_t at = ((((size_t)page * a.Hkv + kh) << a.shift) + off) * kD + 8 * l;
+    if constexpr (kFp8) {
+      const float sc = (key ? a.ks : a.vs)[kh];
+      *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(key ? a.kp : a.vp) + at) =
+          u32x2{codes4(v[0], v[1], v[2], v[3], sc), codes4(v[4], v[5], v[6], v[7], sc)};
+    } else {
+      *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(key ? a.kp : a.vp) + at) =
+          u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                pack_bf16(v[6], v[7])};
+    }
+  }
+}
+
+inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
+inline bool aligned(const void *p, uintptr_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+inline int launched() { return hipGetLastError() == hipSuccess ? ECF8_OK : ECF8_ERR_HIP; }
+
+}  // namespace
+
+extern "C" int64_t ecf8_paged_work_bytes(int64_t seqs, int64_t rows, int Hq, int Hkv) {
+  return sizes_ok(seqs, rows, Hq, Hkv) ? work_layout(seqs, rows, Hq, Hkv).bytes : -1;
+}
+
+extern "C" int ecf8_paged_plan(const ecf8_paged_batch *b, const int *cached,
+                               const int *new_tokens, const int *release, void *stream) {
+  if (!cached || !new_tokens) return ECF8_ERR_INVALID_ARG;
+  if (const int rc = ecf8::paged::check_batch(b)) return rc;
+  if (!aligned(cached, 4) || !aligned(new_tokens, 4) || !aligned(release, 4))
+    return ECF8_ERR_MISALIGNED;
+  const Work w = work_layout(b->seqs, b->rows, b->Hq, b->Hkv);
+  auto *base = static_cast<uint8_t *>(b->work);
+  // one launch while the rows are few enough for one workgroup
+  const bool one = b->rows <= 4 * kPlanThreads;
+  const Plan a{b->table, b->owned, b->free_pages, b->n_free, b->starts, b->lengths, b->slots,
+               b->positions, cached, new_tokens, release, b->refused,
+               reinterpret_cast<Counts *>(base), reinterpret_cast<Item *>(base + w.few_at),
+               reinterpret_cast<Item *>(base + w.tiles_at),
+               reinterpret_cast<Join *>(base + w.few_joins_at),
+               reinterpret_cast<Join *>(base + w.tile_joins_at), b->seqs, b->rows, b->pages,
+               __builtin_ctz((unsigned)b->page_size), b->width, b->Hq / b->Hkv, w.few_parts / 2,
+               w.tile_parts / 2, w.tile_parts, one};
+  plan_kernel<<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
+  if (!one)
+    fill_kernel<<<(unsigned)((b->rows + kFillThreads - 1) / kFillThreads), kFillThreads, 0,
+                  as_stream(stream)>>>(a);
+  return launched();
+}
+
+extern "C" int ecf8_paged_qk_norm_rope(const void *qkv, int64_t rows, const ecf8_paged_batch *b,
+                                       const void *q_norm, const void *k_norm, float eps,
+                                       const float *cos_t, const float *sin_t, int64_t table_len,
+                                       void *q_out, void *k_pool, void *v_pool, int fp8,
+                                       const float *k_scale, const float *v_scale, void *stream) {
+  if (!qkv || !q_norm || !k_norm || !cos_t || !sin_t || !q_out || !k_pool || !v_pool ||
+      rows <= 0 || table_len <= 0 || (fp8 && (!k_scale || !v_scale)))
+    return ECF8_ERR_INVALID_ARG;
+  if (const int rc = ecf8::paged::check_batch(b)) return rc;
+  if (rows > b->rows) return ECF8_ERR_CAPACITY;
+  if (table_len > kMaxLen) return ECF8_ERR_UNSUPPORTED;
+  if (!aligned(qkv, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) || !aligned(cos_t, 16) ||
+      !aligned(sin_t, 16) || !aligned(q_out, 16) || !aligned(k_pool, 16) || !aligned(v_pool, 16) ||
+      !aligned(k_scale, 4) || !aligned(v_scale, 4))
+    return ECF8_ERR_MISALIGNED;
+  const int H = b->Hq + 2 * b->Hkv;
+  const bool wide = rows * ((H + 15) / 16) > 2048;  // enough workgroups either way
+  const int per = wide ? 48 : 16, parts = (H + per - 1) / per;
+  const Write a{static_cast<const uint16_t *>(qkv), static_cast<const uint16_t *>(q_norm),
+                static_cast<const uint16_t *>(k_norm), cos_t, sin_t, b->slots, b->positions,
+                b->starts + b->seqs, b->refused, static_cast<uint16_t *>(q_out), k_pool, v_pool,
+                k_scale, v_scale, eps, b->Hq, b->Hkv, __builtin_ctz((unsigned)b->page_size),
+                (int)table_len, (int)rows, parts,
+                (uint32_t)b->pages * (uint32_t)b->page_size};
+  const unsigned grid = (unsigned)(rows * parts);
+#define ECF8_WRITE(U, F) write_kernel<U, F><<<grid, 256, 0, as_stream(stream)>>>(a)
+  if (wide) {
+    if (fp8) ECF8_WRITE(3, true);
+    else ECF8_WRITE(3, false);
+  } else {
+    if (fp8) ECF8_WRITE(1, true);
+    else ECF8_WRITE(1, false);
+  }
+#undef ECF8_WRITE
+  return launched();
+}
