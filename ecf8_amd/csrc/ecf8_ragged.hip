@@ -20,7 +20,7 @@ using namespace ecf8::paged;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.0e38f;  // running maximum before any score
 
-typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -59,16 +59,22 @@ __device__ __forceinline__ void widen16(u32x4 c, u32x4 (&out)[2]) {
 }
 
 // Keys and values lie in LDS as rows of 16 units of 16 bytes, unit c of row
-// `row` at c ^ turn(row).  The key operand reads one unit of 32 rows, the
-// transposing value reads four units of four rows each half wave: both find
+// `row` at c ^ turn(row).  The key operand reads one unit of 16 rows, the
+// transposing value read two units of eight rows each half wave: both find
 // all 64 banks.
-__device__ __forceinline__ int turn(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+__device__ __forceinline__ int turn(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
 // Orders this wave's LDS accesses (the hardware runs them in order): one
 // lane's writes before another's reads.
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+}
+
+// Lane n of each 16 lanes, in all of them.
+template <int n>
+__device__ __forceinline__ uint32_t row_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + n, 0xF, 0xF, true);
 }
 
 struct Attn {
@@ -91,158 +97,241 @@ struct Attn {
 
 enum Source { kPages, kPagesFp8, kPacked };
 
-// 32 rows of queries against 32 keys a step: the scores of one step, their
-// softmax and the second product.  Scores are computed transposed (S^T = K
-// Q^T), so a lane holds its query's scores of 16 keys: the running maximum
-// takes one exchange with lane ^ 32, and the probabilities are the second
-// product's B operand (O^T += V^T P^T) as they stand.  V^T comes from V's
-// rows in LDS by the transposing reads (ds_read_b64_tr_b16: 16 lanes read 4
-// keys x 16 dims, lane i gets dim i of the four keys).
-struct Wave {
-  v16f o[4];
-  float m, l;  // of query lane & 31; both halves hold the same m, each its own l
+typedef __attribute__((address_space(3))) const uint8_t lds_u8;
+
+// Where a lane finds its operands in 32 keys' rows at an LDS address: the
+// keys' dims 32 kk + 8 (lane / 16) + {0..7} of row 16 tile + lane mod 16, and
+// (transposed) the values' dim 16 d + lane mod 16 of keys 16 half + 4 (lane /
+// 16) + {0..3}.  ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 columns, lane i
+// gets column i.
+struct Operands {
+  uint32_t k, v;
+  __device__ __forceinline__ explicit Operands(int lane) {
+    const int i = lane & 15, g = lane >> 4, key = 4 * g + (i >> 2);
+    k = (uint32_t)(i * 256 + ((g ^ turn(i)) << 4));
+    v = (uint32_t)(key * 256 + ((((i & 3) >> 1) ^ turn(key)) << 4) + 8 * (i & 1));
+  }
+  // (the addresses of a step's reads differ in a few bits, which a block's
+  // 256-byte rows leave to an exclusive-or)
+  __device__ __forceinline__ lds_u8 *keys_at(lds_u8 *at) const { return fresh(at + k); }
+  __device__ __forceinline__ lds_u8 *values_at(lds_u8 *at) const { return fresh(at + v); }
+  static __device__ __forceinline__ lds_u8 *fresh(lds_u8 *p) {
+    uint32_t x = (uint32_t)(uintptr_t)p;
+    asm volatile("" : "+v"(x));  // the addresses below are formed anew, not kept in registers
+    return (lds_u8 *)(uintptr_t)x;
+  }
+  static __device__ __forceinline__ lds_u8 *bits(lds_u8 *p, uint32_t x) {
+    return (lds_u8 *)(uintptr_t)((uint32_t)(uintptr_t)p ^ x);
+  }
+  static __device__ __forceinline__ v8bf key(lds_u8 *p, int tile, int kk) {
+    return *reinterpret_cast<__attribute__((address_space(3))) const v8bf *>(
+        bits(p, (uint32_t)kk << 6) + 4096 * tile);
+  }
+  static __device__ __forceinline__ u32x4 values(lds_u8 *at, int d) {
+    lds_u8 *p = bits(at, (uint32_t)d << 5);
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p));
+    const u32x2 b = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 4096)));
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+};
+
+// T groups of 16 queries (rows) against 32 keys a step.  Scores are computed
+// transposed (S^T = K Q^T, v_mfma_f32_16x16x32_bf16), so a lane holds scores of
+// one query of each group, lane mod 16, and the probabilities are the second
+// product's B operand (O^T += V^T P^T) as they stand.
+template <int T>
+struct Rows {
+  // operands are read from LDS this many ahead of their products (and not all
+  // at once, which would take registers that the other operands live in)
+  static constexpr int kAhead = 3;
+  v4f o[T][8];
+  // of the lane's query: the whole number that its base-2 exponents are taken
+  // from (the same in all four lanes of a query), and this lane's part of the
+  // sum
+  float m[T], l[T];
 
   __device__ __forceinline__ void init() {
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+    for (int t = 0; t < T; ++t) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    m = kLowest, l = 0.f;
+      for (int d = 0; d < 8; ++d) o[t][d] = v4f{0.f, 0.f, 0.f, 0.f};
+      m[t] = kLowest, l[t] = 0.f;
+    }
   }
 
-  static __device__ __forceinline__ v16f scores(const u32x4 *s_k, const v8bf (&qf)[8], int lane) {
-    const int r = lane & 31, h = lane >> 5;
-    v16f s;
+  static __device__ __forceinline__ void scores(const Operands &at, lds_u8 *k,
+                                                const v8bf (&q)[T][4], v4f (&s)[T][2]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    for (int t = 0; t < T; ++t) s[t][0] = s[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    lds_u8 *p = at.keys_at(k);
+    v8bf f[kAhead + 1];
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      const v8bf kf = *reinterpret_cast<const v8bf *>(&s_k[r * 16 + ((2 * kk + h) ^ turn(r))]);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[kk], s, 0, 0, 0);
+    for (int i = 0; i < kAhead; ++i) f[i] = at.key(p, i & 1, i >> 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int n = i + kAhead;
+      if (n < 8) f[n % (kAhead + 1)] = at.key(p, n & 1, n >> 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        s[t][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[i % (kAhead + 1)], q[t][i >> 1],
+                                                              s[t][i & 1], 0, 0, 0);
     }
-    return s;
   }
 
-  // Four keys' values of this lane's dim 32 d + (lane & 31): keys 16 g + 8 half
-  // + 4 (lane >> 5) + {0..3}.
-  static __device__ __forceinline__ u32x2 values(const u32x4 *s_v, int d, int g, int half,
-                                                 int lane) {
-    const int i = lane & 15, key = 16 * g + 8 * half + 4 * (lane >> 5) + (i >> 2);
-    const int unit = 4 * d + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    const uint8_t *p = reinterpret_cast<const uint8_t *>(&s_v[key * 16 + (unit ^ turn(key))]) +
-                       8 * (i & 1);
-    const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_v4s *)(v4s *)const_cast<uint8_t *>(p));
-    return __builtin_bit_cast(u32x2, v);
-  }
-  static __device__ __forceinline__ u32x4 values8(const u32x4 *s_v, int d, int g, int lane) {
-    const u32x2 a = values(s_v, d, g, 0, lane), b = values(s_v, d, g, 1, lane);
-    return u32x4{a[0], a[1], b[0], b[1]};
+  __device__ __forceinline__ void second(const Operands &at, lds_u8 *v, const u32x4 (&p)[T]) {
+    v = at.values_at(v);
+    u32x4 f[kAhead + 1];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) f[d] = at.values(v, d);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      if (d + kAhead < 8) f[(d + kAhead) % (kAhead + 1)] = at.values(v, d + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(v8bf, f[d % (kAhead + 1)]), __builtin_bit_cast(v8bf, p[t]), o[t][d],
+            0, 0, 0);
+    }
   }
 
-  // One step of 32 keys from key0 on; kMasked: this lane's query reads keys
-  // up to `limit` only.
-  template <bool kMasked>
-  __device__ __forceinline__ void step(v16f s, const u32x4 *s_v, int key0, int limit, float c,
-                                       int lane) {
-    const int h = lane >> 5;
-    if constexpr (kMasked) {
+  static __device__ __forceinline__ float largest(const v4f (&s)[2]) {
+    const float a = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    const float b = fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]));
+    return fmaxf(a, b);
+  }
+
+  // Takes m to the new maxima where some query's moved by more than a factor
+  // 2^8 of its exponentials (uniform).  Below that m stays: nothing overflows,
+  // and the quotient of the sums is the same.  m is a whole number, so sums,
+  // and `pending` probabilities in bf16 that are still to be multiplied, are
+  // scaled by powers of two: exactly.
+  template <bool kPending>
+  __device__ __forceinline__ void raise(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
+    float top[T];
+    bool up = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (key0 + 8 * (i >> 2) + 4 * h + (i & 3) > limit) s[i] = -INFINITY;
+    for (int t = 0; t < T; ++t) {
+      top[t] = largest(s[t]);
+      up |= fmaf(top[t], c, -m[t]) > 8.f;
     }
-    float bm = s[0];
+    if (!__any(up)) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[i]);
-    const auto hm = __builtin_amdgcn_permlane32_swap(__float_as_uint(bm), __float_as_uint(bm),
-                                                     false, false);
-    const float mn = fmaxf(m, fmaxf(__uint_as_float(hm[0]), __uint_as_float(hm[1])));
-    // uniform: some query's maximum moved by more than a factor 2^8 of its
-    // exponentials.  Below that m stays: nothing overflows, and the quotient
-    // of the sums is the same.
-    if (__any((mn - m) * c > 8.f)) {
-      const float f = __builtin_amdgcn_exp2f((m - mn) * c);
-      l *= f;
+    for (int t = 0; t < T; ++t) {
+      float b = fmaxf(top[t], __shfl_xor(top[t], 16));
+      b = fmaxf(b, __shfl_xor(b, 32));
+      const float to = fmaxf(m[t], ceilf(b * c));
+      const float f = __builtin_amdgcn_exp2f(m[t] - to);
+      l[t] *= f;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+      for (int d = 0; d < 8; ++d) o[t][d] *= f;
+      if constexpr (kPending) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] *= f;
-      m = mn;
-    }
-    const float mc = m * c;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -mc));
-      l += s[i];
-    }
-    // Probabilities rounded to bf16 (at most 2^-8 of each, like the output's
-    // own rounding): the second product then runs at the bf16 rate.
-    u32x4 p[2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[g][j] = pack_bf16(s[8 * g + 2 * j], s[8 * g + 2 * j + 1]);
-    uint32_t odd = 0;
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        u32x4 v = values8(s_v, d, g, lane);
-        if constexpr (kMasked) {
-          // what a masked position holds must not enter, not even as 0 x inf
-          const u32x4 f = finite_or_zero(v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) odd |= f[j] ^ v[j];
-          v = f;
-        }
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, v),
-                                                       __builtin_bit_cast(v8bf, p[g]), o[d], 0, 0,
-                                                       0);
+        for (int j = 0; j < 4; ++j)
+          p[t][j] = pack_bf16(__uint_as_float(p[t][j] << 16) * f,
+                              __uint_as_float(p[t][j] & 0xffff0000u) * f);
       }
-    if constexpr (kMasked) {
-      if (__any(odd != 0)) not_finite(s, s_v, lane);  // uniform, rare
+      m[t] = to;
     }
   }
 
-  // The infinities and NaNs among a masked step's values, for the queries that
-  // give their keys a probability above zero: counted by products of zeros
-  // and ones, then added.
-  __device__ __forceinline__ void not_finite(const v16f &s, const u32x4 *s_v, int lane) {
-    u32x4 p[2];
+  // Scores -> probabilities, summed in fp32 and rounded to bf16 (at most 2^-8
+  // of each, like the output's own rounding): the second product then runs at
+  // the bf16 rate.
+  __device__ __forceinline__ void weigh(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+    for (int t = 0; t < T; ++t) {
+      v4f e[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        p[g][j] = (s[8 * g + 2 * j] > 0.f ? 0x3f80u : 0u) |
-                  (s[8 * g + 2 * j + 1] > 0.f ? 0x3f800000u : 0u);
+      for (int x = 0; x < 2; ++x) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+        for (int i = 0; i < 4; ++i) e[x][i] = __builtin_amdgcn_exp2f(fmaf(s[t][x][i], c, -m[t]));
+        p[t][2 * x] = pack_bf16(e[x][0], e[x][1]);
+        p[t][2 * x + 1] = pack_bf16(e[x][2], e[x][3]);
+      }
+      l[t] += ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) +
+              ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
+    }
+  }
+
+  // The lane's query of group t reads keys up to limit[t] only.
+  static __device__ __forceinline__ void mask(v4f (&s)[T][2], int key0, const int (&limit)[T],
+                                              int lane) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + 16 * x + 4 * (lane >> 4) + i > limit[t]) s[t][x][i] = -INFINITY;
+  }
+
+  // The second product of a step with masked positions: what they hold must
+  // not enter, not even as 0 x inf.  Infinities and NaNs are left out; returns
+  // whether there was one (uniform).
+  __device__ __forceinline__ bool second_masked(const Operands &at, lds_u8 *v,
+                                                const u32x4 (&p)[T]) {
+    uint32_t odd = 0;
+    v = at.values_at(v);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      __builtin_amdgcn_sched_barrier(0);  // few registers
+      const u32x4 vf = at.values(v, d), f = finite_or_zero(vf);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= f[j] ^ vf[j];
+      asm volatile("" : "+v"(odd));  // now, not all at the end
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, f),
+                                                          __builtin_bit_cast(v8bf, p[t]), o[t][d],
+                                                          0, 0, 0);
+    }
+    return __any(odd != 0);
+  }
+
+  // Adds the infinities and NaNs that second_masked left out of keys [first,
+  // end): each reaches the queries that read its position.  value(key, dim):
+  // four values of a key from dim on.  Rare.
+  template <class Value>
+  __device__ __forceinline__ void add_odd(int first, int end, const int (&limit)[T], int lane,
+                                          Value value) {
 #pragma unroll 1
-      for (int kind = 0; kind < 3; ++kind) {  // +inf, -inf, NaN
-        const uint32_t want = kind == 0 ? 0x7f80u : 0xff80u;
-        v16f n;
+    for (int key = first; key < end; ++key)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) n[i] = 0.f;
+      for (int d = 0; d < 8; ++d) {
+        const u32x2 v = value(key, 16 * d + 4 * (lane >> 4));
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          u32x4 v = values8(s_v, d, g, lane);
+        for (int i = 0; i < 4; ++i) {
+          const float x =
+              __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+          const bool odd = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = v[j] & 0xffffu, hi = v[j] >> 16;
-            const bool a = kind == 2 ? (lo & 0x7fffu) > 0x7f80u : lo == want;
-            const bool b = kind == 2 ? (hi & 0x7fffu) > 0x7f80u : hi == want;
-            v[j] = (a ? 0x3f80u : 0u) | (b ? 0x3f800000u : 0u);
-          }
-          n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, v),
-                                                      __builtin_bit_cast(v8bf, p[g]), n, 0, 0, 0);
+          for (int t = 0; t < T; ++t)
+            if (odd && key <= limit[t]) o[t][d][i] += x;
         }
-        const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (n[i] > 0.f) o[d][i] += add;
       }
   }
 };
+
+// The queries' operands: group t's rows are row0 + 16 t + lane mod 16, rows
+// from `end` on repeat the last; limit: the last position each reads.
+template <int T>
+__device__ __forceinline__ void load_queries(const Attn &a, int kvh, int start, int cached, int row0,
+                                             int end, int lane, v8bf (&q)[T][4],
+                                             int (&limit)[T]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int row = min(row0 + 16 * t + (lane & 15), end - 1);
+    const int tok = row / a.group, head = kvh * a.group + row % a.group;
+    limit[t] = cached + tok;
+    const uint16_t *p = a.q + (int64_t)min(start + tok, a.rows - 1) * a.q_stride + head * kD +
+                        8 * (lane >> 4);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) q[t][kk] = *reinterpret_cast<const v8bf *>(p + 32 * kk);
+  }
+}
 
 // What an item needs to know of its sequence.
 struct Place {
@@ -278,169 +367,438 @@ __device__ __forceinline__ bool find_tile(const Attn &a, int tile_rows, int vt, 
   return true;
 }
 
-// Workgroup of four waves: 32 rows (token, head of the group) of one KV head
-// against positions [k0, k1), 128 a round, 32 a wave; the waves' sums are
-// joined in LDS.  A wave stages its keys and values through registers into
-// LDS of its own, a round ahead, so the loop has no barrier.
+// The item of slot `item`; false past the last.
 template <Source kSrc>
-__global__ __launch_bounds__(256, 2) void attend32_kernel(Attn a) {
+__device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item, Place &p,
+                                         int lane) {
+  if constexpr (kSrc == kPacked) {
+    // the longest tiles of a sequence, its last, first
+    return item < a.grid && find_tile(a, tile_rows, a.grid - 1 - item, p, lane);
+  } else {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused &&
+        (a.starts[a.seqs] > a.rows || (a.others && *a.others > 0)))
+      *a.refused = 1;
+    if (item >= *a.n_items) return false;
+    const Item &it = a.items[item];
+    p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
+    p.start = a.starts[p.seq];
+    p.n = a.starts[p.seq + 1] - p.start;
+    p.cached = a.lengths[p.seq] - p.n;
+    return true;
+  }
+}
+
+// Four bf16 of a sequence's value rows at (key, dim), as they lie in memory.
+template <Source kSrc>
+__device__ __forceinline__ u32x2 value4(const Attn &a, const Place &p, int kvh, int key, int dim) {
+  if constexpr (kSrc == kPacked)
+    return *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(a.v) +
+                                            (int64_t)(p.start + key) * a.v_stride + kvh * kD + dim);
+  const uint32_t page =
+      min((uint32_t)a.table[(size_t)p.seq * a.width + (key >> a.shift)], a.pages - 1);
+  const size_t at =
+      (((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1))) * (size_t)kD + dim;
+  if constexpr (kSrc == kPages)
+    return *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(a.v) + at);
+  const uint32_t codes =
+      *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.v) + at);
+  u32x4 w[2];
+  widen16(u32x4{codes, 0, 0, 0}, w);
+  return u32x2{w[0][0], w[0][1]};
+}
+
+// Workgroup barrier that waits for LDS only (a __syncthreads would also
+// wait for the prefetched global loads).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt((0x3F & 15) | (0x3 << 14) | (0x7 << 4) | (0x0 << 8));  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Workgroup of four waves: up to 16 T rows (token, head of the group) of one
+// KV head against positions [k0, k1), 128 a round, 32 a wave; the waves' sums
+// are joined in LDS.  A wave stages its keys and values through registers into
+// LDS of its own, a round ahead, so the loop has no barrier.
+template <Source kSrc, int T>
+__global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][2][32 * 16];  // a wave's keys and values
-  __shared__ float s_m[4][32], s_l[4][32];
+  __shared__ float s_m[4][16 * T], s_l[4][16 * T];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 31, h = lane >> 5;
   const int kvh = (int)blockIdx.x % a.Hkv;
   u32x4 *s_k = s_kv[wave][0], *s_v = s_kv[wave][1];
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;      // 16-byte units of a row in memory
   constexpr int kLoads = kUnits / 2;         // per lane and 32 rows
-  constexpr int kRowsPer = 64 / kUnits;      // rows per load
+  const int unit = lane % kUnits;
+  const Operands ops(lane);
 
-  for (int item = (int)blockIdx.x / a.Hkv;; item += a.grid) {
-    Place p;
-    if constexpr (kSrc == kPacked) {
-      if (item >= a.grid) return;
-      if (!find_tile(a, kFewRows, a.grid - 1 - item, p, lane)) return;
-    } else {
-      const int count = *a.n_items;
-      if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused &&
-          (a.starts[a.seqs] > a.rows || (a.others && *a.others > 0)))
-        *a.refused = 1;
-      if (item >= count) return;
-      const Item &it = a.items[item];
-      p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
-      p.start = a.starts[p.seq];
-      p.n = a.starts[p.seq + 1] - p.start;
-      p.cached = a.lengths[p.seq] - p.n;
-    }
-    const int n_rows = min(p.n * a.group - p.row0, 32);
-    if (n_rows <= 0 || p.start < 0 || p.cached < 0) continue;  // not the planned step's lengths
-    // this lane's query: rows past the last repeat it, unstored
-    const int row = p.row0 + min(r, n_rows - 1);
-    const int tok = row / a.group, head = kvh * a.group + row % a.group;
-    const int limit = p.cached + tok;
-    const int low = p.cached + p.row0 / a.group;  // the first query's limit
-    const int token = min(p.start + tok, a.rows - 1);
+  Place p;
+  if (!get_item<kSrc>(a, 16 * T, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  const int n_rows = min(p.n * a.group - p.row0, 16 * T);
+  if (n_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned step's lengths
+  const int low = p.cached + p.row0 / a.group;  // the first query's limit
+  v8bf q[T][4];
+  int limit[T];
+  load_queries<T>(a, kvh, p.start, p.cached, p.row0, p.row0 + n_rows, lane, q, limit);
+  float c = a.scale, vscale = 1.f;
+  if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
-    v8bf qf[8];
-    const uint16_t *qp = a.q + (int64_t)token * a.q_stride + head * kD + 8 * h;
+  // the row (page, head, offset) of key key0 + 8 (lane / 16) + lane mod 8; keys
+  // past the last repeat it
+  const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
+  auto locate = [&](int key0) -> uint32_t {
+    const int key = min(key0 + 8 * (lane >> 4) + (lane & 7), p.k1 - 1);
+    if constexpr (kSrc == kPacked) return (uint32_t)(p.start + key);
+    const uint32_t page = min((uint32_t)table[key >> a.shift], a.pages - 1);
+    return ((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1));
+  };
+  u32x4 kr[kLoads], vr[kLoads];
+  auto load = [&](uint32_t at) {
+    const uint32_t rows[8] = {row_lane<0>(at), row_lane<1>(at), row_lane<2>(at),
+                              row_lane<3>(at), row_lane<4>(at), row_lane<5>(at),
+                              row_lane<6>(at), row_lane<7>(at)};
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const v8bf *>(qp + 16 * kk);
-    float c = a.scale, vscale = 1.f;
-    if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
-
-    // the row (page, head, offset) of key key0 + (lane & 31); keys past the
-    // last repeat it
-    const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
-    auto locate = [&](int key0) -> uint32_t {
-      const int key = min(key0 + r, p.k1 - 1);
-      if constexpr (kSrc == kPacked) return (uint32_t)(p.start + key);
-      const uint32_t page = min((uint32_t)table[key >> a.shift], a.pages - 1);
-      return ((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1));
-    };
-    u32x4 kr[kLoads], vr[kLoads];
-    auto load = [&](uint32_t at) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int src = (lane / kUnits) + kRowsPer * i, unit = lane % kUnits;
-        const uint32_t w = (uint32_t)__shfl((int)at, src);
-        if constexpr (kSrc == kPacked) {
-          kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) +
-                                                   (int64_t)w * a.k_stride + kvh * kD + 8 * unit);
-          vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) +
-                                                   (int64_t)w * a.v_stride + kvh * kD + 8 * unit);
-        } else {
-          kr[i] = static_cast<const u32x4 *>(a.k)[(size_t)w * kUnits + unit];
-          vr[i] = static_cast<const u32x4 *>(a.v)[(size_t)w * kUnits + unit];
-        }
-      }
-    };
-    auto store = [&]() {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int row = (lane / kUnits) + kRowsPer * i, unit = lane % kUnits;
-        if constexpr (kFp8) {
-          u32x4 w[2];
-          widen16(kr[i], w);
-          s_k[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-          s_k[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
-          widen16(vr[i], w);
-          s_v[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-          s_v[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
-        } else {
-          s_k[row * 16 + (unit ^ turn(row))] = kr[i];
-          s_v[row * 16 + (unit ^ turn(row))] = vr[i];
-        }
-      }
-    };
-
-    Wave w;
-    w.init();
-    int key0 = p.k0 + 32 * wave;
-    if (key0 < p.k1) {  // uniform
-      uint32_t at = locate(key0);
-      load(at);
-      at = locate(key0 + 128);
-      for (; key0 < p.k1; key0 += 128) {
-        wave_fence();
-        store();
-        wave_fence();
-        if (key0 + 128 < p.k1) {
-          load(at);
-          at = locate(key0 + 256);
-        }
-        const v16f s = Wave::scores(s_k, qf, lane);
-        if (key0 + 31 > low) w.step<true>(s, s_v, key0, limit, c, lane);  // uniform
-        else w.step<false>(s, s_v, key0, limit, c, lane);
-      }
-    }
-    float l = w.l + __shfl_xor(w.l, 32);
-
-    // join the waves
-    if (h == 0) s_m[wave][r] = w.m, s_l[wave][r] = l;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-    const float f = __builtin_amdgcn_exp2f((w.m - top) * c);
-    // 32 rows of 32 units of 4 sums, unit u of row r at u ^ r; over the wave's
-    // own keys and values, which it has read
-    float4 *so = reinterpret_cast<float4 *>(s_kv[wave]);
-    wave_fence();
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        so[r * 32 + ((8 * d + 2 * j + h) ^ r)] =
-            make_float4(w.o[d][4 * j] * f, w.o[d][4 * j + 1] * f, w.o[d][4 * j + 2] * f,
-                        w.o[d][4 * j + 3] * f);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * n_rows; i += 256) {
-      const int row = i >> 5, u = i & 31;
-      float4 t[4];
-      float sum = 0.f, mt = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        t[x] = reinterpret_cast<const float4 *>(s_kv[x])[row * 32 + (u ^ row)];
-        sum += s_l[x][row] * __builtin_amdgcn_exp2f((s_m[x][row] - mt) * c);
-      }
-      const float4 all = make_float4((t[0].x + t[1].x) + (t[2].x + t[3].x),
-                                     (t[0].y + t[1].y) + (t[2].y + t[3].y),
-                                     (t[0].z + t[1].z) + (t[2].z + t[3].z),
-                                     (t[0].w + t[1].w) + (t[2].w + t[3].w));
-      if (p.part >= 0) {
-        const size_t at = ((size_t)p.part * a.Hkv + kvh) * 32 + row;
-        reinterpret_cast<float4 *>(a.sums)[at * 32 + u] = all;
-        if (u == 0) a.stats[at] = make_float2(mt * c, sum);
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t even = rows[kFp8 ? 2 * i : i], odd = rows[kFp8 ? 2 * i + 1 : i];
+      const uint32_t w = lane & (kFp8 ? 8 : 0) ? odd : even;
+      if constexpr (kSrc == kPacked) {
+        kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) +
+                                                 (int64_t)w * a.k_stride + kvh * kD + 8 * unit);
+        vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) +
+                                                 (int64_t)w * a.v_stride + kvh * kD + 8 * unit);
       } else {
-        const int g = p.row0 + row;
-        const int tk = p.start + g / a.group;
-        const float inv = vscale / sum;
-        if (tk < a.rows)
-          *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
-                                     (kvh * a.group + g % a.group) * kD + 4 * u) =
-              u32x2{pack_bf16(all.x * inv, all.y * inv), pack_bf16(all.z * inv, all.w * inv)};
+        kr[i] = static_cast<const u32x4 *>(a.k)[(size_t)w * kUnits + unit];
+        vr[i] = static_cast<const u32x4 *>(a.v)[(size_t)w * kUnits + unit];
       }
     }
-    __syncthreads();  // the next item's stores come after
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = 8 * (lane >> 4) + (kFp8 ? 2 * i + ((lane >> 3) & 1) : i);
+      if constexpr (kFp8) {
+        u32x4 w[2];
+        widen16(kr[i], w);
+        s_k[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_k[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        widen16(vr[i], w);
+        s_v[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_v[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+      } else {
+        s_k[row * 16 + (unit ^ turn(row))] = kr[i];
+        s_v[row * 16 + (unit ^ turn(row))] = vr[i];
+      }
+    }
+  };
+
+  Rows<T> w;
+  w.init();
+  int key0 = p.k0 + 32 * wave;
+  bool odd = false;
+  if (key0 < p.k1) {  // uniform
+    uint32_t at = locate(key0);
+    load(at);
+    at = locate(key0 + 128);
+    for (; key0 < p.k1; key0 += 128) {
+      wave_fence();
+      store();
+      wave_fence();
+      if (key0 + 128 < p.k1) {
+        load(at);
+        at = locate(key0 + 256);
+      }
+      lds_u8 *k = (lds_u8 *)s_k, *v = (lds_u8 *)s_v;
+      v4f s[T][2];
+      u32x4 pr[T];
+      const bool masked = key0 + 31 > low;  // uniform
+      w.scores(ops, k, q, s);
+      if (masked) w.mask(s, key0, limit, lane);
+      w.template raise<false>(s, c, pr);
+      w.weigh(s, c, pr);
+      if (masked) odd |= w.second_masked(ops, v, pr);
+      else w.second(ops, v, pr);
+    }
+    if (odd)
+      for (key0 = p.k0 + 32 * wave; key0 < p.k1; key0 += 128)
+        if (key0 + 31 > low)
+          w.add_odd(key0, min(key0 + 32, p.k1), limit, lane,
+                    [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
+  }
+
+  // join the waves
+  float l[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    l[t] = w.l[t] + __shfl_xor(w.l[t], 16);
+    l[t] += __shfl_xor(l[t], 32);
+    if (lane < 16) s_m[wave][16 * t + lane] = w.m[t], s_l[wave][16 * t + lane] = l[t];
+  }
+  __syncthreads();
+  // rows of 32 units of 4 sums, unit u of row r at u ^ r; over the wave's own
+  // keys and values, which it has read
+  float4 *so = reinterpret_cast<float4 *>(s_kv[wave]);
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int r = 16 * t + (lane & 15);
+    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float f = __builtin_amdgcn_exp2f(w.m[t] - top);
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      so[r * 32 + ((4 * d + (lane >> 4)) ^ r)] =
+          make_float4(w.o[t][d][0] * f, w.o[t][d][1] * f, w.o[t][d][2] * f, w.o[t][d][3] * f);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * n_rows; i += 256) {
+    const int row = i >> 5, u = i & 31;
+    float4 t[4];
+    float sum = 0.f, mt = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      t[x] = reinterpret_cast<const float4 *>(s_kv[x])[row * 32 + (u ^ row)];
+      sum += s_l[x][row] * __builtin_amdgcn_exp2f(s_m[x][row] - mt);
+    }
+    const float4 all = make_float4((t[0].x + t[1].x) + (t[2].x + t[3].x),
+                                   (t[0].y + t[1].y) + (t[2].y + t[3].y),
+                                   (t[0].z + t[1].z) + (t[2].z + t[3].z),
+                                   (t[0].w + t[1].w) + (t[2].w + t[3].w));
+    if (p.part >= 0) {
+      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kFewRows + row;
+      reinterpret_cast<float4 *>(a.sums)[at * 32 + u] = all;
+      if (u == 0) a.stats[at] = make_float2(mt, sum);
+    } else {
+      const int g = p.row0 + row;
+      const int tk = p.start + g / a.group;
+      const float inv = vscale / sum;
+      if (tk < a.rows)
+        *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
+                                   (kvh * a.group + g % a.group) * kD + 4 * u) =
+            u32x2{pack_bf16(all.x * inv, all.y * inv), pack_bf16(all.z * inv, all.w * inv)};
+    }
+  }
+}
+
+constexpr int kT = 3;  // groups of 16 rows a wave of the tile kernel
+static_assert(kTileRows == 8 * 16 * kT, "eight waves");
+
+// Workgroup of eight waves, two a SIMD: 384 rows (token, head of the group) of
+// one KV head, 48 a wave, against positions [k0, k1).  48 rows share every
+// operand that a wave reads from LDS: at 32 the reads alone would take as
+// long as the products.
+//
+// The two waves of a SIMD take turns, a barrier apart: one runs its products
+// (the values' of the last step of 32 keys, then the next step's scores) while
+// the other runs its softmax.  Keys and values go through registers to a ring
+// of three LDS stages of 64 keys: block b + 1 is written in the phase in
+// which the first four waves run the softmax of block b's first step, when
+// its stage was last read four phases before.
+template <Source kSrc>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(Attn a) {
+  constexpr int kStage = 64 * 16;  // 16-byte units of a stage's keys, or values
+  __shared__ u32x4 s_k[3][kStage];
+  __shared__ u32x4 s_v[3][kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool behind = wave >= 4;  // uniform: a phase behind the others
+  const int kvh = (int)blockIdx.x % a.Hkv;
+  const Operands ops(lane);
+  constexpr bool kFp8 = kSrc == kPagesFp8;
+  constexpr int kUnits = kFp8 ? 8 : 16;       // 16-byte units of a row in memory
+  constexpr int kLoads = 64 * kUnits / 512;   // per thread and stage
+  const int unit = threadIdx.x % kUnits, row_of = threadIdx.x / kUnits;
+
+  Place p;
+  if (!get_item<kSrc>(a, kTileRows, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  const int all_rows = min(p.n * a.group - p.row0, kTileRows);
+  if (all_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned lengths
+  const int first_row = 16 * kT * wave, n_rows = min(all_rows - first_row, 16 * kT);
+  // the last position that the wave's last row reads
+  const int high = n_rows > 0 ? p.cached + (p.row0 + first_row + n_rows - 1) / a.group : -1;
+  v8bf q[kT][4];
+  int limit[kT];
+  load_queries<kT>(a, kvh, p.start, p.cached, p.row0 + first_row, p.row0 + all_rows, lane, q,
+                   limit);
+  float c = a.scale, vscale = 1.f;
+  if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
+
+  const int blocks = (p.k1 - p.k0 + 63) / 64;
+  const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
+  int entry[kLoads];  // pages of the rows to be loaded next
+  auto look = [&](int b) {
+    if constexpr (kSrc != kPacked) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        entry[i] = table[min(p.k0 + 64 * b + row_of + (64 / kLoads) * i, p.k1 - 1) >> a.shift];
+    }
+  };
+  u32x4 kr[kLoads], vr[kLoads];
+  auto load = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      // keys past the last repeat it
+      const int key = min(p.k0 + 64 * b + row_of + (64 / kLoads) * i, p.k1 - 1);
+      if constexpr (kSrc == kPacked) {
+        const int64_t at = p.start + key;
+        kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) +
+                                                 at * a.k_stride + kvh * kD + 8 * unit);
+        vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) +
+                                                 at * a.v_stride + kvh * kD + 8 * unit);
+      } else {
+        const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
+        const size_t at = (((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1))) *
+                              (size_t)kUnits + unit;
+        kr[i] = static_cast<const u32x4 *>(a.k)[at];
+        vr[i] = static_cast<const u32x4 *>(a.v)[at];
+      }
+    }
+  };
+  auto store = [&](int st) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = row_of + (64 / kLoads) * i;
+      if constexpr (kFp8) {
+        u32x4 w[2];
+        widen16(kr[i], w);
+        s_k[st][row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_k[st][row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        widen16(vr[i], w);
+        s_v[st][row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_v[st][row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+      } else {
+        s_k[st][row * 16 + (unit ^ turn(row))] = kr[i];
+        s_v[st][row * 16 + (unit ^ turn(row))] = vr[i];
+      }
+    }
+  };
+  // block b + 1 to its stage, block b + 2 on its way
+  auto stage = [&](int b, int st) {
+    if (b + 1 < blocks) {
+      store(st);
+      load(b + 2);
+      look(b + 3);
+    }
+  };
+  auto phase = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  Rows<kT> w;
+  w.init();
+  v4f s[kT][2];
+  u32x4 pr[kT];
+  auto at = [&](const u32x4 (&s)[3][kStage], int st, int half) {
+    return (lds_u8 *)s[st] + 8192 * half;
+  };
+  // (a step without work leaves zeros: nothing stays live through it)
+  auto clear = [](auto &x) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) x[t] = {};
+  };
+  auto clear2 = [](v4f (&x)[kT][2]) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) x[t][0] = x[t][1] = v4f{};
+  };
+  // whether this wave has any of a step
+  auto any = [&](int key0) { return key0 <= high && key0 < p.k1; };
+  auto softmax = [&](int key0) {
+    if (!any(key0)) {
+      clear(pr);
+      return;
+    }
+    w.mask(s, key0, limit, lane);
+    w.template raise<false>(s, c, pr);
+    w.weigh(s, c, pr);
+  };
+
+  look(0);
+  load(0);
+  look(1);
+  store(0);
+  load(1);
+  look(2);
+  phase();
+  if (behind) {
+    phase();
+    stage(0, 1);
+  }
+  clear(pr);
+  clear2(s);
+  if (any(p.k0)) w.scores(ops, at(s_k, 0, 0), q, s);
+  phase();
+  const int steps = 2 * blocks;
+  bool odd = false;
+  int st = 0;  // stage of step j's block
+  int j = 0;
+  // Steps that every row of the workgroup reads in full (and that are not the
+  // last): all waves alike, without a condition.
+  const int full = max(0, min((p.cached + p.row0 / a.group + 1 - p.k0) / 32, steps - 1));
+#pragma unroll 1
+  for (; j < full; ++j) {
+    const int half = j & 1, st1 = st == 2 ? 0 : st + 1;
+    if (!half && !behind) stage(j >> 1, st1);
+    __builtin_amdgcn_s_setprio(1);
+    w.template raise<false>(s, c, pr);
+    w.weigh(s, c, pr);
+    __builtin_amdgcn_s_setprio(0);
+    phase();
+    if (half && behind) stage((j + 1) >> 1, st1 == 2 ? 0 : st1 + 1);
+    w.second(ops, at(s_v, st, half), pr);
+    w.scores(ops, at(s_k, half ? st1 : st, 1 - half), q, s);
+    phase();
+    if (half) st = st1;
+  }
+#pragma unroll 1
+  for (;; ++j) {
+    const int key0 = p.k0 + 32 * j, half = j & 1;
+    const int st1 = st == 2 ? 0 : st + 1;
+    // softmax (the other four waves: products)
+    if (!half && !behind) stage(j >> 1, st1);
+    __builtin_amdgcn_s_setprio(1);
+    softmax(key0);
+    __builtin_amdgcn_s_setprio(0);
+    phase();
+    // products (the other four waves: softmax)
+    if (half && behind) stage((j + 1) >> 1, st1 == 2 ? 0 : st1 + 1);
+    if (any(key0)) odd |= w.second_masked(ops, at(s_v, st, half), pr);
+    if (j + 1 == steps) break;
+    if (any(key0 + 32)) w.scores(ops, at(s_k, half ? st1 : st, 1 - half), q, s);
+    else clear2(s);
+    phase();
+    if (half) st = st1;
+  }
+  if (!behind) phase();
+  if (n_rows <= 0) return;
+  if (odd)
+    w.add_odd(p.k0 + 32 * full, min(high + 1, p.k1), limit, lane,
+              [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    float l = w.l[t] + __shfl_xor(w.l[t], 16);
+    l += __shfl_xor(l, 32);
+    const int row = first_row + 16 * t + (lane & 15), g = lane >> 4;
+    if (row >= all_rows) continue;
+    if (p.part >= 0) {
+      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kTileRows + row;
+      v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
+      if (g == 0) a.stats[at] = make_float2(w.m[t], l);
+    } else {
+      const int at = p.row0 + row, tk = p.start + at / a.group;
+      const float inv = vscale / l;
+      if (tk < a.rows) {
+        uint16_t *op = a.out + (int64_t)tk * a.out_stride +
+                       (kvh * a.group + at % a.group) * kD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          *reinterpret_cast<u32x2 *>(op + 16 * d) =
+              u32x2{pack_bf16(w.o[t][d][0] * inv, w.o[t][d][1] * inv),
+                    pack_bf16(w.o[t][d][2] * inv, w.o[t][d][3] * inv)};
+      }
+    }
   }
 }
 
@@ -534,8 +892,14 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     a.sums = reinterpret_cast<float *>(base + w.few_sums);
     a.grid = w.few_parts / 2 + (int)(rows < b->seqs ? rows : b->seqs);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
-    if (fp8) attend32_kernel<kPagesFp8><<<grid, 256, 0, as_stream(stream)>>>(a);
-    else attend32_kernel<kPages><<<grid, 256, 0, as_stream(stream)>>>(a);
+#define ECF8_FEW(S, T) few_kernel<S, T><<<grid, 256, 0, as_stream(stream)>>>(a)
+    if (max_new * G <= 16) {
+      if (fp8) ECF8_FEW(kPagesFp8, 1);
+      else ECF8_FEW(kPages, 1);
+    } else {
+      if (fp8) ECF8_FEW(kPagesFp8, 2);
+      else ECF8_FEW(kPages, 2);
+    }
     join_kernel<<<dim3((unsigned)(w.few_parts / 2 * a.Hkv), 1), 256, 0, as_stream(stream)>>>(
         a, &counts->few_joins, reinterpret_cast<const Join *>(base + w.few_joins_at), kFewRows);
   }
@@ -547,8 +911,8 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     const int64_t items = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs) + w.tile_parts;
     a.grid = (int)(items < w.tile_items ? items : w.tile_items);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
-    if (fp8) attend32_kernel<kPagesFp8><<<grid, 256, 0, as_stream(stream)>>>(a);
-    else attend32_kernel<kPages><<<grid, 256, 0, as_stream(stream)>>>(a);
+    if (fp8) tile_kernel<kPagesFp8><<<grid, 512, 0, as_stream(stream)>>>(a);
+    else tile_kernel<kPages><<<grid, 512, 0, as_stream(stream)>>>(a);
     join_kernel<<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 32), 256, 0,
                   as_stream(stream)>>>(
         a, &counts->tile_joins, reinterpret_cast<const Join *>(base + w.tile_joins_at), kTileRows);
@@ -577,7 +941,11 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
   a.starts = starts;
   a.Hkv = Hkv, a.group = Hq / Hkv, a.rows = (int)rows, a.seqs = (int)seqs;
   a.scale = kLog2e / sqrtf((float)kD);
-  a.grid = (int)(rows * a.group / kFewRows + seqs);
-  attend32_kernel<kPacked><<<(unsigned)((int64_t)a.grid * Hkv), 256, 0, as_stream(stream)>>>(a);
+  const bool wide_tiles = rows * Hq / kTileRows >= 48;
+  a.grid = (int)(rows * a.group / (wide_tiles ? kTileRows : kFewRows) + seqs);
+  const unsigned grid = (unsigned)((int64_t)a.grid * Hkv);
+  if (wide_tiles) tile_kernel<kPacked><<<grid, 512, 0, as_stream(stream)>>>(a);
+  else ECF8_FEW(kPacked, 2);
+#undef ECF8_FEW
   return launched();
 }
