@@ -18,7 +18,7 @@ namespace {
 using namespace ecf8::paged;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -3.0e38f;  // running maximum before any score
+constexpr float kLowest = -3.0e38f;  // stands for the maximum of no keys
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -156,7 +156,7 @@ struct Rows {
     for (int t = 0; t < T; ++t) {
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[t][d] = v4f{0.f, 0.f, 0.f, 0.f};
-      m[t] = kLowest, l[t] = 0.f;
+      m[t] = l[t] = 0.f;
     }
   }
 
@@ -197,62 +197,57 @@ struct Rows {
     }
   }
 
-  static __device__ __forceinline__ float largest(const v4f (&s)[2]) {
-    const float a = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-    const float b = fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]));
-    return fmaxf(a, b);
-  }
-
-  // Takes m to the new maxima where some query's moved by more than a factor
-  // 2^8 of its exponentials (uniform).  Below that m stays: nothing overflows,
-  // and the quotient of the sums is the same.  m is a whole number, so sums,
-  // and `pending` probabilities in bf16 that are still to be multiplied, are
-  // scaled by powers of two: exactly.
-  template <bool kPending>
-  __device__ __forceinline__ void raise(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
+  // Scores -> probabilities: base-2 exponents from m, summed in fp32 and
+  // rounded to bf16 (at most 2^-8 of each, like the output's own rounding): the
+  // second product then runs at the bf16 rate.
+  //
+  // Where a query's largest exponent is above 8, or it has no sum yet, m goes
+  // to its largest exponent first (uniform, rare).  Otherwise m stays: nothing
+  // overflows, and the quotient of the sums is the same.  m is a whole number,
+  // so sums are scaled by powers of two: exactly.
+  __device__ __forceinline__ void weigh(v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
     float top[T];
     bool up = false;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      top[t] = largest(s[t]);
-      up |= fmaf(top[t], c, -m[t]) > 8.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][x][i] = fmaf(s[t][x][i], c, -m[t]);
+      const v4f a = s[t][0], b = s[t][1];
+      top[t] = fmaxf(fmaxf(fmaxf(fmaxf(a[0], a[1]), a[2]), fmaxf(fmaxf(a[3], b[0]), b[1])),
+                     fmaxf(b[2], b[3]));
+      up |= top[t] > 8.f || !(l[t] > 0.f);
     }
-    if (!__any(up)) return;
+    if (__any(up)) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      float b = fmaxf(top[t], __shfl_xor(top[t], 16));
-      b = fmaxf(b, __shfl_xor(b, 32));
-      const float to = fmaxf(m[t], ceilf(b * c));
-      const float f = __builtin_amdgcn_exp2f(m[t] - to);
-      l[t] *= f;
+      for (int t = 0; t < T; ++t) {
+        float b = fmaxf(top[t], __shfl_xor(top[t], 16));
+        b = ceilf(fmaxf(b, __shfl_xor(b, 32)));
+        float sum = l[t] + __shfl_xor(l[t], 16);
+        sum += __shfl_xor(sum, 32);
+        const bool none = sum == 0.f;  // m may also go down
+        const float by = none ? (b > -INFINITY ? b : 0.f) : fmaxf(b, 0.f);
+        const float f = none ? 1.f : __builtin_amdgcn_exp2f(-by);
+        m[t] += by;
+        l[t] *= f;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) o[t][d] *= f;
-      if constexpr (kPending) {
+        for (int d = 0; d < 8; ++d) o[t][d] *= f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          p[t][j] = pack_bf16(__uint_as_float(p[t][j] << 16) * f,
-                              __uint_as_float(p[t][j] & 0xffff0000u) * f);
+        for (int x = 0; x < 2; ++x) s[t][x] -= by;
       }
-      m[t] = to;
     }
-  }
-
-  // Scores -> probabilities, summed in fp32 and rounded to bf16 (at most 2^-8
-  // of each, like the output's own rounding): the second product then runs at
-  // the bf16 rate.
-  __device__ __forceinline__ void weigh(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      v4f e[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[x][i] = __builtin_amdgcn_exp2f(fmaf(s[t][x][i], c, -m[t]));
-        p[t][2 * x] = pack_bf16(e[x][0], e[x][1]);
-        p[t][2 * x + 1] = pack_bf16(e[x][2], e[x][3]);
+        for (int i = 0; i < 4; ++i) s[t][x][i] = __builtin_amdgcn_exp2f(s[t][x][i]);
+        p[t][2 * x] = pack_bf16(s[t][x][0], s[t][x][1]);
+        p[t][2 * x + 1] = pack_bf16(s[t][x][2], s[t][x][3]);
       }
-      l[t] += ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) +
-              ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
+      l[t] += ((s[t][0][0] + s[t][0][1]) + (s[t][0][2] + s[t][0][3])) +
+              ((s[t][1][0] + s[t][1][1]) + (s[t][1][2] + s[t][1][3]));
     }
   }
 
@@ -515,7 +510,6 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       const bool masked = key0 + 31 > low;  // uniform
       w.scores(ops, k, q, s);
       if (masked) w.mask(s, key0, limit, lane);
-      w.template raise<false>(s, c, pr);
       w.weigh(s, c, pr);
       if (masked) odd |= w.second_masked(ops, v, pr);
       else w.second(ops, v, pr);
@@ -533,6 +527,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   for (int t = 0; t < T; ++t) {
     l[t] = w.l[t] + __shfl_xor(w.l[t], 16);
     l[t] += __shfl_xor(l[t], 32);
+    if (l[t] == 0.f) w.m[t] = kLowest;
     if (lane < 16) s_m[wave][16 * t + lane] = w.m[t], s_l[wave][16 * t + lane] = l[t];
   }
   __syncthreads();
@@ -587,25 +582,27 @@ static_assert(kTileRows == 8 * 16 * kT, "eight waves");
 // operand that a wave reads from LDS: at 32 the reads alone would take as
 // long as the products.
 //
-// The two waves of a SIMD take turns, a barrier apart: one runs its products
-// (the values' of the last step of 32 keys, then the next step's scores) while
-// the other runs its softmax.  Keys and values go through registers to a ring
-// of three LDS stages of 64 keys: block b + 1 is written in the phase in
-// which the first four waves run the softmax of block b's first step, when
-// its stage was last read four phases before.
+// A wave's step of 32 keys is its softmax, the second product, and the next
+// step's scores.  The two waves of a SIMD are half a step apart, so that one
+// multiplies while the other runs its softmax: the waves behind wait for the
+// others' first scores.  Keys and values go through registers to a ring of
+// four LDS stages of 64 keys, two blocks ahead, with one barrier a block:
+// between barriers b and b + 1 the waves read blocks b - 1, b and b + 1, and
+// write b + 2.
 template <Source kSrc>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(Attn a) {
+__global__ __launch_bounds__(512) void tile_kernel(Attn a) {
   constexpr int kStage = 64 * 16;  // 16-byte units of a stage's keys, or values
-  __shared__ u32x4 s_k[3][kStage];
-  __shared__ u32x4 s_v[3][kStage];
+  __shared__ u32x4 s_k[4][kStage];
+  __shared__ u32x4 s_v[4][kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool behind = wave >= 4;  // uniform: a phase behind the others
+  const bool behind = wave >= 4;  // uniform: half a step behind the others
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;       // 16-byte units of a row in memory
   constexpr int kLoads = 64 * kUnits / 512;   // per thread and stage
+  constexpr int kPer = 64 / kLoads;           // rows apart
   const int unit = threadIdx.x % kUnits, row_of = threadIdx.x / kUnits;
 
   Place p;
@@ -622,28 +619,33 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
-  const int blocks = (p.k1 - p.k0 + 63) / 64;
+  const int blocks = (p.k1 - p.k0 + 63) / 64, steps = 2 * blocks;
   const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
   int entry[kLoads];  // pages of the rows to be loaded next
   auto look = [&](int b) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        entry[i] = table[min(p.k0 + 64 * b + row_of + (64 / kLoads) * i, p.k1 - 1) >> a.shift];
+        entry[i] = table[min(p.k0 + 64 * b + row_of + kPer * i, p.k1 - 1) >> a.shift];
     }
   };
   u32x4 kr[kLoads], vr[kLoads];
-  auto load = [&](int b) {
+  auto load = [&](int b, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
+    // keys past the last repeat it
+    const int key0 = p.k0 + 64 * min(b, blocks - 1);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      // keys past the last repeat it
-      const int key = min(p.k0 + 64 * b + row_of + (64 / kLoads) * i, p.k1 - 1);
+      const int key = min(key0 + row_of + kPer * i, p.k1 - 1);
       if constexpr (kSrc == kPacked) {
-        const int64_t at = p.start + key;
-        kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) +
-                                                 at * a.k_stride + kvh * kD + 8 * unit);
-        vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) +
-                                                 at * a.v_stride + kvh * kD + 8 * unit);
+        // a block's base is scalar, a lane's offset has 32 bits
+        const int64_t at = p.start + key0;
+        const auto *kb = reinterpret_cast<const uint8_t *>(
+            static_cast<const uint16_t *>(a.k) + at * a.k_stride + kvh * kD);
+        const auto *vb = reinterpret_cast<const uint8_t *>(
+            static_cast<const uint16_t *>(a.v) + at * a.v_stride + kvh * kD);
+        const uint32_t row = (uint32_t)(key - key0);
+        kr[i] = *reinterpret_cast<const u32x4 *>(kb + (row * (uint32_t)a.k_stride * 2u + 16u * unit));
+        vr[i] = *reinterpret_cast<const u32x4 *>(vb + (row * (uint32_t)a.v_stride * 2u + 16u * unit));
       } else {
         const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
         const size_t at = (((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1))) *
@@ -653,10 +655,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
   };
-  auto store = [&](int st) {
+  auto store = [&](int st, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int row = row_of + (64 / kLoads) * i;
+      const int row = row_of + kPer * i;
       if constexpr (kFp8) {
         u32x4 w[2];
         widen16(kr[i], w);
@@ -671,105 +673,78 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
   };
-  // block b + 1 to its stage, block b + 2 on its way
-  auto stage = [&](int b, int st) {
-    if (b + 1 < blocks) {
-      store(st);
-      load(b + 2);
-      look(b + 3);
-    }
-  };
-  auto phase = [] {
+  // barrier b; then block b + 2 to its stage, block b + 3 on its way
+  auto advance = [&](int b) {
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    if (b + 2 < blocks) {
+      store((b + 2) & 3, kr, vr);
+      load(b + 3, kr, vr);
+      look(b + 4);
+    }
   };
+  auto keys = [&](int j) { return (lds_u8 *)s_k[(j >> 1) & 3] + 8192 * (j & 1); };
+  auto values = [&](int j) { return (lds_u8 *)s_v[(j >> 1) & 3] + 8192 * (j & 1); };
 
   Rows<kT> w;
   w.init();
   v4f s[kT][2];
   u32x4 pr[kT];
-  auto at = [&](const u32x4 (&s)[3][kStage], int st, int half) {
-    return (lds_u8 *)s[st] + 8192 * half;
-  };
-  // (a step without work leaves zeros: nothing stays live through it)
-  auto clear = [](auto &x) {
-#pragma unroll
-    for (int t = 0; t < kT; ++t) x[t] = {};
-  };
-  auto clear2 = [](v4f (&x)[kT][2]) {
-#pragma unroll
-    for (int t = 0; t < kT; ++t) x[t][0] = x[t][1] = v4f{};
-  };
-  // whether this wave has any of a step
-  auto any = [&](int key0) { return key0 <= high && key0 < p.k1; };
-  auto softmax = [&](int key0) {
-    if (!any(key0)) {
-      clear(pr);
-      return;
-    }
-    w.mask(s, key0, limit, lane);
-    w.template raise<false>(s, c, pr);
-    w.weigh(s, c, pr);
-  };
-
-  look(0);
-  load(0);
-  look(1);
-  store(0);
-  load(1);
-  look(2);
-  phase();
-  if (behind) {
-    phase();
-    stage(0, 1);
+  {
+    u32x4 k1[kLoads], v1[kLoads];
+    look(0);
+    load(0, kr, vr);
+    look(1);
+    load(1, k1, v1);
+    look(2);
+    store(0, kr, vr);
+    store(1, k1, v1);
+    load(2, kr, vr);
+    look(3);
+    lds_barrier();
   }
-  clear(pr);
-  clear2(s);
-  if (any(p.k0)) w.scores(ops, at(s_k, 0, 0), q, s);
-  phase();
-  const int steps = 2 * blocks;
-  bool odd = false;
-  int st = 0;  // stage of step j's block
-  int j = 0;
+  if (behind) advance(0);
+  // A step of which this wave has nothing leaves zeros: nothing stays live
+  // through it.
+  auto any = [&](int j) { return p.k0 + 32 * j <= high && p.k0 + 32 * j < p.k1; };
+  auto scores = [&](int j) {
+    if (any(j)) {
+      w.scores(ops, keys(j), q, s);
+    } else {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) s[t][0] = s[t][1] = v4f{};
+    }
+  };
+  scores(0);
   // Steps that every row of the workgroup reads in full (and that are not the
   // last): all waves alike, without a condition.
   const int full = max(0, min((p.cached + p.row0 / a.group + 1 - p.k0) / 32, steps - 1));
+  int j = 0;
 #pragma unroll 1
   for (; j < full; ++j) {
-    const int half = j & 1, st1 = st == 2 ? 0 : st + 1;
-    if (!half && !behind) stage(j >> 1, st1);
-    __builtin_amdgcn_s_setprio(1);
-    w.template raise<false>(s, c, pr);
+    if (!behind && !(j & 1)) advance(j >> 1);
     w.weigh(s, c, pr);
-    __builtin_amdgcn_s_setprio(0);
-    phase();
-    if (half && behind) stage((j + 1) >> 1, st1 == 2 ? 0 : st1 + 1);
-    w.second(ops, at(s_v, st, half), pr);
-    w.scores(ops, at(s_k, half ? st1 : st, 1 - half), q, s);
-    phase();
-    if (half) st = st1;
+    if (behind && (j & 1)) advance((j + 1) >> 1);
+    w.second(ops, values(j), pr);
+    w.scores(ops, keys(j + 1), q, s);
   }
+  bool odd = false;
 #pragma unroll 1
   for (;; ++j) {
-    const int key0 = p.k0 + 32 * j, half = j & 1;
-    const int st1 = st == 2 ? 0 : st + 1;
-    // softmax (the other four waves: products)
-    if (!half && !behind) stage(j >> 1, st1);
-    __builtin_amdgcn_s_setprio(1);
-    softmax(key0);
-    __builtin_amdgcn_s_setprio(0);
-    phase();
-    // products (the other four waves: softmax)
-    if (half && behind) stage((j + 1) >> 1, st1 == 2 ? 0 : st1 + 1);
-    if (any(key0)) odd |= w.second_masked(ops, at(s_v, st, half), pr);
+    if (!behind && !(j & 1)) advance(j >> 1);
+    if (any(j)) {
+      w.mask(s, p.k0 + 32 * j, limit, lane);
+      w.weigh(s, c, pr);
+    } else {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) pr[t] = u32x4{};
+    }
+    if (behind && (j & 1) && j + 1 < steps) advance((j + 1) >> 1);
+    if (any(j)) odd |= w.second_masked(ops, values(j), pr);
     if (j + 1 == steps) break;
-    if (any(key0 + 32)) w.scores(ops, at(s_k, half ? st1 : st, 1 - half), q, s);
-    else clear2(s);
-    phase();
-    if (half) st = st1;
+    scores(j + 1);
   }
-  if (!behind) phase();
   if (n_rows <= 0) return;
   if (odd)
     w.add_odd(p.k0 + 32 * full, min(high + 1, p.k1), limit, lane,
@@ -785,7 +760,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
-      if (g == 0) a.stats[at] = make_float2(w.m[t], l);
+      if (g == 0) a.stats[at] = make_float2(l == 0.f ? kLowest : w.m[t], l);
     } else {
       const int at = p.row0 + row, tk = p.start + at / a.group;
       const float inv = vscale / l;
@@ -928,7 +903,8 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
     return ECF8_ERR_INVALID_ARG;
   const int64_t wide = (int64_t)Hq * kD, kv = (int64_t)Hkv * kD;
   if (!sizes_ok(seqs, rows, Hq, Hkv) || q_stride % 8 || k_stride % 8 || v_stride % 8 ||
-      out_stride % 4 || (rows > 1 && (q_stride < wide || out_stride < wide || k_stride < kv ||
+      out_stride % 4 || k_stride > (1 << 24) || v_stride > (1 << 24) ||
+      (rows > 1 && (q_stride < wide || out_stride < wide || k_stride < kv ||
                                       v_stride < kv)))
     return ECF8_ERR_UNSUPPORTED;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8) ||
