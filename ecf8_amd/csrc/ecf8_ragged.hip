@@ -575,34 +575,30 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
 }
 
 constexpr int kT = 3;  // groups of 16 rows a wave of the tile kernel
-static_assert(kTileRows == 8 * 16 * kT, "eight waves");
+static_assert(kTileRows == 4 * 16 * kT, "four waves");
 
-// Workgroup of eight waves, two a SIMD: 384 rows (token, head of the group) of
-// one KV head, 48 a wave, against positions [k0, k1).  48 rows share every
-// operand that a wave reads from LDS: at 32 the reads alone would take as
-// long as the products.
+// Workgroup of four waves, one a SIMD, two workgroups a CU: 192 rows (token,
+// head of the group) of one KV head, 48 a wave, against positions [k0, k1).
+// 48 rows share every operand that a wave reads from LDS: at 32 the reads
+// alone would take as long as the products.
 //
 // A wave's step of 32 keys is its softmax, the second product, and the next
-// step's scores.  The two waves of a SIMD are half a step apart, so that one
-// multiplies while the other runs its softmax: the waves behind wait for the
-// others' first scores.  Keys and values go through registers to a ring of
-// four LDS stages of 64 keys, two blocks ahead, with one barrier a block:
-// between barriers b and b + 1 the waves read blocks b - 1, b and b + 1, and
-// write b + 2.
+// step's scores; the other workgroup's wave multiplies meanwhile.  Keys and
+// values go through registers to a ring of three LDS stages, two steps ahead,
+// with one barrier a step: after barrier j the waves read the values of step j
+// and the keys of step j + 1, and write step j + 2.
 template <Source kSrc>
-__global__ __launch_bounds__(512) void tile_kernel(Attn a) {
-  constexpr int kStage = 64 * 16;  // 16-byte units of a stage's keys, or values
-  __shared__ u32x4 s_k[4][kStage];
-  __shared__ u32x4 s_v[4][kStage];
+__global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
+  constexpr int kStage = 32 * 16;  // 16-byte units of a stage's keys, or values
+  __shared__ u32x4 s_kv[3][2][kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool behind = wave >= 4;  // uniform: half a step behind the others
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;       // 16-byte units of a row in memory
-  constexpr int kLoads = 64 * kUnits / 512;   // per thread and stage
-  constexpr int kPer = 64 / kLoads;           // rows apart
+  constexpr int kLoads = 32 * kUnits / 256;   // per thread and stage
+  constexpr int kPer = 32 / kLoads;           // rows apart
   const int unit = threadIdx.x % kUnits, row_of = threadIdx.x / kUnits;
 
   Place p;
@@ -619,25 +615,25 @@ __global__ __launch_bounds__(512) void tile_kernel(Attn a) {
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
-  const int blocks = (p.k1 - p.k0 + 63) / 64, steps = 2 * blocks;
+  const int steps = (p.k1 - p.k0 + 31) / 32;
   const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
   int entry[kLoads];  // pages of the rows to be loaded next
-  auto look = [&](int b) {
+  auto look = [&](int j) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        entry[i] = table[min(p.k0 + 64 * b + row_of + kPer * i, p.k1 - 1) >> a.shift];
+        entry[i] = table[min(p.k0 + 32 * j + row_of + kPer * i, p.k1 - 1) >> a.shift];
     }
   };
   u32x4 kr[kLoads], vr[kLoads];
-  auto load = [&](int b, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
+  auto load = [&](int j, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
     // keys past the last repeat it
-    const int key0 = p.k0 + 64 * min(b, blocks - 1);
+    const int key0 = p.k0 + 32 * min(j, steps - 1);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int key = min(key0 + row_of + kPer * i, p.k1 - 1);
       if constexpr (kSrc == kPacked) {
-        // a block's base is scalar, a lane's offset has 32 bits
+        // a step's base is scalar, a lane's offset has 32 bits
         const int64_t at = p.start + key0;
         const auto *kb = reinterpret_cast<const uint8_t *>(
             static_cast<const uint16_t *>(a.k) + at * a.k_stride + kvh * kD);
@@ -656,36 +652,42 @@ __global__ __launch_bounds__(512) void tile_kernel(Attn a) {
     }
   };
   auto store = [&](int st, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
+    u32x4 *s_k = s_kv[st][0], *s_v = s_kv[st][1];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row_of + kPer * i;
       if constexpr (kFp8) {
         u32x4 w[2];
         widen16(kr[i], w);
-        s_k[st][row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_k[st][row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_k[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_k[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
         widen16(vr[i], w);
-        s_v[st][row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_v[st][row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_v[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
+        s_v[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
       } else {
-        s_k[st][row * 16 + (unit ^ turn(row))] = kr[i];
-        s_v[st][row * 16 + (unit ^ turn(row))] = vr[i];
+        s_k[row * 16 + (unit ^ turn(row))] = kr[i];
+        s_v[row * 16 + (unit ^ turn(row))] = vr[i];
       }
     }
   };
-  // barrier b; then block b + 2 to its stage, block b + 3 on its way
-  auto advance = [&](int b) {
+  int st = 0, st1 = 1, st2 = 2;  // stages of steps j, j + 1, j + 2
+  // barrier j; then step j + 2 to its stage, step j + 3 on its way
+  auto advance = [&](int j) {
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (b + 2 < blocks) {
-      store((b + 2) & 3, kr, vr);
-      load(b + 3, kr, vr);
-      look(b + 4);
+    if (j + 2 < steps) {
+      store(st2, kr, vr);
+      load(j + 3, kr, vr);
+      look(j + 4);
     }
   };
-  auto keys = [&](int j) { return (lds_u8 *)s_k[(j >> 1) & 3] + 8192 * (j & 1); };
-  auto values = [&](int j) { return (lds_u8 *)s_v[(j >> 1) & 3] + 8192 * (j & 1); };
+  auto turn_ring = [&] {
+    const int s = st;
+    st = st1, st1 = st2, st2 = s;
+  };
+  auto keys = [&](int s) { return (lds_u8 *)s_kv[s][0]; };
+  auto values = [&](int s) { return (lds_u8 *)s_kv[s][1]; };
 
   Rows<kT> w;
   w.init();
@@ -704,35 +706,34 @@ __global__ __launch_bounds__(512) void tile_kernel(Attn a) {
     look(3);
     lds_barrier();
   }
-  if (behind) advance(0);
   // A step of which this wave has nothing leaves zeros: nothing stays live
   // through it.
   auto any = [&](int j) { return p.k0 + 32 * j <= high && p.k0 + 32 * j < p.k1; };
-  auto scores = [&](int j) {
+  auto scores = [&](int j, int st) {
     if (any(j)) {
-      w.scores(ops, keys(j), q, s);
+      w.scores(ops, keys(st), q, s);
     } else {
 #pragma unroll
       for (int t = 0; t < kT; ++t) s[t][0] = s[t][1] = v4f{};
     }
   };
-  scores(0);
+  scores(0, 0);
   // Steps that every row of the workgroup reads in full (and that are not the
   // last): all waves alike, without a condition.
   const int full = max(0, min((p.cached + p.row0 / a.group + 1 - p.k0) / 32, steps - 1));
   int j = 0;
 #pragma unroll 1
   for (; j < full; ++j) {
-    if (!behind && !(j & 1)) advance(j >> 1);
+    advance(j);
     w.weigh(s, c, pr);
-    if (behind && (j & 1)) advance((j + 1) >> 1);
-    w.second(ops, values(j), pr);
-    w.scores(ops, keys(j + 1), q, s);
+    w.second(ops, values(st), pr);
+    w.scores(ops, keys(st1), q, s);
+    turn_ring();
   }
   bool odd = false;
 #pragma unroll 1
   for (;; ++j) {
-    if (!behind && !(j & 1)) advance(j >> 1);
+    advance(j);
     if (any(j)) {
       w.mask(s, p.k0 + 32 * j, limit, lane);
       w.weigh(s, c, pr);
@@ -740,10 +741,10 @@ __global__ __launch_bounds__(512) void tile_kernel(Attn a) {
 #pragma unroll
       for (int t = 0; t < kT; ++t) pr[t] = u32x4{};
     }
-    if (behind && (j & 1) && j + 1 < steps) advance((j + 1) >> 1);
-    if (any(j)) odd |= w.second_masked(ops, values(j), pr);
+    if (any(j)) odd |= w.second_masked(ops, values(st), pr);
     if (j + 1 == steps) break;
-    scores(j + 1);
+    scores(j + 1, st1);
+    turn_ring();
   }
   if (n_rows <= 0) return;
   if (odd)
@@ -886,8 +887,8 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     const int64_t items = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs) + w.tile_parts;
     a.grid = (int)(items < w.tile_items ? items : w.tile_items);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
-    if (fp8) tile_kernel<kPagesFp8><<<grid, 512, 0, as_stream(stream)>>>(a);
-    else tile_kernel<kPages><<<grid, 512, 0, as_stream(stream)>>>(a);
+    if (fp8) tile_kernel<kPagesFp8><<<grid, 256, 0, as_stream(stream)>>>(a);
+    else tile_kernel<kPages><<<grid, 256, 0, as_stream(stream)>>>(a);
     join_kernel<<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 32), 256, 0,
                   as_stream(stream)>>>(
         a, &counts->tile_joins, reinterpret_cast<const Join *>(base + w.tile_joins_at), kTileRows);
@@ -920,7 +921,7 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
   const bool wide_tiles = rows * Hq / kTileRows >= 48;
   a.grid = (int)(rows * a.group / (wide_tiles ? kTileRows : kFewRows) + seqs);
   const unsigned grid = (unsigned)((int64_t)a.grid * Hkv);
-  if (wide_tiles) tile_kernel<kPacked><<<grid, 512, 0, as_stream(stream)>>>(a);
+  if (wide_tiles) tile_kernel<kPacked><<<grid, 256, 0, as_stream(stream)>>>(a);
   else ECF8_FEW(kPacked, 2);
 #undef ECF8_FEW
   return launched();
