@@ -19,6 +19,7 @@ using namespace ecf8::paged;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.0e38f;  // stands for the maximum of no keys
+constexpr float kNone = -1048576.f;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -58,11 +59,11 @@ __device__ __forceinline__ void widen16(u32x4 c, u32x4 (&out)[2]) {
   }
 }
 
-// Keys and values lie in LDS as rows of 16 units of 16 bytes, unit c of row
-// `row` at c ^ turn(row).  The key operand reads one unit of 16 rows, the
-// transposing value read two units of eight rows each half wave: both find
-// all 64 banks.
-__device__ __forceinline__ int turn(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
+// Keys and values lie in LDS as rows of 128 bf16, 272 and 288 bytes apart: the
+// key operand reads 16 bytes of 16 rows, the transposing value read 32 bytes
+// of eight rows each half wave, and both find all 64 banks, at addresses that
+// differ by constants.
+constexpr int kKeyRow = 17, kValueRow = 18;  // in units of 16 bytes
 
 // Orders this wave's LDS accesses (the hardware runs them in order): one
 // lane's writes before another's reads.
@@ -107,31 +108,19 @@ typedef __attribute__((address_space(3))) const uint8_t lds_u8;
 struct Operands {
   uint32_t k, v;
   __device__ __forceinline__ explicit Operands(int lane) {
-    const int i = lane & 15, g = lane >> 4, key = 4 * g + (i >> 2);
-    k = (uint32_t)(i * 256 + ((g ^ turn(i)) << 4));
-    v = (uint32_t)(key * 256 + ((((i & 3) >> 1) ^ turn(key)) << 4) + 8 * (i & 1));
-  }
-  // (the addresses of a step's reads differ in a few bits, which a block's
-  // 256-byte rows leave to an exclusive-or)
-  __device__ __forceinline__ lds_u8 *keys_at(lds_u8 *at) const { return fresh(at + k); }
-  __device__ __forceinline__ lds_u8 *values_at(lds_u8 *at) const { return fresh(at + v); }
-  static __device__ __forceinline__ lds_u8 *fresh(lds_u8 *p) {
-    uint32_t x = (uint32_t)(uintptr_t)p;
-    asm volatile("" : "+v"(x));  // the addresses below are formed anew, not kept in registers
-    return (lds_u8 *)(uintptr_t)x;
-  }
-  static __device__ __forceinline__ lds_u8 *bits(lds_u8 *p, uint32_t x) {
-    return (lds_u8 *)(uintptr_t)((uint32_t)(uintptr_t)p ^ x);
+    const int i = lane & 15, g = lane >> 4;
+    k = (uint32_t)(i * (16 * kKeyRow) + 16 * g);
+    v = (uint32_t)((4 * g + (i >> 2)) * (16 * kValueRow) + 8 * (i & 3));
   }
   static __device__ __forceinline__ v8bf key(lds_u8 *p, int tile, int kk) {
     return *reinterpret_cast<__attribute__((address_space(3))) const v8bf *>(
-        bits(p, (uint32_t)kk << 6) + 4096 * tile);
+        p + 64 * kk + 256 * kKeyRow * tile);
   }
-  static __device__ __forceinline__ u32x4 values(lds_u8 *at, int d) {
-    lds_u8 *p = bits(at, (uint32_t)d << 5);
-    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p));
+  static __device__ __forceinline__ u32x4 values(lds_u8 *p, int d) {
+    const u32x2 a = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 32 * d)));
     const u32x2 b = __builtin_bit_cast(
-        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 4096)));
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 32 * d + 256 * kValueRow)));
     return u32x4{a[0], a[1], b[0], b[1]};
   }
 };
@@ -146,17 +135,18 @@ struct Rows {
   // at once, which would take registers that the other operands live in)
   static constexpr int kAhead = 3;
   v4f o[T][8];
-  // of the lane's query: the whole number that its base-2 exponents are taken
-  // from (the same in all four lanes of a query), and this lane's part of the
-  // sum
-  float m[T], l[T];
+  // of the lane's query (alike in its four lanes): the whole number that its
+  // base-2 exponents are taken from, and the sum of its probabilities, as a
+  // product with ones (four times the same)
+  float m[T];
+  v4f l[T];
 
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int t = 0; t < T; ++t) {
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[t][d] = v4f{0.f, 0.f, 0.f, 0.f};
-      m[t] = l[t] = 0.f;
+      m[t] = 0.f, l[t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
   }
 
@@ -164,7 +154,7 @@ struct Rows {
                                                 const v8bf (&q)[T][4], v4f (&s)[T][2]) {
 #pragma unroll
     for (int t = 0; t < T; ++t) s[t][0] = s[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
-    lds_u8 *p = at.keys_at(k);
+    lds_u8 *p = k + at.k;
     v8bf f[kAhead + 1];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f[i] = at.key(p, i & 1, i >> 1);
@@ -181,10 +171,11 @@ struct Rows {
   }
 
   __device__ __forceinline__ void second(const Operands &at, lds_u8 *v, const u32x4 (&p)[T]) {
-    v = at.values_at(v);
+    v = v + at.v;
     u32x4 f[kAhead + 1];
 #pragma unroll
     for (int d = 0; d < kAhead; ++d) f[d] = at.values(v, d);
+    sum(p);
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
       if (d + kAhead < 8) f[(d + kAhead) % (kAhead + 1)] = at.values(v, d + kAhead);
@@ -197,58 +188,56 @@ struct Rows {
     }
   }
 
-  // Scores -> probabilities: base-2 exponents from m, summed in fp32 and
-  // rounded to bf16 (at most 2^-8 of each, like the output's own rounding): the
-  // second product then runs at the bf16 rate.
-  //
-  // Where a query's largest exponent is above 8, or it has no sum yet, m goes
-  // to its largest exponent first (uniform, rare).  Otherwise m stays: nothing
-  // overflows, and the quotient of the sums is the same.  m is a whole number,
-  // so sums are scaled by powers of two: exactly.
-  __device__ __forceinline__ void weigh(v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
-    float top[T];
-    bool up = false;
+  // Scores -> probabilities, powers of two from m rounded to bf16 (at most 2^-8
+  // of each, like the output's own rounding): the second product then runs at
+  // the bf16 rate.  At first, and where a probability reaches 2 (uniform,
+  // rare), m goes to 6 above the query's largest exponent so far.  Otherwise it
+  // stays: nothing overflows, and the quotient of the sums is the same.  m is a
+  // whole number, so sums are scaled by powers of two: exactly.
+  __device__ __forceinline__ void weigh(const v4f (&s)[T][2], float c, u32x4 (&p)[T], bool first) {
+    powers(s, c, p);
+    uint32_t bits = 0;
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][x][i] = fmaf(s[t][x][i], c, -m[t]);
-      const v4f a = s[t][0], b = s[t][1];
-      top[t] = fmaxf(fmaxf(fmaxf(fmaxf(a[0], a[1]), a[2]), fmaxf(fmaxf(a[3], b[0]), b[1])),
-                     fmaxf(b[2], b[3]));
-      up |= top[t] > 8.f || !(l[t] > 0.f);
-    }
-    if (__any(up)) {
+    for (int t = 0; t < T; ++t) bits |= (p[t][0] | p[t][1]) | (p[t][2] | p[t][3]);
+    if (first || __any((bits & 0x40004000u) != 0)) {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        float b = fmaxf(top[t], __shfl_xor(top[t], 16));
-        b = ceilf(fmaxf(b, __shfl_xor(b, 32)));
-        float sum = l[t] + __shfl_xor(l[t], 16);
-        sum += __shfl_xor(sum, 32);
-        const bool none = sum == 0.f;  // m may also go down
-        const float by = none ? (b > -INFINITY ? b : 0.f) : fmaxf(b, 0.f);
-        const float f = none ? 1.f : __builtin_amdgcn_exp2f(-by);
-        m[t] += by;
+        const v4f a = s[t][0], b = s[t][1];
+        float top = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
+                          fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // (kNone, below any exponent, while there was no score above -inf)
+        float to = fmaxf(ceilf(top * c) + 6.f, kNone);
+        if (!first) to = fmaxf(to, m[t]);
+        const float f = first ? 1.f : __builtin_amdgcn_exp2f(m[t] - to);
+        m[t] = to;
         l[t] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[t][d] *= f;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) s[t][x] -= by;
       }
+      powers(s, c, p);
     }
+  }
+  __device__ __forceinline__ void powers(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
+    for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
+        v4f e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][x][i] = __builtin_amdgcn_exp2f(s[t][x][i]);
-        p[t][2 * x] = pack_bf16(s[t][x][0], s[t][x][1]);
-        p[t][2 * x + 1] = pack_bf16(s[t][x][2], s[t][x][3]);
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[t][x][i], c, -m[t]));
+        p[t][2 * x] = pack_bf16(e[0], e[1]);
+        p[t][2 * x + 1] = pack_bf16(e[2], e[3]);
       }
-      l[t] += ((s[t][0][0] + s[t][0][1]) + (s[t][0][2] + s[t][0][3])) +
-              ((s[t][1][0] + s[t][1][1]) + (s[t][1][2] + s[t][1][3]));
-    }
+  }
+  __device__ __forceinline__ void sum(const u32x4 (&p)[T]) {
+    constexpr uint32_t one = 0x3f803f80u;
+    const v8bf ones = __builtin_bit_cast(v8bf, u32x4{one, one, one, one});
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(v8bf, p[t]), l[t], 0,
+                                                     0, 0);
   }
 
   // The lane's query of group t reads keys up to limit[t] only.
@@ -269,7 +258,8 @@ struct Rows {
   __device__ __forceinline__ bool second_masked(const Operands &at, lds_u8 *v,
                                                 const u32x4 (&p)[T]) {
     uint32_t odd = 0;
-    v = at.values_at(v);
+    v = v + at.v;
+    sum(p);
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
       __builtin_amdgcn_sched_barrier(0);  // few registers
@@ -417,12 +407,12 @@ __device__ __forceinline__ void lds_barrier() {
 // LDS of its own, a round ahead, so the loop has no barrier.
 template <Source kSrc, int T>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
-  __shared__ u32x4 s_kv[4][2][32 * 16];  // a wave's keys and values
+  __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
   __shared__ float s_m[4][16 * T], s_l[4][16 * T];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = (int)blockIdx.x % a.Hkv;
-  u32x4 *s_k = s_kv[wave][0], *s_v = s_kv[wave][1];
+  u32x4 *s_k = s_kv[wave], *s_v = s_kv[wave] + 32 * kKeyRow;
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;      // 16-byte units of a row in memory
   constexpr int kLoads = kUnits / 2;         // per lane and 32 rows
@@ -476,14 +466,14 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       if constexpr (kFp8) {
         u32x4 w[2];
         widen16(kr[i], w);
-        s_k[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_k[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_k[row * kKeyRow + 2 * unit] = w[0];
+        s_k[row * kKeyRow + 2 * unit + 1] = w[1];
         widen16(vr[i], w);
-        s_v[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_v[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_v[row * kValueRow + 2 * unit] = w[0];
+        s_v[row * kValueRow + 2 * unit + 1] = w[1];
       } else {
-        s_k[row * 16 + (unit ^ turn(row))] = kr[i];
-        s_v[row * 16 + (unit ^ turn(row))] = vr[i];
+        s_k[row * kKeyRow + unit] = kr[i];
+        s_v[row * kValueRow + unit] = vr[i];
       }
     }
   };
@@ -510,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       const bool masked = key0 + 31 > low;  // uniform
       w.scores(ops, k, q, s);
       if (masked) w.mask(s, key0, limit, lane);
-      w.weigh(s, c, pr);
+      w.weigh(s, c, pr, key0 == p.k0 + 32 * wave);
       if (masked) odd |= w.second_masked(ops, v, pr);
       else w.second(ops, v, pr);
     }
@@ -525,8 +515,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   float l[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    l[t] = w.l[t] + __shfl_xor(w.l[t], 16);
-    l[t] += __shfl_xor(l[t], 32);
+    l[t] = w.l[t][0];
     if (l[t] == 0.f) w.m[t] = kLowest;
     if (lane < 16) s_m[wave][16 * t + lane] = w.m[t], s_l[wave][16 * t + lane] = l[t];
   }
@@ -589,17 +578,17 @@ static_assert(kTileRows == 4 * 16 * kT, "four waves");
 // and the keys of step j + 1, and write step j + 2.
 template <Source kSrc>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
-  constexpr int kStage = 32 * 16;  // 16-byte units of a stage's keys, or values
-  __shared__ u32x4 s_kv[3][2][kStage];
+  __shared__ u32x4 s_kv[3][32 * (kKeyRow + kValueRow)];  // a step's keys and values
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
   constexpr bool kFp8 = kSrc == kPagesFp8;
-  constexpr int kUnits = kFp8 ? 8 : 16;       // 16-byte units of a row in memory
-  constexpr int kLoads = 32 * kUnits / 256;   // per thread and stage
-  constexpr int kPer = 32 / kLoads;           // rows apart
-  const int unit = threadIdx.x % kUnits, row_of = threadIdx.x / kUnits;
+  // A wave loads 1 KB pieces: kRows rows of a step, kLoads of them for the keys
+  // and as many for the values.
+  constexpr int kUnits = kFp8 ? 8 : 16;      // 16-byte units of a row in memory
+  constexpr int kRows = 64 / kUnits, kLoads = 8 / kRows;
+  const int unit = lane % kUnits, sub = lane / kUnits;
 
   Place p;
   if (!get_item<kSrc>(a, kTileRows, (int)blockIdx.x / a.Hkv, p, lane)) return;
@@ -617,56 +606,74 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
 
   const int steps = (p.k1 - p.k0 + 31) / 32;
   const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
-  int entry[kLoads];  // pages of the rows to be loaded next
+  // the first key of this wave's piece i of step j, in rows of the last one
+  // past the end
+  auto piece = [&](int j, int i) {
+    return min(p.k0 + 32 * j + (32 / kLoads) * i + kRows * wave, (p.k1 - 1) & -kRows);
+  };
+  // Pages of the pieces to be loaded next.  Pages of kRows positions or more
+  // hold whole pieces; in smaller ones a lane looks up its own row.
+  const bool whole = (1 << a.shift) >= kRows;
+  int entry[kLoads];
   auto look = [&](int j) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        entry[i] = table[min(p.k0 + 32 * j + row_of + kPer * i, p.k1 - 1) >> a.shift];
+        entry[i] = table[min(piece(j, i) + sub, p.k1 - 1) >> a.shift];
     }
   };
   u32x4 kr[kLoads], vr[kLoads];
   auto load = [&](int j, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
-    // keys past the last repeat it
-    const int key0 = p.k0 + 32 * min(j, steps - 1);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int key = min(key0 + row_of + kPer * i, p.k1 - 1);
+      // a piece's base is scalar, a lane's offset has 32 bits; rows past the
+      // last repeat it
+      const int key = piece(j, i), row = min(sub, p.k1 - 1 - key);
+      const uint8_t *kb, *vb;
+      uint32_t ko, vo;
       if constexpr (kSrc == kPacked) {
-        // a step's base is scalar, a lane's offset has 32 bits
-        const int64_t at = p.start + key0;
-        const auto *kb = reinterpret_cast<const uint8_t *>(
-            static_cast<const uint16_t *>(a.k) + at * a.k_stride + kvh * kD);
-        const auto *vb = reinterpret_cast<const uint8_t *>(
-            static_cast<const uint16_t *>(a.v) + at * a.v_stride + kvh * kD);
-        const uint32_t row = (uint32_t)(key - key0);
-        kr[i] = *reinterpret_cast<const u32x4 *>(kb + (row * (uint32_t)a.k_stride * 2u + 16u * unit));
-        vr[i] = *reinterpret_cast<const u32x4 *>(vb + (row * (uint32_t)a.v_stride * 2u + 16u * unit));
+        const int64_t at = p.start + key;
+        kb = static_cast<const uint8_t *>(a.k) + 2 * (at * a.k_stride + kvh * kD);
+        vb = static_cast<const uint8_t *>(a.v) + 2 * (at * a.v_stride + kvh * kD);
+        ko = __umul24(row, 2 * (uint32_t)a.k_stride) + 16 * unit;
+        vo = __umul24(row, 2 * (uint32_t)a.v_stride) + 16 * unit;
       } else {
-        const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
-        const size_t at = (((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1))) *
-                              (size_t)kUnits + unit;
-        kr[i] = static_cast<const u32x4 *>(a.k)[at];
-        vr[i] = static_cast<const u32x4 *>(a.v)[at];
+        const uint32_t mask = (1u << a.shift) - 1;
+        if (whole) {
+          const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry[i]), a.pages - 1);
+          const size_t at = (size_t)((((page * a.Hkv + kvh) << a.shift) + (key & mask))) * (16 * kUnits);
+          kb = static_cast<const uint8_t *>(a.k) + at;
+          vb = static_cast<const uint8_t *>(a.v) + at;
+          ko = vo = (uint32_t)row * (16 * kUnits) + 16 * unit;
+        } else {
+          const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
+          const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + ((key + row) & mask)) *
+                            (16 * kUnits);
+          kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.k) + at + 16 * unit);
+          vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.v) + at + 16 * unit);
+          continue;
+        }
       }
+      kr[i] = *reinterpret_cast<const u32x4 *>(kb + ko);
+      vr[i] = *reinterpret_cast<const u32x4 *>(vb + vo);
     }
   };
   auto store = [&](int st, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
-    u32x4 *s_k = s_kv[st][0], *s_v = s_kv[st][1];
+    u32x4 *s_k = s_kv[st], *s_v = s_kv[st] + 32 * kKeyRow;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int row = row_of + kPer * i;
+      const int row = (32 / kLoads) * i + kRows * wave + sub;
       if constexpr (kFp8) {
         u32x4 w[2];
         widen16(kr[i], w);
-        s_k[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_k[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_k[row * kKeyRow + 2 * unit] = w[0];
+        s_k[row * kKeyRow + 2 * unit + 1] = w[1];
         widen16(vr[i], w);
-        s_v[row * 16 + ((2 * unit) ^ turn(row))] = w[0];
-        s_v[row * 16 + ((2 * unit + 1) ^ turn(row))] = w[1];
+        s_v[row * kValueRow + 2 * unit] = w[0];
+        s_v[row * kValueRow + 2 * unit + 1] = w[1];
       } else {
-        s_k[row * 16 + (unit ^ turn(row))] = kr[i];
-        s_v[row * 16 + (unit ^ turn(row))] = vr[i];
+        s_k[row * kKeyRow + unit] = kr[i];
+        s_v[row * kValueRow + unit] = vr[i];
       }
     }
   };
@@ -686,8 +693,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
     const int s = st;
     st = st1, st1 = st2, st2 = s;
   };
-  auto keys = [&](int s) { return (lds_u8 *)s_kv[s][0]; };
-  auto values = [&](int s) { return (lds_u8 *)s_kv[s][1]; };
+  auto keys = [&](int s) { return (lds_u8 *)s_kv[s]; };
+  auto values = [&](int s) { return (lds_u8 *)(s_kv[s] + 32 * kKeyRow); };
 
   Rows<kT> w;
   w.init();
@@ -725,7 +732,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
 #pragma unroll 1
   for (; j < full; ++j) {
     advance(j);
-    w.weigh(s, c, pr);
+    w.weigh(s, c, pr, j == 0);
     w.second(ops, values(st), pr);
     w.scores(ops, keys(st1), q, s);
     turn_ring();
@@ -736,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
     advance(j);
     if (any(j)) {
       w.mask(s, p.k0 + 32 * j, limit, lane);
-      w.weigh(s, c, pr);
+      w.weigh(s, c, pr, j == 0);
     } else {
 #pragma unroll
       for (int t = 0; t < kT; ++t) pr[t] = u32x4{};
@@ -752,8 +759,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
               [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
-    float l = w.l[t] + __shfl_xor(w.l[t], 16);
-    l += __shfl_xor(l, 32);
+    const float l = w.l[t][0];
     const int row = first_row + 16 * t + (lane & 15), g = lane >> 4;
     if (row >= all_rows) continue;
     if (p.part >= 0) {
@@ -904,7 +910,7 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
     return ECF8_ERR_INVALID_ARG;
   const int64_t wide = (int64_t)Hq * kD, kv = (int64_t)Hkv * kD;
   if (!sizes_ok(seqs, rows, Hq, Hkv) || q_stride % 8 || k_stride % 8 || v_stride % 8 ||
-      out_stride % 4 || k_stride > (1 << 24) || v_stride > (1 << 24) ||
+      out_stride % 4 || k_stride > (1 << 22) || v_stride > (1 << 22) ||
       (rows > 1 && (q_stride < wide || out_stride < wide || k_stride < kv ||
                                       v_stride < kv)))
     return ECF8_ERR_UNSUPPORTED;
