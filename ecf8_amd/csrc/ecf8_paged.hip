@@ -194,7 +194,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   int sums[3] = {0, 0, 0};
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    items[i] = (units[i] + per - 1) / per;
+    items[i] = units[i] ? max(1, (2 * units[i] + per) / (2 * per)) : 0;
     parts[i] = items[i] > 1 ? items[i] : 0;
     joins[i] = items[i] > 1;
     sums[0] += items[i], sums[1] += parts[i], sums[2] += joins[i];
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       const int ns = s_start[s + 1] - s_start[s];
       ext = a.cached[s] + min(ns, (row0 + kTileRows - 1) / a.group + 1);
       u = (ext + kTileKeys - 1) / kTileKeys;
-      k = (u + tper - 1) / tper;
+      k = max(1, (2 * u + tper) / (2 * tper));  // rounded: no part far below the others
     }
     int all;
     int p = block_scan(k > 1 ? k : 0, s_waves, all);

@@ -21,10 +21,10 @@ constexpr int kMaxLen = 1 << 24;   // positions of a sequence
 // are split along their keys in kFewKeys steps, the others also into tiles of
 // kTileRows rows with kTileKeys steps.
 constexpr int kFewRows = 32, kFewKeys = 128;
-constexpr int kTileRows = 192, kTileKeys = 64;
+constexpr int kTileRows = 384, kTileKeys = 64;
 constexpr int kTileMinSteps = 4;  // a part of a tile is at least this long
 // workgroups that a split aims at, over all KV heads
-constexpr int kFewSlots = 512, kTileSlots = 512;
+constexpr int kFewSlots = 512, kTileSlots = 256;
 
 // One workgroup's part of the attention, per KV head.
 struct Item {

@@ -36,7 +36,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// Eight bf16 with their infinities and NaNs replaced by zeros.
+// Eight bf16 with their infinities and NaNs replaced by zeros.  Values of steps
+// with masked positions are staged like this: what a masked position holds
+// must not enter the sums, not even as 0 x inf.
 __device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -44,6 +46,10 @@ __device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
     if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] &= 0xffffu;
   }
   return v;
+}
+
+__device__ __forceinline__ bool differ(u32x4 a, u32x4 b) {
+  return ((a[0] ^ b[0]) | (a[1] ^ b[1]) | (a[2] ^ b[2]) | (a[3] ^ b[3])) != 0;
 }
 
 // 16 e4m3 codes -> bf16, exact.
@@ -133,7 +139,7 @@ template <int T>
 struct Rows {
   // operands are read from LDS this many ahead of their products (and not all
   // at once, which would take registers that the other operands live in)
-  static constexpr int kAhead = 3;
+  static constexpr int kAhead = 2;
   v4f o[T][8];
   // of the lane's query (alike in its four lanes): the whole number that its
   // base-2 exponents are taken from, and the sum of its probabilities, as a
@@ -199,25 +205,26 @@ struct Rows {
     uint32_t bits = 0;
 #pragma unroll
     for (int t = 0; t < T; ++t) bits |= (p[t][0] | p[t][1]) | (p[t][2] | p[t][3]);
-    if (first || __any((bits & 0x40004000u) != 0)) {
+    if (first || __any((bits & 0x40004000u) != 0)) raise(s, c, p, first);
+  }
+  __device__ __forceinline__ void raise(const v4f (&s)[T][2], float c, u32x4 (&p)[T], bool first) {
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const v4f a = s[t][0], b = s[t][1];
-        float top = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
-                          fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // (kNone, below any exponent, while there was no score above -inf)
-        float to = fmaxf(ceilf(top * c) + 6.f, kNone);
-        if (!first) to = fmaxf(to, m[t]);
-        const float f = first ? 1.f : __builtin_amdgcn_exp2f(m[t] - to);
-        m[t] = to;
-        l[t] *= f;
+    for (int t = 0; t < T; ++t) {
+      const v4f a = s[t][0], b = s[t][1];
+      float top = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
+                        fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // (kNone, below any exponent, while there was no score above -inf)
+      float to = fmaxf(ceilf(top * c) + 6.f, kNone);
+      if (!first) to = fmaxf(to, m[t]);
+      const float f = first ? 1.f : __builtin_amdgcn_exp2f(m[t] - to);
+      m[t] = to;
+      l[t] *= f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[t][d] *= f;
-      }
-      powers(s, c, p);
+      for (int d = 0; d < 8; ++d) o[t][d] *= f;
     }
+    powers(s, c, p);
   }
   __device__ __forceinline__ void powers(const v4f (&s)[T][2], float c, u32x4 (&p)[T]) {
 #pragma unroll
@@ -240,6 +247,61 @@ struct Rows {
                                                      0, 0);
   }
 
+  // One step j of a run of steps without masked positions, as one stream: the
+  // second product of step j - 1 (its probabilities `was`) with the softmax of
+  // step j between its instructions, then the scores of step j + 1.  A product
+  // takes half of its time from the vector unit, so the two have to be mixed
+  // finely to run beside each other: 3 products, 3 exponents and exponentials at
+  // a time.  Operands are read from LDS kAhead products' operands ahead.
+  // between(i), i < 8: other work beside the scores.
+  static __device__ __forceinline__ u32x4 operand(lds_u8 *v, lds_u8 *k, int i) {
+    if (i < 8) return Operands::values(v, i);
+    return __builtin_bit_cast(u32x4, Operands::key(k, i & 1, (i - 8) >> 1));
+  }
+  template <class Between>
+  __device__ __forceinline__ void stream(lds_u8 *v, lds_u8 *k, u32x4 (&was)[T],
+                                         const v8bf (&q)[T][4], v4f (&s)[T][2], float c,
+                                         Between between) {
+    u32x4 f[kAhead + 1], p[T];
+    float e[T][2];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = operand(v, k, i);
+    __builtin_amdgcn_sched_barrier(0);
+    sum(was);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[(i + kAhead) % (kAhead + 1)] = operand(v, k, i + kAhead);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        e[t][i & 1] = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], c, -m[t]));
+        if (i & 1) p[t][i >> 1] = pack_bf16(e[t][0], e[t][1]);
+      }
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(v8bf, f[i % (kAhead + 1)]), __builtin_bit_cast(v8bf, was[t]),
+            o[t][i], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int t = 0; t < T; ++t) bits |= (p[t][0] | p[t][1]) | (p[t][2] | p[t][3]);
+    if (__any((bits & 0x40004000u) != 0)) raise(s, c, p, false);
+#pragma unroll
+    for (int t = 0; t < T; ++t) was[t] = p[t];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i + kAhead < 8) f[(8 + i + kAhead) % (kAhead + 1)] = operand(v, k, 8 + i + kAhead);
+      between(i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        s[t][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(v8bf, f[(8 + i) % (kAhead + 1)]), q[t][i >> 1],
+            i < 2 ? v4f{0.f, 0.f, 0.f, 0.f} : s[t][i & 1], 0, 0, 0);
+    }
+  }
+
   // The lane's query of group t reads keys up to limit[t] only.
   static __device__ __forceinline__ void mask(v4f (&s)[T][2], int key0, const int (&limit)[T],
                                               int lane) {
@@ -252,33 +314,9 @@ struct Rows {
           if (key0 + 16 * x + 4 * (lane >> 4) + i > limit[t]) s[t][x][i] = -INFINITY;
   }
 
-  // The second product of a step with masked positions: what they hold must
-  // not enter, not even as 0 x inf.  Infinities and NaNs are left out; returns
-  // whether there was one (uniform).
-  __device__ __forceinline__ bool second_masked(const Operands &at, lds_u8 *v,
-                                                const u32x4 (&p)[T]) {
-    uint32_t odd = 0;
-    v = v + at.v;
-    sum(p);
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      __builtin_amdgcn_sched_barrier(0);  // few registers
-      const u32x4 vf = at.values(v, d), f = finite_or_zero(vf);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) odd |= f[j] ^ vf[j];
-      asm volatile("" : "+v"(odd));  // now, not all at the end
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, f),
-                                                          __builtin_bit_cast(v8bf, p[t]), o[t][d],
-                                                          0, 0, 0);
-    }
-    return __any(odd != 0);
-  }
-
-  // Adds the infinities and NaNs that second_masked left out of keys [first,
-  // end): each reaches the queries that read its position.  value(key, dim):
-  // four values of a key from dim on.  Rare.
+  // Adds the infinities and NaNs of keys [first, end), whose values were
+  // staged without them: each reaches the queries that read its position.
+  // value(key, dim): four values of a key from dim on.  Rare.
   template <class Value>
   __device__ __forceinline__ void add_odd(int first, int end, const int (&limit)[T], int lane,
                                           Value value) {
@@ -303,14 +341,19 @@ struct Rows {
 // The queries' operands: group t's rows are row0 + 16 t + lane mod 16, rows
 // from `end` on repeat the last; limit: the last position each reads.
 template <int T>
-__device__ __forceinline__ void load_queries(const Attn &a, int kvh, int start, int cached, int row0,
-                                             int end, int lane, v8bf (&q)[T][4],
+__device__ __forceinline__ void query_limits(const Attn &a, int cached, int row0, int end, int lane,
                                              int (&limit)[T]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+    limit[t] = cached + min(row0 + 16 * t + (lane & 15), end - 1) / a.group;
+}
+template <int T>
+__device__ __forceinline__ void load_queries(const Attn &a, int kvh, int start, int row0, int end,
+                                             int lane, v8bf (&q)[T][4]) {
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int row = min(row0 + 16 * t + (lane & 15), end - 1);
     const int tok = row / a.group, head = kvh * a.group + row % a.group;
-    limit[t] = cached + tok;
     const uint16_t *p = a.q + (int64_t)min(start + tok, a.rows - 1) * a.q_stride + head * kD +
                         8 * (lane >> 4);
 #pragma unroll
@@ -426,7 +469,8 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const int low = p.cached + p.row0 / a.group;  // the first query's limit
   v8bf q[T][4];
   int limit[T];
-  load_queries<T>(a, kvh, p.start, p.cached, p.row0, p.row0 + n_rows, lane, q, limit);
+  load_queries<T>(a, kvh, p.start, p.row0, p.row0 + n_rows, lane, q);
+  query_limits<T>(a, p.cached, p.row0, p.row0 + n_rows, lane, limit);
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
@@ -440,6 +484,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
     return ((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1));
   };
   u32x4 kr[kLoads], vr[kLoads];
+  bool odd = false;
   auto load = [&](uint32_t at) {
     const uint32_t rows[8] = {row_lane<0>(at), row_lane<1>(at), row_lane<2>(at),
                               row_lane<3>(at), row_lane<4>(at), row_lane<5>(at),
@@ -459,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       }
     }
   };
-  auto store = [&]() {
+  auto store = [&](bool masked) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = 8 * (lane >> 4) + (kFp8 ? 2 * i + ((lane >> 3) & 1) : i);
@@ -469,10 +514,20 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
         s_k[row * kKeyRow + 2 * unit] = w[0];
         s_k[row * kKeyRow + 2 * unit + 1] = w[1];
         widen16(vr[i], w);
+        if (masked) {
+          const u32x4 f0 = finite_or_zero(w[0]), f1 = finite_or_zero(w[1]);
+          odd |= differ(f0, w[0]) || differ(f1, w[1]);
+          w[0] = f0, w[1] = f1;
+        }
         s_v[row * kValueRow + 2 * unit] = w[0];
         s_v[row * kValueRow + 2 * unit + 1] = w[1];
       } else {
         s_k[row * kKeyRow + unit] = kr[i];
+        if (masked) {
+          const u32x4 f = finite_or_zero(vr[i]);
+          odd |= differ(f, vr[i]);
+          vr[i] = f;
+        }
         s_v[row * kValueRow + unit] = vr[i];
       }
     }
@@ -481,14 +536,14 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   Rows<T> w;
   w.init();
   int key0 = p.k0 + 32 * wave;
-  bool odd = false;
   if (key0 < p.k1) {  // uniform
     uint32_t at = locate(key0);
     load(at);
     at = locate(key0 + 128);
     for (; key0 < p.k1; key0 += 128) {
+      const bool masked = key0 + 31 > low;  // uniform
       wave_fence();
-      store();
+      store(masked);
       wave_fence();
       if (key0 + 128 < p.k1) {
         load(at);
@@ -497,14 +552,12 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       lds_u8 *k = (lds_u8 *)s_k, *v = (lds_u8 *)s_v;
       v4f s[T][2];
       u32x4 pr[T];
-      const bool masked = key0 + 31 > low;  // uniform
       w.scores(ops, k, q, s);
       if (masked) w.mask(s, key0, limit, lane);
       w.weigh(s, c, pr, key0 == p.k0 + 32 * wave);
-      if (masked) odd |= w.second_masked(ops, v, pr);
-      else w.second(ops, v, pr);
+      w.second(ops, v, pr);
     }
-    if (odd)
+    if (__any(odd))
       for (key0 = p.k0 + 32 * wave; key0 < p.k1; key0 += 128)
         if (key0 + 31 > low)
           w.add_odd(key0, min(key0 + 32, p.k1), limit, lane,
@@ -564,198 +617,211 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
 }
 
 constexpr int kT = 3;  // groups of 16 rows a wave of the tile kernel
-static_assert(kTileRows == 4 * 16 * kT, "four waves");
+constexpr int kTileWaves = kTileRows / (16 * kT);
 
 // Workgroup of four waves, one a SIMD, two workgroups a CU: 192 rows (token,
 // head of the group) of one KV head, 48 a wave, against positions [k0, k1).
 // 48 rows share every operand that a wave reads from LDS: at 32 the reads
 // alone would take as long as the products.
 //
-// A wave's step of 32 keys is its softmax, the second product, and the next
-// step's scores; the other workgroup's wave multiplies meanwhile.  Keys and
-// values go through registers to a ring of three LDS stages, two steps ahead,
-// with one barrier a step: after barrier j the waves read the values of step j
-// and the keys of step j + 1, and write step j + 2.
-template <Source kSrc>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
-  __shared__ u32x4 s_kv[3][32 * (kKeyRow + kValueRow)];  // a step's keys and values
+// A wave's softmax of a step of 32 keys runs beside the second product of the
+// step before (Rows::stream).  Keys and values go through registers to a ring
+// of LDS stages.
+template <Source kSrc, bool kWhole, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(Attn a) {
+  // Stages of a step's keys and values each, and steps a barrier: after a
+  // barrier before step j the waves read steps j - 1 to j + kEvery, and write
+  // j + 2 kEvery to j + 3 kEvery - 1.
+  constexpr int kEvery = kWaves == 8 ? 2 : 1, kRing = 4 * kEvery;
+  __shared__ u32x4 s_kv[kRing][32 * (kKeyRow + kValueRow)];
+  __shared__ int s_odd;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
   constexpr bool kFp8 = kSrc == kPagesFp8;
+  constexpr int kRowsAll = 16 * kT * kWaves;
   // A wave loads 1 KB pieces: kRows rows of a step, kLoads of them for the keys
-  // and as many for the values.
+  // and as many for the values (with eight waves and e4m3, four waves do).
   constexpr int kUnits = kFp8 ? 8 : 16;      // 16-byte units of a row in memory
-  constexpr int kRows = 64 / kUnits, kLoads = 8 / kRows;
+  constexpr int kRows = 64 / kUnits, kPieces = 32 / kRows;
+  constexpr int kLoads = kPieces > kWaves ? kPieces / kWaves : 1;
+  const bool loads = kPieces >= kWaves || wave < kPieces;  // uniform
   const int unit = lane % kUnits, sub = lane / kUnits;
 
   Place p;
-  if (!get_item<kSrc>(a, kTileRows, (int)blockIdx.x / a.Hkv, p, lane)) return;
-  const int all_rows = min(p.n * a.group - p.row0, kTileRows);
+  if (!get_item<kSrc>(a, kRowsAll, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  const int all_rows = min(p.n * a.group - p.row0, kRowsAll);
   if (all_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned lengths
   const int first_row = 16 * kT * wave, n_rows = min(all_rows - first_row, 16 * kT);
-  // the last position that the wave's last row reads
-  const int high = n_rows > 0 ? p.cached + (p.row0 + first_row + n_rows - 1) / a.group : -1;
+  // the last position that all rows of the wave read, and of the workgroup
+  const int low = p.cached + (p.row0 + min(first_row, all_rows - 1)) / a.group;
+  const int low0 = p.cached + p.row0 / a.group;
   v8bf q[kT][4];
-  int limit[kT];
-  load_queries<kT>(a, kvh, p.start, p.cached, p.row0 + first_row, p.row0 + all_rows, lane, q,
-                   limit);
+  load_queries<kT>(a, kvh, p.start, p.row0 + first_row, p.row0 + all_rows, lane, q);
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
   const int steps = (p.k1 - p.k0 + 31) / 32;
+  const int full = max(0, (low0 + 1 - p.k0) / 32);  // the steps that all rows read in full
   const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
   // the first key of this wave's piece i of step j, in rows of the last one
   // past the end
   auto piece = [&](int j, int i) {
-    return min(p.k0 + 32 * j + (32 / kLoads) * i + kRows * wave, (p.k1 - 1) & -kRows);
+    return min(p.k0 + 32 * j + (32 / kLoads) * i + kRows * (wave % kPieces), (p.k1 - 1) & -kRows);
   };
-  // Pages of the pieces to be loaded next.  Pages of kRows positions or more
-  // hold whole pieces; in smaller ones a lane looks up its own row.
-  const bool whole = (1 << a.shift) >= kRows;
+  // Pages of the pieces to be loaded next.  kWhole: a page has kRows positions
+  // or more, so a piece lies in one; otherwise a lane looks up its own row.
   int entry[kLoads];
   auto look = [&](int j) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        entry[i] = table[min(piece(j, i) + sub, p.k1 - 1) >> a.shift];
+      for (int i = 0; i < kLoads; ++i) {
+        // (a vector load also where the lanes read the same: a scalar one would
+        // make every wait for LDS wait for all of LDS)
+        const int key = min(piece(j, i) + (kWhole ? 0 : sub), p.k1 - 1);
+        uint32_t at = (uint32_t)(key >> a.shift) * 4u;
+        asm volatile("" : "+v"(at));
+        entry[i] = *reinterpret_cast<const int *>(reinterpret_cast<const uint8_t *>(table) + at);
+      }
     }
   };
   u32x4 kr[kLoads], vr[kLoads];
+  auto load_piece = [&](int j, int i, u32x4 &kr, u32x4 &vr) {
+    // a piece's base is scalar, a lane's offset has 32 bits; rows past the
+    // last repeat it
+    const int key = piece(j, i), row = min(sub, p.k1 - 1 - key);
+    const uint8_t *kb, *vb;
+    uint32_t ko, vo;
+    if constexpr (kSrc == kPacked) {
+      const int64_t at = p.start + key;
+      kb = static_cast<const uint8_t *>(a.k) + 2 * (at * a.k_stride + kvh * kD);
+      vb = static_cast<const uint8_t *>(a.v) + 2 * (at * a.v_stride + kvh * kD);
+      ko = __umul24(row, 2 * (uint32_t)a.k_stride) + 16 * unit;
+      vo = __umul24(row, 2 * (uint32_t)a.v_stride) + 16 * unit;
+    } else {
+      const uint32_t mask = (1u << a.shift) - 1;
+      if constexpr (kWhole) {
+        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry[i]), a.pages - 1);
+        const size_t at = (size_t)((((page * a.Hkv + kvh) << a.shift) + (key & mask))) * (16 * kUnits);
+        kb = static_cast<const uint8_t *>(a.k) + at;
+        vb = static_cast<const uint8_t *>(a.v) + at;
+        ko = vo = (uint32_t)row * (16 * kUnits) + 16 * unit;
+      } else {
+        const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
+        const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + ((key + row) & mask)) *
+                          (16 * kUnits);
+        kr = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.k) + at + 16 * unit);
+        vr = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.v) + at + 16 * unit);
+        return;
+      }
+    }
+    kr = *reinterpret_cast<const u32x4 *>(kb + ko);
+    vr = *reinterpret_cast<const u32x4 *>(vb + vo);
+  };
+  // piece i of step j to its stage
+  auto store_piece = [&](int j, int i, u32x4 kr, u32x4 vr) {
+    if (!loads) return;
+    u32x4 *s_k = s_kv[j % kRing], *s_v = s_kv[j % kRing] + 32 * kKeyRow;
+    const int row = (32 / kLoads) * i + kRows * wave + sub;
+    if constexpr (kFp8) {
+      u32x4 w[2];
+      widen16(kr, w);
+      s_k[row * kKeyRow + 2 * unit] = w[0];
+      s_k[row * kKeyRow + 2 * unit + 1] = w[1];
+      widen16(vr, w);
+      if (j >= full) {  // uniform
+        const u32x4 f0 = finite_or_zero(w[0]), f1 = finite_or_zero(w[1]);
+        if (differ(f0, w[0]) || differ(f1, w[1])) s_odd = 1;
+        w[0] = f0, w[1] = f1;
+      }
+      s_v[row * kValueRow + 2 * unit] = w[0];
+      s_v[row * kValueRow + 2 * unit + 1] = w[1];
+    } else {
+      s_k[row * kKeyRow + unit] = kr;
+      if (j >= full) {  // uniform
+        const u32x4 f = finite_or_zero(vr);
+        if (differ(f, vr)) s_odd = 1;
+        vr = f;
+      }
+      s_v[row * kValueRow + unit] = vr;
+    }
+  };
   auto load = [&](int j, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      // a piece's base is scalar, a lane's offset has 32 bits; rows past the
-      // last repeat it
-      const int key = piece(j, i), row = min(sub, p.k1 - 1 - key);
-      const uint8_t *kb, *vb;
-      uint32_t ko, vo;
-      if constexpr (kSrc == kPacked) {
-        const int64_t at = p.start + key;
-        kb = static_cast<const uint8_t *>(a.k) + 2 * (at * a.k_stride + kvh * kD);
-        vb = static_cast<const uint8_t *>(a.v) + 2 * (at * a.v_stride + kvh * kD);
-        ko = __umul24(row, 2 * (uint32_t)a.k_stride) + 16 * unit;
-        vo = __umul24(row, 2 * (uint32_t)a.v_stride) + 16 * unit;
-      } else {
-        const uint32_t mask = (1u << a.shift) - 1;
-        if (whole) {
-          const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry[i]), a.pages - 1);
-          const size_t at = (size_t)((((page * a.Hkv + kvh) << a.shift) + (key & mask))) * (16 * kUnits);
-          kb = static_cast<const uint8_t *>(a.k) + at;
-          vb = static_cast<const uint8_t *>(a.v) + at;
-          ko = vo = (uint32_t)row * (16 * kUnits) + 16 * unit;
-        } else {
-          const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
-          const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + ((key + row) & mask)) *
-                            (16 * kUnits);
-          kr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.k) + at + 16 * unit);
-          vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.v) + at + 16 * unit);
-          continue;
-        }
-      }
-      kr[i] = *reinterpret_cast<const u32x4 *>(kb + ko);
-      vr[i] = *reinterpret_cast<const u32x4 *>(vb + vo);
-    }
+    for (int i = 0; i < kLoads; ++i) load_piece(j, i, kr[i], vr[i]);
   };
-  auto store = [&](int st, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
-    u32x4 *s_k = s_kv[st], *s_v = s_kv[st] + 32 * kKeyRow;
+  auto store = [&](int j, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = (32 / kLoads) * i + kRows * wave + sub;
-      if constexpr (kFp8) {
-        u32x4 w[2];
-        widen16(kr[i], w);
-        s_k[row * kKeyRow + 2 * unit] = w[0];
-        s_k[row * kKeyRow + 2 * unit + 1] = w[1];
-        widen16(vr[i], w);
-        s_v[row * kValueRow + 2 * unit] = w[0];
-        s_v[row * kValueRow + 2 * unit + 1] = w[1];
-      } else {
-        s_k[row * kKeyRow + unit] = kr[i];
-        s_v[row * kValueRow + unit] = vr[i];
-      }
-    }
+    for (int i = 0; i < kLoads; ++i) store_piece(j, i, kr[i], vr[i]);
   };
-  int st = 0, st1 = 1, st2 = 2;  // stages of steps j, j + 1, j + 2
-  // barrier j; then step j + 2 to its stage, step j + 3 on its way
-  auto advance = [&](int j) {
+  auto barrier = [] {
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (j + 2 < steps) {
-      store(st2, kr, vr);
-      load(j + 3, kr, vr);
-      look(j + 4);
-    }
   };
-  auto turn_ring = [&] {
-    const int s = st;
-    st = st1, st1 = st2, st2 = s;
-  };
-  auto keys = [&](int s) { return (lds_u8 *)s_kv[s]; };
-  auto values = [&](int s) { return (lds_u8 *)(s_kv[s] + 32 * kKeyRow); };
+  auto keys = [&](int j) { return (lds_u8 *)s_kv[j % kRing]; };
+  auto values = [&](int j) { return (lds_u8 *)(s_kv[j % kRing] + 32 * kKeyRow); };
 
   Rows<kT> w;
   w.init();
   v4f s[kT][2];
   u32x4 pr[kT];
   {
-    u32x4 k1[kLoads], v1[kLoads];
+    u32x4 k1[2 * kEvery][kLoads], v1[2 * kEvery][kLoads];
+    if (threadIdx.x == 0) s_odd = 0;
     look(0);
-    load(0, kr, vr);
-    look(1);
-    load(1, k1, v1);
-    look(2);
-    store(0, kr, vr);
-    store(1, k1, v1);
-    load(2, kr, vr);
-    look(3);
+#pragma unroll
+    for (int x = 0; x < 2 * kEvery; ++x) {
+      load(x, k1[x], v1[x]);
+      look(x + 1);
+    }
+    __syncthreads();  // s_odd
+#pragma unroll
+    for (int x = 0; x < 2 * kEvery; ++x) store(x, k1[x], v1[x]);
+    load(2 * kEvery, kr, vr);
+    look(2 * kEvery + 1);
     lds_barrier();
   }
-  // A step of which this wave has nothing leaves zeros: nothing stays live
-  // through it.
-  auto any = [&](int j) { return p.k0 + 32 * j <= high && p.k0 + 32 * j < p.k1; };
-  auto scores = [&](int j, int st) {
-    if (any(j)) {
-      w.scores(ops, keys(st), q, s);
-    } else {
-#pragma unroll
-      for (int t = 0; t < kT; ++t) s[t][0] = s[t][1] = v4f{};
+  // (a step past the last is the last again, and never read)
+  auto between = [&](int j, int i) {
+    if (i == 0 || i == 1) {
+      if (i < kLoads) store_piece(j + 2 * kEvery, i, kr[i], vr[i]);
+    } else if (i == 2 || i == 4) {
+      const int x = i == 4;
+      if (x < kLoads) load_piece(j + 2 * kEvery + 1, x, kr[x], vr[x]);
+    } else if (i == 6) {
+      look(j + 2 * kEvery + 2);
     }
   };
-  scores(0, 0);
-  // Steps that every row of the workgroup reads in full (and that are not the
-  // last): all waves alike, without a condition.
-  const int full = max(0, min((p.cached + p.row0 / a.group + 1 - p.k0) / 32, steps - 1));
-  int j = 0;
+  if (n_rows <= 0) {  // uniform: a wave without rows stages its share
 #pragma unroll 1
-  for (; j < full; ++j) {
-    advance(j);
-    w.weigh(s, c, pr, j == 0);
-    w.second(ops, values(st), pr);
-    w.scores(ops, keys(st1), q, s);
-    turn_ring();
-  }
-  bool odd = false;
-#pragma unroll 1
-  for (;; ++j) {
-    advance(j);
-    if (any(j)) {
-      w.mask(s, p.k0 + 32 * j, limit, lane);
-      w.weigh(s, c, pr, j == 0);
-    } else {
+    for (int j = 0; j < steps; ++j) {
+      if (j % kEvery == 0) barrier();
 #pragma unroll
-      for (int t = 0; t < kT; ++t) pr[t] = u32x4{};
+      for (int i = 0; i < 8; ++i) between(j, i);
     }
-    if (any(j)) odd |= w.second_masked(ops, values(st), pr);
-    if (j + 1 == steps) break;
-    scores(j + 1, st1);
-    turn_ring();
+    return;
   }
-  if (n_rows <= 0) return;
-  if (odd)
-    w.add_odd(p.k0 + 32 * full, min(high + 1, p.k1), limit, lane,
+  int limit[kT];
+  query_limits<kT>(a, p.cached, p.row0 + first_row, p.row0 + all_rows, lane, limit);
+  w.scores(ops, keys(0), q, s);
+  barrier();
+  if (p.k0 + 31 > low) w.mask(s, p.k0, limit, lane);
+  w.weigh(s, c, pr, true);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) between(0, i);
+  w.scores(ops, keys(1), q, s);
+#pragma unroll 1
+  for (int j = 1; j < steps; ++j) {
+    if (j % kEvery == 0) barrier();
+    if (p.k0 + 32 * j + 31 > low) w.mask(s, p.k0 + 32 * j, limit, lane);  // uniform
+    w.stream(values(j - 1) + ops.v, keys(j + 1) + ops.k, pr, q, s, c,
+             [&](int i) { between(j, i); });
+  }
+  w.second(ops, values(steps - 1), pr);
+  if (s_odd)  // (written before the last barrier)
+    w.add_odd(p.k0 + 32 * full, p.k1, limit, lane,
               [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
@@ -763,7 +829,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Attn a) {
     const int row = first_row + 16 * t + (lane & 15), g = lane >> 4;
     if (row >= all_rows) continue;
     if (p.part >= 0) {
-      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kTileRows + row;
+      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kRowsAll + row;
       v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
@@ -893,8 +959,14 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     const int64_t items = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs) + w.tile_parts;
     a.grid = (int)(items < w.tile_items ? items : w.tile_items);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
-    if (fp8) tile_kernel<kPagesFp8><<<grid, 256, 0, as_stream(stream)>>>(a);
-    else tile_kernel<kPages><<<grid, 256, 0, as_stream(stream)>>>(a);
+#define ECF8_TILES(S, W, N) tile_kernel<S, W, N><<<grid, 64 * (N), 0, as_stream(stream)>>>(a)
+    if (b->page_size >= 8) {
+      if (fp8) ECF8_TILES(kPagesFp8, true, kTileWaves);
+      else ECF8_TILES(kPages, true, kTileWaves);
+    } else {
+      if (fp8) ECF8_TILES(kPagesFp8, false, kTileWaves);
+      else ECF8_TILES(kPages, false, kTileWaves);
+    }
     join_kernel<<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 32), 256, 0,
                   as_stream(stream)>>>(
         a, &counts->tile_joins, reinterpret_cast<const Join *>(base + w.tile_joins_at), kTileRows);
@@ -927,8 +999,9 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
   const bool wide_tiles = rows * Hq / kTileRows >= 48;
   a.grid = (int)(rows * a.group / (wide_tiles ? kTileRows : kFewRows) + seqs);
   const unsigned grid = (unsigned)((int64_t)a.grid * Hkv);
-  if (wide_tiles) tile_kernel<kPacked><<<grid, 256, 0, as_stream(stream)>>>(a);
+  if (wide_tiles) ECF8_TILES(kPacked, true, kTileWaves);
   else ECF8_FEW(kPacked, 2);
 #undef ECF8_FEW
+#undef ECF8_TILES
   return launched();
 }
