@@ -24,7 +24,7 @@ constexpr int kFewRows = 32, kFewKeys = 128;
 constexpr int kTileRows = 384, kTileKeys = 64;
 constexpr int kTileMinSteps = 4;  // a part of a tile is at least this long
 // workgroups that a split aims at, over all KV heads
-constexpr int kFewSlots = 512, kTileSlots = 256;
+constexpr int kFewSlots = 2048, kTileSlots = 256;
 
 // One workgroup's part of the attention, per KV head.
 struct Item {
