@@ -30,11 +30,12 @@ struct Plan {
   Item *few, *tiles;
   Join *few_joins, *tile_joins;
   int seqs, rows, pages, shift, width, group;  // page size 1 << shift
-  int few_target, tile_target, tile_parts, fill_rows;
+  int few_target, tile_target, fill_rows;
 };
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPer = kMaxSeqs / kPlanThreads;  // most sequences per thread
+constexpr int kBuckets = 64;  // lengths that the order of tiles tells apart
 
 // The i-th sequence of this thread: seqs / kPlanThreads consecutive ones
 // each, rounded up; -1 past its last.
@@ -44,31 +45,36 @@ __device__ __forceinline__ int seq_of(int i, int seqs) {
   return i < step && s < seqs ? s : -1;
 }
 
-// The exclusive prefix sums of v over the workgroup, and the total.
-__device__ __forceinline__ int block_scan(int v, int *waves, int &total) {
+// The exclusive prefix sums of N values over the workgroup, and their totals.
+// Calls in a row alternate between the two halves of `waves`.
+constexpr int kPlanWaves = kPlanThreads / 64;
+template <int N>
+__device__ __forceinline__ void block_scan(const int (&v)[N], int (*waves)[kPlanWaves],
+                                           int (&before)[N], int (&total)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int inc = ecf8::dev::wave_inclusive_scan(v);
-  __syncthreads();  // waves may still be read from the last scan
-  if (lane == 63) waves[wave] = inc;
-  __syncthreads();
-  int before = 0, all = 0;
+  int inc[N];
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    const int t = waves[w];
-    if (w < wave) before += t;
-    all += t;
+  for (int x = 0; x < N; ++x) {
+    inc[x] = ecf8::dev::wave_inclusive_scan(v[x]);
+    if (lane == 63) waves[x][wave] = inc[x];
   }
-  total = all;
-  return before + inc - v;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    before[x] = inc[x] - v[x], total[x] = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int t = waves[x][w];
+      if (w < wave) before[x] += t;
+      total[x] += t;
+    }
+  }
 }
 
-// Exclusive prefix sums of the threads' sequences' values, into LDS (and the
-// total at out[seqs]).
-__device__ __forceinline__ int scan_seqs(const int (&v)[kPer], int seqs, int *out, int *waves) {
-  int sum = 0, total;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) sum += v[i];
-  int at = block_scan(sum, waves, total);
+// Writes exclusive prefix sums of the threads' sequences' values, of which
+// `at` come before this thread's.
+__device__ __forceinline__ void put_firsts(const int (&v)[kPer], int at, int total, int seqs,
+                                           int *out) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int s = seq_of(i, seqs);
@@ -76,8 +82,12 @@ __device__ __forceinline__ int scan_seqs(const int (&v)[kPer], int seqs, int *ou
     at += v[i];
   }
   if (threadIdx.x == 0) out[seqs] = total;
-  __syncthreads();
-  return total;
+}
+__device__ __forceinline__ int sum_of(const int (&v)[kPer]) {
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += v[i];
+  return sum;
 }
 
 // The last s < seqs with first[s] <= i: the sequence that element i of a
@@ -104,17 +114,18 @@ __device__ __forceinline__ void fill_row(const Plan &a, const int *first, int i)
   a.positions[i] = pos;
 }
 
-// One workgroup plans the step: three prefix sums over the sequences (rows,
+// One workgroup plans the step: prefix sums over the sequences (rows,
 // pages to take, pages to give back) say where everything goes, then pages,
 // items and rows are written element by element, each finding its sequence by
 // bisection in LDS.  All of it is latency: ~15 dependent rounds.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   __shared__ int s_start[kMaxSeqs + 1], s_take[kMaxSeqs + 1], s_back[kMaxSeqs + 1];
-  __shared__ int s_waves[kPlanThreads / 64];
-  __shared__ int s_bad;
+  __shared__ int s_waves[2][3][kPlanWaves];  // (of two scans in a row)
+  __shared__ int s_bad, s_bucket[kBuckets];
   const int tid = threadIdx.x, S = a.seqs;
   const int page = 1 << a.shift;
   if (tid == 0) s_bad = 0;
+  if (tid < kBuckets) s_bucket[tid] = 0;
   __syncthreads();
   const int n_free = a.n_free[0];
   int c[kPer], n[kPer], own[kPer], take[kPer], back[kPer];
@@ -134,9 +145,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
     take[i] = max(0, ((c[i] + n[i] + page - 1) >> a.shift) - own[i]);
   }
   if (bad) s_bad = 1;
-  const int rows = scan_seqs(n, S, s_start, s_waves);
-  const int taken = scan_seqs(take, S, s_take, s_waves);
-  const int given = scan_seqs(back, S, s_back, s_waves);
+  const int sums[3] = {sum_of(n), sum_of(take), sum_of(back)};
+  int at0[3], all0[3];
+  block_scan(sums, s_waves[0], at0, all0);
+  const int rows = all0[0], taken = all0[1], given = all0[2];
+  put_firsts(n, at0[0], rows, S, s_start);
+  put_firsts(take, at0[1], taken, S, s_take);
+  put_firsts(back, at0[2], given, S, s_back);
+  __syncthreads();
   if (s_bad || rows > a.rows || taken > n_free + given || given > a.pages - n_free) {
     for (int s = tid; s <= S; s += kPlanThreads) {
       s_start[s] = 0;
@@ -181,27 +197,28 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   // The attention's schedule.  Sequences of few rows: split into parts of
   // `per` steps of kFewKeys keys, so that about few_target parts make up
   // the whole.
-  int units[kPer], items[kPer], parts[kPer], joins[kPer], total;
-  int sum = 0;
+  int units[kPer], items[kPer], parts[kPer], joins[kPer], tiles[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const bool few = n[i] > 0 && n[i] * a.group <= kFewRows;
-    units[i] = few ? (c[i] + n[i] + kFewKeys - 1) / kFewKeys : 0;
-    sum += units[i];
+    const int r = n[i] * a.group;
+    units[i] = r > 0 && r <= kFewRows ? (c[i] + n[i] + kFewKeys - 1) / kFewKeys : 0;
+    tiles[i] = r > kFewRows ? (r + kTileRows - 1) / kTileRows : 0;
   }
-  block_scan(sum, s_waves, total);
-  const int per = max(1, (total + a.few_target - 1) / a.few_target);
-  int sums[3] = {0, 0, 0};
+  const int sums1[2] = {sum_of(units), sum_of(tiles)};
+  int at1[2], all1[2];
+  block_scan(sums1, s_waves[1], at1, all1);
+  const int per = max(1, (all1[0] + a.few_target - 1) / a.few_target), n_tiles = all1[1];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     items[i] = units[i] ? max(1, (2 * units[i] + per) / (2 * per)) : 0;
     parts[i] = items[i] > 1 ? items[i] : 0;
     joins[i] = items[i] > 1;
-    sums[0] += items[i], sums[1] += parts[i], sums[2] += joins[i];
   }
-  int n_items, n_parts, n_joins;
-  int at = block_scan(sums[0], s_waves, n_items), part = block_scan(sums[1], s_waves, n_parts),
-      join = block_scan(sums[2], s_waves, n_joins);
+  const int sums2[3] = {sum_of(items), sum_of(parts), sum_of(joins)};
+  int at2[3], all2[3];
+  block_scan(sums2, s_waves[0], at2, all2);
+  int at = at2[0], part = at2[1], join = at2[2];
+  const int n_items = all2[0], n_joins = all2[2];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int s = seq_of(i, S);
@@ -215,47 +232,84 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
     if (joins[i]) a.few_joins[join] = Join{s, 0, part, parts[i]};
     at += items[i], part += parts[i], join += joins[i];
   }
-  // Tiles of the others.  The target's estimate takes a tile's keys as those
-  // of the middle of its sequence.
-  int tiles[kPer];
-  sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const bool many = n[i] * a.group > kFewRows;
-    tiles[i] = many ? (n[i] * a.group + kTileRows - 1) / kTileRows : 0;
-    const int mid = (c[i] + (n[i] + 1) / 2 + kTileKeys - 1) / kTileKeys;
-    sum += (int)min((int64_t)tiles[i] * mid, (int64_t)(1 << 18));
-  }
-  block_scan(sum, s_waves, total);
-  const int n_tiles = scan_seqs(tiles, S, s_back, s_waves);
-  const int tper = max(kTileMinSteps, (total + a.tile_target - 1) / a.tile_target);
-  int t_items = 0, t_parts = 0, t_joins = 0;
-  for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {  // uniform
-    int k = 0, s = 0, row0 = 0, ext = 0, u = 0;
-    // the last tiles of a sequence, which read the most keys, first
-    const int i = n_tiles - 1 - (i0 + tid);
-    if (i >= 0) {
-      s = find_seq(s_back, S, i);
-      row0 = (i - s_back[s]) * kTileRows;
-      const int ns = s_start[s + 1] - s_start[s];
-      ext = a.cached[s] + min(ns, (row0 + kTileRows - 1) / a.group + 1);
-      u = (ext + kTileKeys - 1) / kTileKeys;
-      k = max(1, (2 * u + tper) / (2 * tper));  // rounded: no part far below the others
+  // Tiles of the others, in units of kTileKeys keys.  A tile of more than half
+  // a workgroup's share is long: the long ones, laid end to end, are cut at
+  // the multiples of the share.  Items are listed from the longest on: that
+  // way a tile's last piece and the next one's first follow each other on a CU,
+  // and short tiles fill up what is left.  (1024 rows over 8700 keys: 135 us,
+  // 254 us in equal parts, of which 33 met 32 CUs.)
+  int t_items = 0, t_joins = 0;
+  if (n_tiles > 0) {  // uniform
+    put_firsts(tiles, at1[1], n_tiles, S, s_back);
+    __syncthreads();
+    struct Tile {
+      int seq, row0, end, units;
+    };
+    auto tile_at = [&](int i) {
+      Tile t{0, 0, 0, 0};
+      if (i >= n_tiles) return t;
+      t.seq = find_seq(s_back, S, i);
+      t.row0 = (i - s_back[t.seq]) * kTileRows;
+      const int ns = s_start[t.seq + 1] - s_start[t.seq];
+      t.end = a.lengths[t.seq] - ns + min(ns, (t.row0 + kTileRows - 1) / a.group + 1);
+      t.units = (t.end + kTileKeys - 1) / kTileKeys;
+      return t;
+    };
+    // (past kPlanThreads tiles, in 256 units, rounded up: the total fits)
+    const int scale = n_tiles > kPlanThreads ? 256 : 1;
+    int mine = 0;
+    for (int i = tid; i < n_tiles; i += kPlanThreads) mine += tile_at(i).units;
+    const int sum_units[1] = {(mine + scale - 1) / scale};
+    int skip[1], all_units[1];
+    block_scan(sum_units, s_waves[1], skip, all_units);
+    // (more units than a tile can have are as good as any)
+    const int64_t exact = ((int64_t)all_units[0] * scale + a.tile_target - 1) / a.tile_target;
+    const int share = (int)min(max(exact, (int64_t)(2 * kTileMinUnits)), (int64_t)1 << 20);
+    auto bucket = [&](int len) {
+      return kBuckets - 1 - min(kBuckets - 1, (int)(48ll * len / share));
+    };
+    // Twice over the tiles: count the items of each length, then write them.
+    for (int write = 0; write < 2; ++write) {
+      int from0 = 0, t_parts = 0;
+      for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {  // uniform
+        const Tile t = tile_at(i0 + tid);
+        const bool is_long = 2 * t.units > share;
+        const int units_long[1] = {is_long ? t.units : 0};
+        int from[1], all_long[1];
+        block_scan(units_long, s_waves[0], from, all_long);
+        from[0] += from0;
+        // cuts that leave kTileMinUnits on both sides
+        const int c0 = (from[0] + kTileMinUnits + share - 1) / share;
+        const int c1 = (from[0] + t.units - kTileMinUnits) / share;
+        const int k = t.units ? (is_long ? max(0, c1 - c0 + 1) : 0) + 1 : 0;
+        const int cut[2] = {k > 1 ? k : 0, k > 1};
+        int p[2], all_cut[2];
+        block_scan(cut, s_waves[1], p, all_cut);
+        p[0] += t_parts, p[1] += t_joins;
+        for (int j = 0; j < k; ++j) {
+          const int u0 = j ? (c0 + j - 1) * share - from[0] : 0;
+          const int u1 = j + 1 < k ? (c0 + j) * share - from[0] : t.units;
+          const int at = atomicAdd(&s_bucket[bucket(u1 - u0)], 1);
+          if (write)
+            a.tiles[at] = Item{t.seq, t.row0, u0 * kTileKeys, min(u1 * kTileKeys, t.end),
+                               k > 1 ? p[0] + j : -1, {0, 0, 0}};
+        }
+        if (write) {
+          if (k > 1) a.tile_joins[p[1]] = Join{t.seq, t.row0, p[0], k};
+          t_parts += all_cut[0], t_joins += all_cut[1];
+        }
+        from0 += all_long[0];
+      }
+      __syncthreads();
+      if (!write) {
+        const int count[1] = {tid < kBuckets ? s_bucket[tid] : 0};
+        int first[1], all[1];
+        block_scan(count, s_waves[0], first, all);
+        if (tid < kBuckets) s_bucket[tid] = first[0];
+        t_items = all[0];
+        __syncthreads();
+      }
     }
-    int all;
-    int p = block_scan(k > 1 ? k : 0, s_waves, all);
-    const bool room = t_parts + p + k <= a.tile_parts;
-    if (!room) k = k > 0;  // beyond the estimate: unsplit
-    int n_p, n_i, n_j;
-    p = t_parts + block_scan(k > 1 ? k : 0, s_waves, n_p);
-    const int q = t_items + block_scan(k, s_waves, n_i), jn = t_joins + block_scan(k > 1, s_waves, n_j);
-    for (int j = 0; j < k; ++j) {
-      const int k0 = (int)((int64_t)u * j / k) * kTileKeys;
-      const int k1 = (int)((int64_t)u * (j + 1) / k) * kTileKeys;
-      a.tiles[q + j] = Item{s, row0, k0, min(k1, ext), k > 1 ? p + j : -1, {0, 0, 0}};
-    }
-    if (k > 1) a.tile_joins[jn] = Join{s, row0, p, k};
-    t_items += n_i, t_parts += n_p, t_joins += n_j;
   }
   if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins};
   if (a.fill_rows) {
@@ -424,7 +478,7 @@ extern "C" int ecf8_paged_plan(const ecf8_paged_batch *b, const int *cached,
                reinterpret_cast<Join *>(base + w.few_joins_at),
                reinterpret_cast<Join *>(base + w.tile_joins_at), b->seqs, b->rows, b->pages,
                __builtin_ctz((unsigned)b->page_size), b->width, b->Hq / b->Hkv, w.few_parts / 2,
-               w.tile_parts / 2, w.tile_parts, one};
+               w.tile_parts / 2, one};
   plan_kernel<<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
   if (!one)
     fill_kernel<<<(unsigned)((b->rows + kFillThreads - 1) / kFillThreads), kFillThreads, 0,

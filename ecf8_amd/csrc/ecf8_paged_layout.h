@@ -18,11 +18,11 @@ constexpr int kMaxLen = 1 << 24;   // positions of a sequence
 
 // A "row" of the attention is a (new token, query head of the group) pair:
 // row t * G + g of a sequence and KV head.  Sequences of up to kFewRows rows
-// are split along their keys in kFewKeys steps, the others also into tiles of
-// kTileRows rows with kTileKeys steps.
+// are split along their keys at multiples of kFewKeys, the others also into
+// tiles of kTileRows rows, split at multiples of kTileKeys.
 constexpr int kFewRows = 32, kFewKeys = 128;
 constexpr int kTileRows = 384, kTileKeys = 64;
-constexpr int kTileMinSteps = 4;  // a part of a tile is at least this long
+constexpr int kTileMinUnits = 4;  // a part of a tile is at least this long
 // workgroups that a split aims at, over all KV heads
 constexpr int kFewSlots = 2048, kTileSlots = 256;
 

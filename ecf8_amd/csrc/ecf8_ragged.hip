@@ -991,7 +991,10 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     a.items = reinterpret_cast<const Item *>(base + w.few_at);
     a.stats = reinterpret_cast<float2 *>(base + w.few_stats);
     a.sums = reinterpret_cast<float *>(base + w.few_sums);
-    a.grid = w.few_parts / 2 + (int)(rows < b->seqs ? rows : b->seqs);
+    // items that the parts' target and the longest sequence allow
+    const int64_t seqs = rows < b->seqs ? rows : b->seqs;
+    const int64_t most = seqs * (((int64_t)b->width * b->page_size + kFewKeys - 1) / kFewKeys);
+    a.grid = (int)(w.few_parts / 2 + seqs < most ? w.few_parts / 2 + seqs : most);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
 #define ECF8_FEW(S, T) few_kernel<S, T><<<grid, 256, 0, as_stream(stream)>>>(a)
     if (max_new * G <= 16) {
@@ -1001,10 +1004,13 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
       if (fp8) ECF8_FEW(kPagesFp8, 2);
       else ECF8_FEW(kPages, 2);
     }
-    const unsigned most_rows = (unsigned)(max_new * G < kFewRows ? max_new * G : kFewRows);
-    join_kernel<4><<<dim3((unsigned)(w.few_parts / 2 * a.Hkv), most_rows), 256, 0,
-                     as_stream(stream)>>>(
-        a, &counts->few_joins, reinterpret_cast<const Join *>(base + w.few_joins_at), kFewRows);
+    if (most > seqs) {  // something may be split
+      const int64_t joins = seqs < w.few_parts / 2 ? seqs : w.few_parts / 2;
+      const int64_t most_rows = max_new * G < 8 ? max_new * G : 8;
+      join_kernel<4><<<dim3((unsigned)(joins * a.Hkv), (unsigned)most_rows), 256, 0,
+                       as_stream(stream)>>>(
+          a, &counts->few_joins, reinterpret_cast<const Join *>(base + w.few_joins_at), kFewRows);
+    }
   }
   if (many) {
     a.n_items = &counts->tiles, a.others = nullptr;
