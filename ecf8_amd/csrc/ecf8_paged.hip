@@ -227,9 +227,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       const int k0 = (int)((int64_t)units[i] * j / items[i]) * kFewKeys;
       const int k1 = (int)((int64_t)units[i] * (j + 1) / items[i]) * kFewKeys;
       a.few[at + j] =
-          Item{s, 0, k0, min(k1, c[i] + n[i]), parts[i] ? part + j : -1, {0, 0, 0}};
+          Item{s, 0, k0, min(k1, c[i] + n[i]), parts[i] ? part + j : -1, s_start[s], n[i], c[i]};
     }
-    if (joins[i]) a.few_joins[join] = Join{s, 0, part, parts[i]};
+    if (joins[i]) a.few_joins[join] = Join{0, part, parts[i], s_start[s], n[i], {0, 0, 0}};
     at += items[i], part += parts[i], join += joins[i];
   }
   // Tiles of the others, in units of kTileKeys keys.  A tile of more than half
@@ -243,22 +243,23 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
     put_firsts(tiles, at1[1], n_tiles, S, s_back);
     __syncthreads();
     struct Tile {
-      int seq, row0, end, units;
+      int seq, row0, end, units, n, cached;
     };
     auto tile_at = [&](int i) {
-      Tile t{0, 0, 0, 0};
+      Tile t{};
       if (i >= n_tiles) return t;
       t.seq = find_seq(s_back, S, i);
       t.row0 = (i - s_back[t.seq]) * kTileRows;
-      const int ns = s_start[t.seq + 1] - s_start[t.seq];
-      t.end = a.lengths[t.seq] - ns + min(ns, (t.row0 + kTileRows - 1) / a.group + 1);
+      t.n = s_start[t.seq + 1] - s_start[t.seq];
+      t.cached = a.lengths[t.seq] - t.n;
+      t.end = t.cached + min(t.n, (t.row0 + kTileRows - 1) / a.group + 1);
       t.units = (t.end + kTileKeys - 1) / kTileKeys;
       return t;
     };
     // (past kPlanThreads tiles, in 256 units, rounded up: the total fits)
     const int scale = n_tiles > kPlanThreads ? 256 : 1;
     int mine = 0;
-    for (int i = tid; i < n_tiles; i += kPlanThreads) mine += tile_at(i).units;
+    for (int i = tid; i < n_tiles; i += kPlanThreads) mine += tile_at(i).units + kTileStart;
     const int sum_units[1] = {(mine + scale - 1) / scale};
     int skip[1], all_units[1];
     block_scan(sum_units, s_waves[1], skip, all_units);
@@ -274,10 +275,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {  // uniform
         const Tile t = tile_at(i0 + tid);
         const bool is_long = 2 * t.units > share;
-        const int units_long[1] = {is_long ? t.units : 0};
+        const int units_long[1] = {is_long ? kTileStart + t.units : 0};
         int from[1], all_long[1];
         block_scan(units_long, s_waves[0], from, all_long);
-        from[0] += from0;
+        from[0] += from0 + kTileStart;
         // cuts that leave kTileMinUnits on both sides
         const int c0 = (from[0] + kTileMinUnits + share - 1) / share;
         const int c1 = (from[0] + t.units - kTileMinUnits) / share;
@@ -292,10 +293,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
           const int at = atomicAdd(&s_bucket[bucket(u1 - u0)], 1);
           if (write)
             a.tiles[at] = Item{t.seq, t.row0, u0 * kTileKeys, min(u1 * kTileKeys, t.end),
-                               k > 1 ? p[0] + j : -1, {0, 0, 0}};
+                               k > 1 ? p[0] + j : -1, s_start[t.seq], t.n, t.cached};
         }
         if (write) {
-          if (k > 1) a.tile_joins[p[1]] = Join{t.seq, t.row0, p[0], k};
+          if (k > 1) a.tile_joins[p[1]] = Join{t.row0, p[0], k, s_start[t.seq], t.n, {0, 0, 0}};
           t_parts += all_cut[0], t_joins += all_cut[1];
         }
         from0 += all_long[0];

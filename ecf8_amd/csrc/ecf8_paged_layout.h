@@ -23,6 +23,7 @@ constexpr int kMaxLen = 1 << 24;   // positions of a sequence
 constexpr int kFewRows = 32, kFewKeys = 128;
 constexpr int kTileRows = 384, kTileKeys = 64;
 constexpr int kTileMinUnits = 4;  // a part of a tile is at least this long
+constexpr int kTileStart = 4;     // what a tile costs beside its keys, in the same units
 // workgroups that a split aims at, over all KV heads
 constexpr int kFewSlots = 2048, kTileSlots = 256;
 
@@ -31,11 +32,13 @@ struct Item {
   int seq, row0;  // rows [row0, row0 + kFewRows or kTileRows)
   int k0, k1;     // positions
   int part;       // index of the partial sums, -1: the only part, final
-  int pad[3];
+  int start, n, cached;  // first packed row, new tokens, tokens before them
 };
 // Rows whose parts [part, part + n) are to be joined.
 struct Join {
-  int seq, row0, part, n;
+  int row0, part, n;
+  int start, tokens;  // of the sequence: first packed row, new tokens
+  int pad[3];
 };
 
 struct Counts {

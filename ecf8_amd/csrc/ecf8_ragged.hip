@@ -372,22 +372,26 @@ struct Place {
 // ones whatever the other lengths are.  64 probes a round.
 __device__ __forceinline__ bool find_tile(const Attn &a, int tile_rows, int vt, Place &p,
                                           int lane) {
-  int lo = 0, hi = a.seqs;
-  auto first = [&](int s) {
-    return (int)((int64_t)min(max(a.starts[s], 0), a.rows) * a.group / tile_rows) + s;
+  int lo = 0, hi = a.seqs, here = 0, next = 0;
+  auto first = [&](int start, int s) {
+    return (int)((uint32_t)(start * a.group) / (uint32_t)tile_rows) + s;
   };
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-    const uint64_t below = __ballot(s < hi && first(s) <= vt);
+  for (;;) {
+    const int step = (hi - lo + 63) / 64;
+    const int s = min(lo + lane * step, a.seqs - 1);
+    here = min(max(a.starts[s], 0), a.rows), next = min(a.starts[s + 1], a.rows);
+    const uint64_t below = __ballot(lo + lane * step < hi && first(here, s) <= vt);
     const int k = below ? 63 - __builtin_clzll(below) : 0;
+    here = __builtin_amdgcn_readlane(here, k), next = __builtin_amdgcn_readlane(next, k);
     lo += k * step;
     hi = min(hi, lo + step);
+    if (step == 1) break;
   }
   p.seq = lo;
-  p.start = min(max(a.starts[lo], 0), a.rows);
-  p.n = max(min(a.starts[lo + 1], a.rows) - p.start, 0);
+  p.start = here;
+  p.n = max(next - here, 0);
   p.cached = 0;
-  p.row0 = (vt - first(lo)) * tile_rows;
+  p.row0 = (vt - first(here, lo)) * tile_rows;
   if (p.row0 < 0 || p.row0 >= p.n * a.group) return false;
   p.k0 = 0;
   p.k1 = min(p.n, (p.row0 + tile_rows - 1) / a.group + 1);
@@ -403,15 +407,15 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
     // the longest tiles of a sequence, its last, first
     return item < a.grid && find_tile(a, tile_rows, a.grid - 1 - item, p, lane);
   } else {
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused &&
+    // (the last workgroup, which has no item or a short one)
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused &&
         (a.starts[a.seqs] > a.rows || (a.others && *a.others > 0)))
       *a.refused = 1;
+    const Item it = a.items[item];  // item < a.grid: in the list, filled or not
+    asm volatile("" ::"s"(it.seq), "s"(it.start));  // not after the wait for n_items
     if (item >= *a.n_items) return false;
-    const Item &it = a.items[item];
     p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
-    p.start = a.starts[p.seq];
-    p.n = a.starts[p.seq + 1] - p.start;
-    p.cached = a.lengths[p.seq] - p.n;
+    p.start = it.start, p.n = it.n, p.cached = it.cached;
     return true;
   }
 }
@@ -467,10 +471,6 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const int n_rows = min(p.n * a.group - p.row0, 16 * T);
   if (n_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned step's lengths
   const int low = p.cached + p.row0 / a.group;  // the first query's limit
-  v8bf q[T][4];
-  int limit[T];
-  load_queries<T>(a, kvh, p.start, p.row0, p.row0 + n_rows, lane, q);
-  query_limits<T>(a, p.cached, p.row0, p.row0 + n_rows, lane, limit);
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
@@ -483,6 +483,12 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
     const uint32_t page = min((uint32_t)table[key >> a.shift], a.pages - 1);
     return ((page * a.Hkv + kvh) << a.shift) + (key & ((1 << a.shift) - 1));
   };
+  int key0 = p.k0 + 32 * wave;
+  uint32_t at = locate(key0), next = locate(key0 + 128);
+  v8bf q[T][4];
+  int limit[T];
+  load_queries<T>(a, kvh, p.start, p.row0, p.row0 + n_rows, lane, q);
+  query_limits<T>(a, p.cached, p.row0, p.row0 + n_rows, lane, limit);
   u32x4 kr[kLoads], vr[kLoads];
   bool odd = false;
   auto load = [&](uint32_t at) {
@@ -537,11 +543,9 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
 
   Rows<T> w;
   w.init();
-  int key0 = p.k0 + 32 * wave;
   if (key0 < p.k1) {  // uniform
-    uint32_t at = locate(key0);
     load(at);
-    at = locate(key0 + 128);
+    at = next;
     for (; key0 < p.k1; key0 += 128) {
       const bool masked = key0 + 31 > low;  // uniform
       wave_fence();
@@ -659,8 +663,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   // the last position that all rows of the wave read, and of the workgroup
   const int low = p.cached + (p.row0 + min(first_row, all_rows - 1)) / a.group;
   const int low0 = p.cached + p.row0 / a.group;
-  v8bf q[kT][4];
-  load_queries<kT>(a, kvh, p.start, p.row0 + first_row, p.row0 + all_rows, lane, q);
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
@@ -675,7 +677,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   // Pages of the pieces to be loaded next.  kWhole: a page has kRows positions
   // or more, so a piece lies in one; otherwise a lane looks up its own row.
   int entry[kLoads];
-  auto look = [&](int j) {
+  auto look = [&](int j, int (&entry)[kLoads]) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
@@ -688,8 +690,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
       }
     }
   };
+  int first[2 * kEvery + 1][kLoads];
+#pragma unroll
+  for (int x = 0; x <= 2 * kEvery; ++x) look(x, first[x]);
+  v8bf q[kT][4];
+  load_queries<kT>(a, kvh, p.start, p.row0 + first_row, p.row0 + all_rows, lane, q);
   u32x4 kr[kLoads], vr[kLoads];
-  auto load_piece = [&](int j, int i, u32x4 &kr, u32x4 &vr) {
+  auto load_piece = [&](int j, int i, int entry, u32x4 &kr, u32x4 &vr) {
     // a piece's base is scalar, a lane's offset has 32 bits; rows past the
     // last repeat it
     const int key = piece(j, i), row = min(sub, p.k1 - 1 - key);
@@ -704,13 +711,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
     } else {
       const uint32_t mask = (1u << a.shift) - 1;
       if constexpr (kWhole) {
-        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry[i]), a.pages - 1);
-        const size_t at = (size_t)((((page * a.Hkv + kvh) << a.shift) + (key & mask))) * (16 * kUnits);
+        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry), a.pages - 1);
+        const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + (key & mask)) *
+                          (16 * kUnits);
         kb = static_cast<const uint8_t *>(a.k) + at;
         vb = static_cast<const uint8_t *>(a.v) + at;
         ko = vo = (uint32_t)row * (16 * kUnits) + 16 * unit;
       } else {
-        const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
+        const uint32_t page = min((uint32_t)entry, a.pages - 1);
         const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + ((key + row) & mask)) *
                           (16 * kUnits);
         kr = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.k) + at + 16 * unit);
@@ -751,9 +759,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
       s_v[row * kValueRow + unit] = vr;
     }
   };
-  auto load = [&](int j, u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
+  auto load = [&](int j, const int (&entry)[kLoads], u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_piece(j, i, kr[i], vr[i]);
+    for (int i = 0; i < kLoads; ++i) load_piece(j, i, entry[i], kr[i], vr[i]);
   };
   auto store = [&](int j, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
 #pragma unroll
@@ -774,17 +782,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   {
     u32x4 k1[2 * kEvery][kLoads], v1[2 * kEvery][kLoads];
     if (threadIdx.x == 0) s_odd = 0;
-    look(0);
 #pragma unroll
-    for (int x = 0; x < 2 * kEvery; ++x) {
-      load(x, k1[x], v1[x]);
-      look(x + 1);
-    }
+    for (int x = 0; x < 2 * kEvery; ++x) load(x, first[x], k1[x], v1[x]);
+    load(2 * kEvery, first[2 * kEvery], kr, vr);
+    look(2 * kEvery + 1, entry);
     __syncthreads();  // s_odd
 #pragma unroll
     for (int x = 0; x < 2 * kEvery; ++x) store(x, k1[x], v1[x]);
-    load(2 * kEvery, kr, vr);
-    look(2 * kEvery + 1);
     lds_barrier();
   }
   // (a step past the last is the last again, and never read)
@@ -793,9 +797,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
       if (i < kLoads) store_piece(tail, j + 2 * kEvery, i, kr[i], vr[i]);
     } else if (i == 2 || i == 4) {
       const int x = i == 4;
-      if (x < kLoads) load_piece(j + 2 * kEvery + 1, x, kr[x], vr[x]);
+      if (x < kLoads) load_piece(j + 2 * kEvery + 1, x, entry[x], kr[x], vr[x]);
     } else if (i == 6) {
-      look(j + 2 * kEvery + 2);
+      look(j + 2 * kEvery + 2, entry);
     }
   };
   if (n_rows <= 0) {  // uniform: a wave without rows stages its share
@@ -876,74 +880,77 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   }
 }
 
-// The parts of split rows, joined: two dims a lane, kSplit waves a row (each
-// every kSplit-th part), four parts' loads at a time.
+// The parts of split rows, joined: four dims a lane, kSplit halves of a wave a
+// row (each every kSplit-th part), four parts' loads at a time.  Latency: for
+// 11 tiles in 43 parts, 8 heads (67 MB), 12 us.
 template <int kSplit>
 __global__ __launch_bounds__(256) void join_kernel(Attn a, const int *n_joins, const Join *joins,
                                                    int part_rows) {
-  __shared__ float s_top[4], s_l[4];
-  __shared__ float2 s_sum[4][64];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float s_top[8], s_l[8];
+  __shared__ v4f s_sum[8][32];
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5;
   const int kvh = (int)blockIdx.x % a.Hkv, j = (int)blockIdx.x / a.Hkv;
+  const Join jn = joins[j];  // j: in the list, filled or not
+  asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for n_joins
   if (j >= *n_joins) return;
-  const Join jn = joins[j];
-  const int start = a.starts[jn.seq], n = a.starts[jn.seq + 1] - start;
-  const int n_rows = min(n * a.group - jn.row0, part_rows);
+  const int n_rows = min(jn.tokens * a.group - jn.row0, part_rows);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
-  constexpr int kRows = 4 / kSplit;  // at a time
+  constexpr int kRows = 8 / kSplit;  // at a time
   for (int row0 = kRows * (int)blockIdx.y; row0 < n_rows; row0 += kRows * (int)gridDim.y) {
-    const int row = min(row0 + wave / kSplit, n_rows - 1);
+    const int row = min(row0 + half / kSplit, n_rows - 1);
     const size_t at = ((size_t)jn.part * a.Hkv + kvh) * part_rows + row;
     const size_t step = (size_t)a.Hkv * part_rows;
     // (maxima of parts without a key are below every other's)
-    float top = kLowest, l = 0.f, s0 = 0.f, s1 = 0.f;
-    for (int x0 = wave % kSplit; x0 < jn.n; x0 += 4 * kSplit) {
-      float2 v[4], st[4];
+    float top = kLowest, l = 0.f;
+    v4f sum = {};
+    for (int x0 = half % kSplit; x0 < jn.n; x0 += 4 * kSplit) {
+      v4f v[4];
+      float2 st[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const size_t p = at + min(x0 + u * kSplit, jn.n - 1) * step;
-        v[u] = reinterpret_cast<const float2 *>(a.sums)[p * 64 + lane];
+        v[u] = reinterpret_cast<const v4f *>(a.sums)[p * 32 + lane];
         st[u] = a.stats[p];
-        if (x0 + u * kSplit >= jn.n) st[u] = make_float2(kLowest, 0.f), v[u] = st[u];
       }
       float to = top;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) to = fmaxf(to, st[u].x);
+      for (int u = 0; u < 4; ++u) to = fmaxf(to, st[u].x);  // (past the last: that again)
       const float f0 = __builtin_amdgcn_exp2f(top - to);
-      l *= f0, s0 *= f0, s1 *= f0;
+      l *= f0, sum *= f0;
       top = to;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (x0 + u * kSplit >= jn.n) break;
         const float f = __builtin_amdgcn_exp2f(st[u].x - top);
         l = fmaf(f, st[u].y, l);
-        s0 = fmaf(f, v[u].x, s0);
-        s1 = fmaf(f, v[u].y, s1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = fmaf(f, v[u][i], sum[i]);
       }
     }
     if constexpr (kSplit > 1) {
-      if (lane == 0) s_top[wave] = top, s_l[wave] = l;
-      s_sum[wave][lane] = make_float2(s0, s1);
+      if (lane == 0) s_top[half] = top, s_l[half] = l;
+      s_sum[half][lane] = sum;
       __syncthreads();
-      if (wave == 0) {
-        const float to = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-        l = s0 = s1 = 0.f;
+      if (half == 0) {
+        float to = s_top[0];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 1; x < 8; ++x) to = fmaxf(to, s_top[x]);
+        l = 0.f, sum = v4f{};
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
           const float f = __builtin_amdgcn_exp2f(s_top[x] - to);
           l = fmaf(f, s_l[x], l);
-          s0 = fmaf(f, s_sum[x][lane].x, s0);
-          s1 = fmaf(f, s_sum[x][lane].y, s1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = fmaf(f, s_sum[x][lane][i], sum[i]);
         }
       }
     }
-    const int g = jn.row0 + row, tk = start + g / a.group;
+    const int g = jn.row0 + row, tk = jn.start + g / a.group;
     const float inv = vscale / l;
-    if ((kSplit == 1 ? row0 + wave < n_rows : wave == 0) && tk < a.rows)
-      *reinterpret_cast<uint32_t *>(a.out + (int64_t)tk * a.out_stride +
-                                    (kvh * a.group + g % a.group) * kD + 2 * lane) =
-          pack_bf16(s0 * inv, s1 * inv);
+    if ((kSplit == 1 ? row0 + half < n_rows : half == 0) && tk < a.rows)
+      *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
+                                 (kvh * a.group + g % a.group) * kD + 4 * lane) =
+          u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
     if constexpr (kSplit > 1) __syncthreads();
   }
 }
@@ -1007,7 +1014,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     if (most > seqs) {  // something may be split
       const int64_t joins = seqs < w.few_parts / 2 ? seqs : w.few_parts / 2;
       const int64_t most_rows = max_new * G < 8 ? max_new * G : 8;
-      join_kernel<4><<<dim3((unsigned)(joins * a.Hkv), (unsigned)most_rows), 256, 0,
+      join_kernel<8><<<dim3((unsigned)(joins * a.Hkv), (unsigned)most_rows), 256, 0,
                        as_stream(stream)>>>(
           a, &counts->few_joins, reinterpret_cast<const Join *>(base + w.few_joins_at), kFewRows);
     }
@@ -1028,7 +1035,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
       if (fp8) ECF8_TILES(kPagesFp8, false, kTileWaves);
       else ECF8_TILES(kPages, false, kTileWaves);
     }
-    join_kernel<1><<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 16), 256, 0,
+    join_kernel<1><<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 8), 256, 0,
                      as_stream(stream)>>>(
         a, &counts->tile_joins, reinterpret_cast<const Join *>(base + w.tile_joins_at), kTileRows);
   }
