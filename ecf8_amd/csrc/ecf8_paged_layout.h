@@ -21,11 +21,11 @@ constexpr int kMaxLen = 1 << 24;   // positions of a sequence
 // are split along their keys at multiples of kFewKeys, the others also into
 // tiles of kTileRows rows, split at multiples of kTileKeys.
 constexpr int kFewRows = 32, kFewKeys = 128;
-constexpr int kTileRows = 384, kTileKeys = 64;
+constexpr int kTileRows = 192, kTileKeys = 64;
 constexpr int kTileMinUnits = 4;  // a part of a tile is at least this long
 constexpr int kTileStart = 4;     // what a tile costs beside its keys, in the same units
 // workgroups that a split aims at, over all KV heads
-constexpr int kFewSlots = 2048, kTileSlots = 256;
+constexpr int kFewSlots = 2048, kTileSlots = 512;
 
 // One workgroup's part of the attention, per KV head.
 struct Item {

@@ -11,6 +11,7 @@
 
 #include "ecf8.h"
 #include "ecf8_paged.h"
+#include "ecf8_dev.h"
 #include "ecf8_paged_layout.h"
 
 namespace {
@@ -34,6 +35,14 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const v2bf v = {(__bf16)lo, (__bf16)hi};
   return __builtin_bit_cast(uint32_t, v);
+}
+
+// The maximum of the lanes of the same number mod 16.
+__device__ __forceinline__ float max_of_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // Eight bf16 with their infinities and NaNs replaced by zeros.  Values of steps
@@ -105,6 +114,7 @@ struct Attn {
 enum Source { kPages, kPagesFp8, kPacked };
 
 typedef __attribute__((address_space(3))) const uint8_t lds_u8;
+typedef const __attribute__((address_space(1))) uint8_t global_u8;
 
 // Where a lane finds its operands in 32 keys' rows at an LDS address: the
 // keys' dims 32 kk + 8 (lane / 16) + {0..7} of row 16 tile + lane mod 16, and
@@ -139,7 +149,7 @@ template <int T>
 struct Rows {
   // operands are read from LDS this many ahead of their products (and not all
   // at once, which would take registers that the other operands live in)
-  static constexpr int kAhead = 2;
+  static constexpr int kAhead = 1;
   v4f o[T][8];
   // of the lane's query (alike in its four lanes): the whole number that its
   // base-2 exponents are taken from, and the sum of its probabilities, as a
@@ -213,8 +223,7 @@ struct Rows {
       const v4f a = s[t][0], b = s[t][1];
       float top = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
                         fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = max_of_groups(top);
       // (kNone, below any exponent, while there was no score above -inf)
       float to = fmaxf(ceilf(top * c) + 6.f, kNone);
       if (!first) to = fmaxf(to, m[t]);
@@ -367,11 +376,66 @@ struct Place {
   int start, n, cached;  // first packed row, new tokens, tokens before them
 };
 
-// Sequence and tile of virtual tile `vt` of packed prompts: sequence s has
-// tiles floor(starts[s] G / R) + s on, which is room for its ceil(n G / R)
-// ones whatever the other lengths are.  64 probes a round.
-__device__ __forceinline__ bool find_tile(const Attn &a, int tile_rows, int vt, Place &p,
-                                          int lane) {
+// The item-th tile of packed prompts, the ones that read the most keys first:
+// i-th tiles of all sequences before (i - 1)-th ones.  Up to kSorted sequences:
+// bisection for the level i, of which every lane counts kSorted / 64
+// sequences' tiles.  24 prompts of 8192 rows: 82 us, 104 us in packed order.
+constexpr int kSorted = 128;
+__device__ __forceinline__ bool sorted_tile(const Attn &a, int tile_rows, int item, Place &p,
+                                            int lane) {
+  int here[kSorted / 64], n[kSorted / 64], tiles[kSorted / 64], most = 0;
+#pragma unroll
+  for (int i = 0; i < kSorted / 64; ++i) {
+    const int s = 64 * i + lane;
+    here[i] = n[i] = tiles[i] = 0;
+    if (64 * i >= a.seqs) continue;  // uniform
+    if (s < a.seqs) {
+      here[i] = min(max(a.starts[s], 0), a.rows);
+      n[i] = max(min(a.starts[s + 1], a.rows) - here[i], 0);
+    }
+    tiles[i] = (int)((uint32_t)(n[i] * a.group + tile_rows - 1) / (uint32_t)tile_rows);
+    most = max(most, tiles[i]);
+  }
+  auto above = [&](int level) {  // tiles of this level or a higher one
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSorted / 64; ++i)
+      if (64 * i < a.seqs) sum += max(tiles[i] - level, 0);
+    return __builtin_amdgcn_readlane(ecf8::dev::wave_inclusive_scan(sum), 63);
+  };
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane(most), next = 0;  // next = above(hi)
+  if (item >= above(0)) return false;
+  while (hi - lo > 1) {  // above(lo) > item >= above(hi)
+    const int mid = (lo + hi) >> 1, t = above(mid);
+    if (t > item) lo = mid;
+    else hi = mid, next = t;
+  }
+  int rank = item - next;
+#pragma unroll
+  for (int i = 0; i < kSorted / 64; ++i) {
+    if (64 * i >= a.seqs) continue;
+    const uint64_t has = __ballot(tiles[i] > lo);
+    const int before = __popcll(has & ((1ull << lane) - 1));
+    const uint64_t is = __ballot(tiles[i] > lo && before == rank);
+    if (is) {  // uniform
+      const int k = __builtin_ctzll(is);
+      p.seq = 64 * i + k;
+      p.start = __builtin_amdgcn_readlane(here[i], k), p.n = __builtin_amdgcn_readlane(n[i], k);
+    }
+    rank -= __popcll(has);
+  }
+  p.row0 = lo * tile_rows;
+  return true;
+}
+
+// The same of more sequences, the last in memory first: sequence s has places
+// floor(starts[s] G / R) + s on, which is room for its ceil(n G / R) tiles
+// whatever the other lengths are.  64 probes a round.
+__device__ __forceinline__ bool packed_tile(const Attn &a, int tile_rows, int item, Place &p,
+                                            int lane) {
+  const int vt = a.grid - 1 - item;
   int lo = 0, hi = a.seqs, here = 0, next = 0;
   auto first = [&](int start, int s) {
     return (int)((uint32_t)(start * a.group) / (uint32_t)tile_rows) + s;
@@ -390,9 +454,16 @@ __device__ __forceinline__ bool find_tile(const Attn &a, int tile_rows, int vt, 
   p.seq = lo;
   p.start = here;
   p.n = max(next - here, 0);
-  p.cached = 0;
   p.row0 = (vt - first(here, lo)) * tile_rows;
-  if (p.row0 < 0 || p.row0 >= p.n * a.group) return false;
+  return p.row0 >= 0 && p.row0 < p.n * a.group;
+}
+
+__device__ __forceinline__ bool find_tile(const Attn &a, int tile_rows, int item, Place &p,
+                                          int lane) {
+  if (item >= a.grid || !(a.seqs <= kSorted ? sorted_tile(a, tile_rows, item, p, lane)
+                                            : packed_tile(a, tile_rows, item, p, lane)))
+    return false;
+  p.cached = 0;
   p.k0 = 0;
   p.k1 = min(p.n, (p.row0 + tile_rows - 1) / a.group + 1);
   p.part = -1;
@@ -404,8 +475,7 @@ template <Source kSrc>
 __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item, Place &p,
                                          int lane) {
   if constexpr (kSrc == kPacked) {
-    // the longest tiles of a sequence, its last, first
-    return item < a.grid && find_tile(a, tile_rows, a.grid - 1 - item, p, lane);
+    return find_tile(a, tile_rows, item, p, lane);
   } else {
     // (the last workgroup, which has no item or a short one)
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused &&
@@ -633,12 +703,11 @@ constexpr int kTileWaves = kTileRows / (16 * kT);
 // A wave's softmax of a step of 32 keys runs beside the second product of the
 // step before (Rows::stream).  Keys and values go through registers to a ring
 // of LDS stages.
-template <Source kSrc, bool kWhole, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(Attn a) {
-  // Stages of a step's keys and values each, and steps a barrier: after a
-  // barrier before step j the waves read steps j - 1 to j + kEvery, and write
-  // j + 2 kEvery to j + 3 kEvery - 1.
-  constexpr int kEvery = kWaves == 8 ? 2 : 1, kRing = 4 * kEvery;
+template <Source kSrc, bool kWhole>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
+  // Stages of a step's keys and values each: after the barrier before step j
+  // the waves read steps j - 1 to j + 1 and write j + 2.
+  constexpr int kRing = 4;
   __shared__ u32x4 s_kv[kRing][32 * (kKeyRow + kValueRow)];
   __shared__ int s_odd;
   const int lane = threadIdx.x & 63;
@@ -646,18 +715,16 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
   constexpr bool kFp8 = kSrc == kPagesFp8;
-  constexpr int kRowsAll = 16 * kT * kWaves;
   // A wave loads 1 KB pieces: kRows rows of a step, kLoads of them for the keys
-  // and as many for the values (with eight waves and e4m3, four waves do).
+  // and as many for the values.
   constexpr int kUnits = kFp8 ? 8 : 16;      // 16-byte units of a row in memory
   constexpr int kRows = 64 / kUnits, kPieces = 32 / kRows;
-  constexpr int kLoads = kPieces > kWaves ? kPieces / kWaves : 1;
-  const bool loads = kPieces >= kWaves || wave < kPieces;  // uniform
+  constexpr int kLoads = kPieces / kTileWaves;
   const int unit = lane % kUnits, sub = lane / kUnits;
 
   Place p;
-  if (!get_item<kSrc>(a, kRowsAll, (int)blockIdx.x / a.Hkv, p, lane)) return;
-  const int all_rows = min(p.n * a.group - p.row0, kRowsAll);
+  if (!get_item<kSrc>(a, kTileRows, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  const int all_rows = min(p.n * a.group - p.row0, kTileRows);
   if (all_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned lengths
   const int first_row = 16 * kT * wave, n_rows = min(all_rows - first_row, 16 * kT);
   // the last position that all rows of the wave read, and of the workgroup
@@ -667,39 +734,45 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
   const int steps = (p.k1 - p.k0 + 31) / 32;
-  const int full = max(0, (low0 + 1 - p.k0) / 32);  // the steps that all rows read in full
+  // the steps that all rows read in full
+  const int full = max(0, (min(low0 + 1, p.k1) - p.k0) / 32);
   const int *table = kSrc == kPacked ? nullptr : a.table + (size_t)p.seq * a.width;
-  // the first key of this wave's piece i of step j, in rows of the last one
-  // past the end
-  auto piece = [&](int j, int i) {
-    return min(p.k0 + 32 * j + (32 / kLoads) * i + kRows * (wave % kPieces), (p.k1 - 1) & -kRows);
+  // the first key of this wave's piece i of step j; (kTail: past the end the
+  // last piece, and its last row)
+  auto piece = [&](auto tail, int j, int i) {
+    const int key = p.k0 + 32 * j + (32 / kLoads) * i + kRows * wave;
+    return decltype(tail)::value ? min(key, (p.k1 - 1) & -kRows) : key;
   };
   // Pages of the pieces to be loaded next.  kWhole: a page has kRows positions
-  // or more, so a piece lies in one; otherwise a lane looks up its own row.
-  int entry[kLoads];
-  auto look = [&](int j, int (&entry)[kLoads]) {
+  // or more, so a piece lies in one, and lane i looks up that of piece i;
+  // otherwise a lane looks up its own rows.
+  constexpr int kEntries = kWhole ? 1 : kLoads;
+  int entry[kEntries];
+  auto look = [&](auto tail, int j, int (&entry)[kEntries]) {
     if constexpr (kSrc != kPacked) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        // (a vector load also where the lanes read the same: a scalar one would
-        // make every wait for LDS wait for all of LDS)
-        const int key = min(piece(j, i) + (kWhole ? 0 : sub), p.k1 - 1);
+      for (int i = 0; i < kEntries; ++i) {
+        // (never a scalar load: it would make every wait for LDS wait for all
+        // of LDS)
+        int key = kWhole ? piece(tail, j, 0) : piece(tail, j, i) + sub;
+        if constexpr (kWhole && kLoads > 1) key += (32 / kLoads) * (lane & (kLoads - 1));
+        if (decltype(tail)::value) key = min(key, p.k1 - 1);
         uint32_t at = (uint32_t)(key >> a.shift) * 4u;
         asm volatile("" : "+v"(at));
         entry[i] = *reinterpret_cast<const int *>(reinterpret_cast<const uint8_t *>(table) + at);
       }
     }
   };
-  int first[2 * kEvery + 1][kLoads];
+  int first[3][kEntries];
 #pragma unroll
-  for (int x = 0; x <= 2 * kEvery; ++x) look(x, first[x]);
+  for (int x = 0; x <= 2; ++x) look(std::true_type(), x, first[x]);
   v8bf q[kT][4];
   load_queries<kT>(a, kvh, p.start, p.row0 + first_row, p.row0 + all_rows, lane, q);
   u32x4 kr[kLoads], vr[kLoads];
-  auto load_piece = [&](int j, int i, int entry, u32x4 &kr, u32x4 &vr) {
-    // a piece's base is scalar, a lane's offset has 32 bits; rows past the
-    // last repeat it
-    const int key = piece(j, i), row = min(sub, p.k1 - 1 - key);
+  auto load_piece = [&](auto tail, int j, int i, int entry, u32x4 &kr, u32x4 &vr) {
+    // a piece's base is scalar, a lane's offset has 32 bits
+    const int key = piece(tail, j, i);
+    const int row = decltype(tail)::value ? min(sub, p.k1 - 1 - key) : sub;
     const uint8_t *kb, *vb;
     uint32_t ko, vo;
     if constexpr (kSrc == kPacked) {
@@ -711,7 +784,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
     } else {
       const uint32_t mask = (1u << a.shift) - 1;
       if constexpr (kWhole) {
-        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(entry), a.pages - 1);
+        const uint32_t page = min((uint32_t)__builtin_amdgcn_readlane(entry, i), a.pages - 1);
         const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) + (key & mask)) *
                           (16 * kUnits);
         kb = static_cast<const uint8_t *>(a.k) + at;
@@ -726,14 +799,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
         return;
       }
     }
-    kr = *reinterpret_cast<const u32x4 *>(kb + ko);
-    vr = *reinterpret_cast<const u32x4 *>(vb + vo);
+    global_u8 *kg = (global_u8 *)kb, *vg = (global_u8 *)vb;
+    asm volatile("" : "+s"(kg), "+s"(vg));  // (else 64-bit offsets stay in vector registers)
+    kr = *(const __attribute__((address_space(1))) u32x4 *)(kg + ko);
+    vr = *(const __attribute__((address_space(1))) u32x4 *)(vg + vo);
   };
-  // piece i of step j to its stage
-  // (kTail: it may have masked positions)
+  // piece i of step j to its stage (kTail: it may have masked positions)
   auto store_piece = [&](auto tail, int j, int i, u32x4 kr, u32x4 vr) {
     constexpr bool kTail = decltype(tail)::value;
-    if (!loads) return;
     u32x4 *s_k = s_kv[j % kRing], *s_v = s_kv[j % kRing] + 32 * kKeyRow;
     const int row = (32 / kLoads) * i + kRows * wave + sub;
     if constexpr (kFp8) {
@@ -759,9 +832,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
       s_v[row * kValueRow + unit] = vr;
     }
   };
-  auto load = [&](int j, const int (&entry)[kLoads], u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
+  auto load = [&](int j, const int (&entry)[kEntries], u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_piece(j, i, entry[i], kr[i], vr[i]);
+    for (int i = 0; i < kLoads; ++i) load_piece(std::true_type(), j, i, entry[kWhole ? 0 : i], kr[i], vr[i]);
   };
   auto store = [&](int j, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
 #pragma unroll
@@ -780,32 +853,32 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   v4f s[kT][2];
   u32x4 pr[kT];
   {
-    u32x4 k1[2 * kEvery][kLoads], v1[2 * kEvery][kLoads];
+    u32x4 k1[2][kLoads], v1[2][kLoads];
     if (threadIdx.x == 0) s_odd = 0;
 #pragma unroll
-    for (int x = 0; x < 2 * kEvery; ++x) load(x, first[x], k1[x], v1[x]);
-    load(2 * kEvery, first[2 * kEvery], kr, vr);
-    look(2 * kEvery + 1, entry);
+    for (int x = 0; x < 2; ++x) load(x, first[x], k1[x], v1[x]);
+    load(2, first[2], kr, vr);
+    look(std::true_type(), 3, entry);
     __syncthreads();  // s_odd
 #pragma unroll
-    for (int x = 0; x < 2 * kEvery; ++x) store(x, k1[x], v1[x]);
+    for (int x = 0; x < 2; ++x) store(x, k1[x], v1[x]);
     lds_barrier();
   }
   // (a step past the last is the last again, and never read)
   auto between = [&](auto tail, int j, int i) {
     if (i == 0 || i == 1) {
-      if (i < kLoads) store_piece(tail, j + 2 * kEvery, i, kr[i], vr[i]);
+      if (i < kLoads) store_piece(tail, j + 2, i, kr[i], vr[i]);
     } else if (i == 2 || i == 4) {
       const int x = i == 4;
-      if (x < kLoads) load_piece(j + 2 * kEvery + 1, x, entry[x], kr[x], vr[x]);
+      if (x < kLoads) load_piece(tail, j + 3, x, entry[kWhole ? 0 : x], kr[x], vr[x]);
     } else if (i == 6) {
-      look(j + 2 * kEvery + 2, entry);
+      look(tail, j + 4, entry);
     }
   };
   if (n_rows <= 0) {  // uniform: a wave without rows stages its share
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
-      if (j % kEvery == 0) barrier();
+      barrier();
 #pragma unroll
       for (int i = 0; i < 8; ++i) between(std::true_type(), j, i);
     }
@@ -833,14 +906,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
   w.scores(ops, keys(1), q, s);
   int j = 1;
 #pragma unroll 1
-  for (; j < min(full - 2 * kEvery, steps); ++j) {
-    if (j % kEvery == 0) barrier();
+  for (; j < full - 4; ++j) {
+    barrier();
     w.stream(values(j - 1) + ops.v, keys(j + 1) + ops.k, pr, q, s, c,
              [&](int i) { between(std::false_type(), j, i); });
   }
 #pragma unroll 1
   for (; j < steps; ++j) {
-    if (j % kEvery == 0) barrier();
+    barrier();
     if (p.k0 + 32 * j + 31 > low) mask(j);  // uniform
     w.stream(values(j - 1) + ops.v, keys(j + 1) + ops.k, pr, q, s, c,
              [&](int i) { between(std::true_type(), j, i); });
@@ -859,7 +932,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 8 ? 1 : 2) void tile_kernel(
     const int row = first_row + 16 * t + (late & 15), g = late >> 4;
     if (row >= all_rows) continue;
     if (p.part >= 0) {
-      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kRowsAll + row;
+      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kTileRows + row;
       v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
@@ -1027,13 +1100,13 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     const int64_t items = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs) + w.tile_parts;
     a.grid = (int)(items < w.tile_items ? items : w.tile_items);
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
-#define ECF8_TILES(S, W, N) tile_kernel<S, W, N><<<grid, 64 * (N), 0, as_stream(stream)>>>(a)
+#define ECF8_TILES(S, W) tile_kernel<S, W><<<grid, 64 * kTileWaves, 0, as_stream(stream)>>>(a)
     if (b->page_size >= 8) {
-      if (fp8) ECF8_TILES(kPagesFp8, true, kTileWaves);
-      else ECF8_TILES(kPages, true, kTileWaves);
+      if (fp8) ECF8_TILES(kPagesFp8, true);
+      else ECF8_TILES(kPages, true);
     } else {
-      if (fp8) ECF8_TILES(kPagesFp8, false, kTileWaves);
-      else ECF8_TILES(kPages, false, kTileWaves);
+      if (fp8) ECF8_TILES(kPagesFp8, false);
+      else ECF8_TILES(kPages, false);
     }
     join_kernel<1><<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 8), 256, 0,
                      as_stream(stream)>>>(
@@ -1064,10 +1137,12 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
   a.starts = starts;
   a.Hkv = Hkv, a.group = Hq / Hkv, a.rows = (int)rows, a.seqs = (int)seqs;
   a.scale = kLog2e / sqrtf((float)kD);
-  const bool wide_tiles = rows * Hq / kTileRows >= 48;
-  a.grid = (int)(rows * a.group / (wide_tiles ? kTileRows : kFewRows) + seqs);
+  // Tiles once they make up a workgroup for every CU: 2048 rows of 32 heads take
+  // 68 us in tiles and 79 us in 32 rows a workgroup, 1024 rows 37 and 30 us.
+  const bool tiles = rows * Hq / kTileRows >= kTileSlots / 2;
+  a.grid = (int)(rows * a.group / (tiles ? kTileRows : kFewRows) + seqs);
   const unsigned grid = (unsigned)((int64_t)a.grid * Hkv);
-  if (wide_tiles) ECF8_TILES(kPacked, true, kTileWaves);
+  if (tiles) ECF8_TILES(kPacked, true);
   else ECF8_FEW(kPacked, 2);
 #undef ECF8_FEW
 #undef ECF8_TILES
