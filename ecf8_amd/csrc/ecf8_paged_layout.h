@@ -25,7 +25,7 @@ constexpr int kTileRows = 192, kTileKeys = 64;
 constexpr int kTileMinUnits = 4;  // a part of a tile is at least this long
 constexpr int kTileStart = 4;     // what a tile costs beside its keys, in the same units
 // workgroups that a split aims at, over all KV heads
-constexpr int kFewSlots = 2048, kTileSlots = 512;
+constexpr int kFewSlots = 512, kTileSlots = 512;
 
 // One workgroup's part of the attention, per KV head.
 struct Item {
