@@ -539,6 +539,8 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   Place p;
   if (!get_item<kSrc>(a, 16 * T, (int)blockIdx.x / a.Hkv, p, lane)) return;
   const int n_rows = min(p.n * a.group - p.row0, 16 * T);
+  // (pages: an item is a whole sequence, of more tokens than the call was for)
+  if (kSrc != kPacked && p.n * a.group > 16 * T && threadIdx.x == 0 && a.refused) *a.refused = 1;
   if (n_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned step's lengths
   const int low = p.cached + p.row0 / a.group;  // the first query's limit
   float c = a.scale, vscale = 1.f;

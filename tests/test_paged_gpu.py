@@ -1,9 +1,10 @@
 """GPU numerics of the ragged-batch kernels (include/ecf8_paged.h) against a
 plain model of the page bookkeeping and float64 restatements in torch.
 
-Tolerance of the attention, per output: probabilities are rounded to bf16
-(half a step: at most 2^-8 of each, so at most 2^-8 of A = sum p |v|), the
-output is rounded to bf16 (2^-8 of it).  The rest is fp32: a score's 128
+Tolerance of the attention, per output o: probabilities are rounded to bf16
+by factors 1 + d, |d| <= 2^-8 (half a step), in both sums, so that the quotient
+is off by sum p d (v - o): at most 2^-8 of A = sum p |v| and of |o|.  The output
+is rounded to bf16 (2^-8 of it).  The rest is fp32: a score's 128
 products sum to within 128 * 2^-24 of sum |q k| / sqrt(128), below 64 here:
 2^-11 in the exponent; sums of at most 2^12 terms are within 2^-12, the
 exponential within 2^-20.  Together below 2^-10 of A."""
@@ -267,7 +268,7 @@ def _attention64(q, k, v, first):
 
 
 def _close(got, want, A):
-    bound = (want.abs() + A) * 2.0 ** -8 + A * 2.0 ** -10
+    bound = (2 * want.abs() + A) * 2.0 ** -8 + A * 2.0 ** -10
     return bool(((got.double() - want).abs() <= bound).all())
 
 
@@ -280,7 +281,11 @@ PAGED = [
     ([700, 64, 1], [5, 3, 8], 16, 8, 2, 8), ([40, 2000], [33, 1], 16, 12, 4, None),
     ([0, 0, 0], [1, 129, 70], 64, 6, 3, None), ([513, 0, 9], [257, 1, 0], 32, 8, 1, None),
     ([3000, 1], [70, 300], 128, 32, 8, None), ([0], [1000], 512, 4, 2, None),
-    ([5], [600], 4, 3, 3, 600), ([4000] * 9, [2] * 9, 16, 16, 2, 2)]
+    ([5], [600], 4, 3, 3, 600), ([4000] * 9, [2] * 9, 16, 16, 2, 2),
+    ([60000, 0, 33000], [1, 1, 1], 128, 8, 1, 1),           # many parts
+    ([9000, 200], [200, 2], 16, 12, 2, None),               # tiles in many parts
+    ([0, 100, 0, 31], [48, 47, 49, 96], 64, 4, 1, None),    # tiles of 191 to 193 rows
+    ([3] * 300, [1, 2, 0] * 100, 2, 4, 4, 2)]
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -334,7 +339,10 @@ def test_paged_attention_matches_fp64(cuda_device, cached, new, page, Hq, Hkv, m
 RAGGED = [
     ([1], 4, 1), ([1, 1, 1], 8, 8), ([31, 32, 33], 8, 2), ([0, 5, 0, 64, 0], 4, 4),
     ([127, 1, 128, 129], 16, 4), ([257, 63], 6, 1), ([300, 0, 511], 32, 8), ([1100], 4, 1),
-    ([7] * 70, 12, 4), ([2, 900, 40], 40, 1), ([513], 5, 5)]
+    ([7] * 70, 12, 4), ([2, 900, 40], 40, 1), ([513], 5, 5),
+    # in tiles: 49152 rows and heads on
+    ([1600], 32, 8), ([700, 0, 1100, 3], 32, 8), ([47, 48, 49, 1000], 48, 12), ([130, 33], 320, 2),
+    ([200], 250, 250), ([20] * 140 + [300], 32, 4), ([1] * 600 + [950], 32, 32)]
 
 
 @pytest.mark.parametrize("lens,Hq,Hkv", RAGGED)
@@ -362,22 +370,24 @@ def test_ragged_attention_matches_fp64(cuda_device, lens, Hq, Hkv):
     assert bool((out[:before] == 3.0).all()) and bool((out[N - after:] == 3.0).all())
 
 
-@pytest.mark.parametrize("paged", [False, True])
-def test_attention_of_infinite_and_nan_values(cuda_device, paged):
+@pytest.mark.parametrize("paged,T,Hq", [(False, 150, 4), (True, 150, 4), (False, 150, 384),
+                                        (True, 7, 4)])
+def test_attention_of_infinite_and_nan_values(cuda_device, paged, T, Hq):
     """A value of infinity or NaN reaches the queries at and after its
     position, in its own dimension, and no query before it; a key of NaN
     reaches its later queries, in every dimension."""
     from ecf8_amd.paged_kernels import paged_attention, ragged_attention
 
-    dev, T, Hq, Hkv = cuda_device, 150, 4, 2
+    dev, Hkv = cuda_device, 2
     gen = torch.Generator(device=dev).manual_seed(3)
     q, k, v = (_rand(T, h, D, gen=gen) for h in (Hq, Hkv, Hkv))
     clean, A = _attention64(q, k, v, 0)
     marks = [(5, 3, math.inf), (66, 40, -math.inf), (9, 77, math.nan), (7, 100, math.inf),
-             (68, 100, -math.inf)]
+             (68, 100, -math.inf)] if T > 100 else [(1, 3, math.inf), (2, 5, math.nan)]
     for t, d, x in marks:
         v[t, :, d] = x
-    k[140, :, 0] = math.nan
+    last = T - 10 if T > 100 else T - 2
+    k[last, :, 0] = math.nan
     out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
     if paged:
         b = _batch(dev, [0], [T], 16, Hq, Hkv, 1)
@@ -392,12 +402,12 @@ def test_attention_of_infinite_and_nan_values(cuda_device, paged):
     for t, d, x in marks:
         # the earlier mark of a dimension, added to: inf - inf is NaN
         want[t:, :, d] = want[t:, :, d].where(want[t:, :, d].isinf(), torch.zeros((), dtype=torch.float64, device=dev)) + x
-    want[140:] = math.nan
+    want[last:] = math.nan
     assert torch.equal(out.isnan(), want.isnan())
     inf = want.isinf()
     assert torch.equal(out[inf].double(), want[inf])
     # where the marked values do not reach: the clean result
     fine = want.isfinite()
-    bound = (clean.abs() + A) * 2.0 ** -8 + A * 2.0 ** -10
+    bound = (2 * clean.abs() + A) * 2.0 ** -8 + A * 2.0 ** -10
     assert bool(((out.double() - clean).abs() <= bound)[fine].all())
     assert int(fine.sum()) > T * Hq * D // 2
