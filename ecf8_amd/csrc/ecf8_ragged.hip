@@ -10,8 +10,8 @@
 #include <type_traits>
 
 #include "ecf8.h"
-#include "ecf8_paged.h"
 #include "ecf8_dev.h"
+#include "ecf8_paged.h"
 #include "ecf8_paged_layout.h"
 
 namespace {
@@ -20,7 +20,7 @@ using namespace ecf8::paged;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.0e38f;  // stands for the maximum of no keys
-constexpr float kNone = -1048576.f;
+constexpr float kNone = -0x1p100f;   // and for the exponents' while all scores are -inf
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -39,9 +39,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // The maximum of the lanes of the same number mod 16.
 __device__ __forceinline__ float max_of_groups(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  u = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
@@ -521,7 +523,13 @@ __device__ __forceinline__ void lds_barrier() {
 // Workgroup of four waves: up to 16 T rows (token, head of the group) of one
 // KV head against positions [k0, k1), 128 a round, 32 a wave; the waves' sums
 // are joined in LDS.  A wave stages its keys and values through registers into
-// LDS of its own, a round ahead, so the loop has no barrier.
+// LDS of its own, a round ahead, so the loop has no barrier.  T = 1 where the
+// step's rows allow it: 174 registers instead of 238.
+//
+// Bound by the pages' bytes: 64 sequences of up to 8192 keys, 8 heads (1.11 GB),
+// 168 us, 6.6 TB/s; six of 100000 keys in e4m3, 4 heads (390 MB), 66 us, 5.9
+// TB/s.  Page loads bypass the caches, since a page is read once: 186 and 83 us
+// when they did not, 205 and 97 us.
 template <Source kSrc, int T>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
@@ -704,7 +712,16 @@ constexpr int kTileWaves = kTileRows / (16 * kT);
 //
 // A wave's softmax of a step of 32 keys runs beside the second product of the
 // step before (Rows::stream).  Keys and values go through registers to a ring
-// of LDS stages.
+// of LDS stages.  Steps without masked positions have a loop of their own: with
+// the masks' branches in it a step took 8% longer.
+//
+// Bound by the products (51 MFMA of 16 cycles a wave and step) and the vector
+// instructions beside them (140): 1.25 PFLOP/s in the loop of unmasked steps,
+// where a large library product reaches 1.34.  One prompt of 8192 tokens, 32
+// heads: 485 us, of which the loop takes 440; 24 prompts of 8192 tokens together:
+// 80 us, mostly the first loads and the last steps of ~100 short tiles.  Tiles of
+// 384 rows and eight waves reach the same rate in the loop, but take 505 and 104
+// us: fewer tiles fill the card less evenly.
 template <Source kSrc, bool kWhole>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
   // Stages of a step's keys and values each: after the barrier before step j

@@ -411,3 +411,21 @@ def test_attention_of_infinite_and_nan_values(cuda_device, paged, T, Hq):
     bound = (2 * clean.abs() + A) * 2.0 ** -8 + A * 2.0 ** -10
     assert bool(((out.double() - clean).abs() <= bound)[fine].all())
     assert int(fine.sum()) > T * Hq * D // 2
+
+
+@pytest.mark.parametrize("T,Hq", [(70, 4), (150, 384)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_very_large_scores(cuda_device, T, Hq, sign):
+    """Equal scores of +-1.6e7 (in powers of two): the mean of the values."""
+    from ecf8_amd.paged_kernels import ragged_attention
+
+    dev, Hkv = cuda_device, 2
+    gen = torch.Generator(device=dev).manual_seed(6)
+    q = torch.full((T, Hq, D), 1000.0, dtype=torch.bfloat16, device=dev)
+    k = torch.full((T, Hkv, D), sign * 1000.0, dtype=torch.bfloat16, device=dev)
+    v = _rand(T, Hkv, D, gen=gen)
+    out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
+    ragged_attention(q, k, v, _ints([0, T], dev), out)
+    counts = torch.arange(1, T + 1, device=dev, dtype=torch.float64)[:, None, None]
+    mean, A = ((x.double().cumsum(0) / counts).repeat_interleave(Hq // Hkv, 1) for x in (v, v.abs()))
+    assert _close(out, mean, A)
