@@ -853,7 +853,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
   };
   auto load = [&](int j, const int (&entry)[kEntries], u32x4 (&kr)[kLoads], u32x4 (&vr)[kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_piece(std::true_type(), j, i, entry[kWhole ? 0 : i], kr[i], vr[i]);
+    for (int i = 0; i < kLoads; ++i)
+      load_piece(std::true_type(), j, i, entry[kWhole ? 0 : i], kr[i], vr[i]);
   };
   auto store = [&](int j, const u32x4 (&kr)[kLoads], const u32x4 (&vr)[kLoads]) {
 #pragma unroll
@@ -972,23 +973,33 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
   }
 }
 
+// One class's joins: the plan's list, and the workgroups of a join (over the
+// rows) and of all of them.
+struct Joins {
+  const int *n;
+  const Join *list;
+  const float *sums;
+  const float2 *stats;
+  int rows_groups, groups;
+};
+
 // The parts of split rows, joined: four dims a lane, kSplit halves of a wave a
-// row (each every kSplit-th part), four parts' loads at a time.  Latency: for
-// 11 tiles in 43 parts, 8 heads (67 MB), 12 us.
-template <int kSplit>
-__global__ __launch_bounds__(256) void join_kernel(Attn a, const int *n_joins, const Join *joins,
-                                                   int part_rows) {
+// row (each every kSplit-th part), four parts' loads at a time.
+template <int kSplit, int kPartRows>
+__device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int group) {
   __shared__ float s_top[8], s_l[8];
   __shared__ v4f s_sum[8][32];
   const int lane = threadIdx.x & 31, half = threadIdx.x >> 5;
-  const int kvh = (int)blockIdx.x % a.Hkv, j = (int)blockIdx.x / a.Hkv;
-  const Join jn = joins[j];  // j: in the list, filled or not
-  asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for n_joins
-  if (j >= *n_joins) return;
+  const int y = group % o.rows_groups, kvh = group / o.rows_groups % a.Hkv;
+  const int j = group / o.rows_groups / a.Hkv;
+  const Join jn = o.list[j];  // j: in the list, filled or not
+  asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for the count
+  if (j >= *o.n) return;
+  constexpr int part_rows = kPartRows;
   const int n_rows = min(jn.tokens * a.group - jn.row0, part_rows);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
   constexpr int kRows = 8 / kSplit;  // at a time
-  for (int row0 = kRows * (int)blockIdx.y; row0 < n_rows; row0 += kRows * (int)gridDim.y) {
+  for (int row0 = kRows * y; row0 < n_rows; row0 += kRows * o.rows_groups) {
     const int row = min(row0 + half / kSplit, n_rows - 1);
     const size_t at = ((size_t)jn.part * a.Hkv + kvh) * part_rows + row;
     const size_t step = (size_t)a.Hkv * part_rows;
@@ -1001,8 +1012,8 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, const int *n_joins, c
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const size_t p = at + min(x0 + u * kSplit, jn.n - 1) * step;
-        v[u] = reinterpret_cast<const v4f *>(a.sums)[p * 32 + lane];
-        st[u] = a.stats[p];
+        v[u] = reinterpret_cast<const v4f *>(o.sums)[p * 32 + lane];
+        st[u] = o.stats[p];
       }
       float to = top;
 #pragma unroll
@@ -1047,6 +1058,14 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, const int *n_joins, c
   }
 }
 
+// Both classes in one launch.  Latency: two joins of 85 parts, 3 us; 22 tiles in
+// 86 parts, 8 heads (67 MB), 13 us.
+__global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tiles) {
+  const int i = (int)blockIdx.x;
+  if (i < few.groups) join_parts<8, kFewRows>(a, few, i);
+  else join_parts<1, kTileRows>(a, tiles, i - few.groups);
+}
+
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 inline bool aligned(const void *p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
@@ -1085,6 +1104,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   a.shift = __builtin_ctz((unsigned)b->page_size), a.pages = (uint32_t)b->pages;
   a.scale = kLog2e / sqrtf((float)kD);
   const bool many = max_new * G > kFewRows;
+  Joins few{}, tiles{};
   if (G <= kFewRows) {
     a.n_items = &counts->few, a.others = many ? nullptr : &counts->tiles;
     a.items = reinterpret_cast<const Item *>(base + w.few_at);
@@ -1104,11 +1124,11 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
       else ECF8_FEW(kPages, 2);
     }
     if (most > seqs) {  // something may be split
-      const int64_t joins = seqs < w.few_parts / 2 ? seqs : w.few_parts / 2;
-      const int64_t most_rows = max_new * G < 8 ? max_new * G : 8;
-      join_kernel<8><<<dim3((unsigned)(joins * a.Hkv), (unsigned)most_rows), 256, 0,
-                       as_stream(stream)>>>(
-          a, &counts->few_joins, reinterpret_cast<const Join *>(base + w.few_joins_at), kFewRows);
+      few.rows_groups = (int)(max_new * G < 8 ? max_new * G : 8);
+      few.groups = (int)(seqs < w.few_parts / 2 ? seqs : w.few_parts / 2) * a.Hkv * few.rows_groups;
+      few.n = &counts->few_joins;
+      few.list = reinterpret_cast<const Join *>(base + w.few_joins_at);
+      few.stats = a.stats, few.sums = a.sums;
     }
   }
   if (many) {
@@ -1116,8 +1136,9 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     a.items = reinterpret_cast<const Item *>(base + w.tiles_at);
     a.stats = reinterpret_cast<float2 *>(base + w.tile_stats);
     a.sums = reinterpret_cast<float *>(base + w.tile_sums);
-    const int64_t items = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs) + w.tile_parts;
-    a.grid = (int)(items < w.tile_items ? items : w.tile_items);
+    const int64_t most = rows * G / kTileRows + (rows < b->seqs ? rows : b->seqs);  // tiles
+    const int64_t joins = most < w.tile_parts / 2 ? most : w.tile_parts / 2;
+    a.grid = (int)most + w.tile_parts / 2;  // a cut adds an item
     const unsigned grid = (unsigned)(a.grid * a.Hkv);
 #define ECF8_TILES(S, W) tile_kernel<S, W><<<grid, 64 * kTileWaves, 0, as_stream(stream)>>>(a)
     if (b->page_size >= 8) {
@@ -1127,10 +1148,13 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
       if (fp8) ECF8_TILES(kPagesFp8, false);
       else ECF8_TILES(kPages, false);
     }
-    join_kernel<1><<<dim3((unsigned)(w.tile_parts / 2 * a.Hkv), kTileRows / 8), 256, 0,
-                     as_stream(stream)>>>(
-        a, &counts->tile_joins, reinterpret_cast<const Join *>(base + w.tile_joins_at), kTileRows);
+    tiles.rows_groups = kTileRows / 8, tiles.groups = (int)joins * a.Hkv * tiles.rows_groups;
+    tiles.n = &counts->tile_joins;
+    tiles.list = reinterpret_cast<const Join *>(base + w.tile_joins_at);
+    tiles.stats = a.stats, tiles.sums = a.sums;
   }
+  if (const int groups = few.groups + tiles.groups)
+    join_kernel<<<(unsigned)groups, 256, 0, as_stream(stream)>>>(a, few, tiles);
   return launched();
 }
 
