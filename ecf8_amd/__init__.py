@@ -5,6 +5,8 @@
   ``include/ecf8.h`` and ``include/ecf8_llm.h``;
 * ``decode``, ``llm_kernels``: ctypes wrappers of that ABI with argument
   checks;
+* ``paged_kernels``: sequences of different lengths over a paged KV cache
+  (``include/ecf8_paged.h``);
 * ``llm``, ``moe``, ``dit``, ``prefetch``: the Qwen3-8B-, Qwen3-30B-A3B- and
   FLUX-shaped engines that consume the decoded weights.
 

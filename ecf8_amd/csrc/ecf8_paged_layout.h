@@ -24,7 +24,7 @@ constexpr int kFewRows = 32, kFewKeys = 128;
 constexpr int kTileRows = 192, kTileKeys = 64;
 constexpr int kTileMinUnits = 4;  // a part of a tile is at least this long
 constexpr int kTileStart = 4;     // what a tile costs beside its keys, in the same units
-// workgroups that a split aims at, over all KV heads
+// workgroups that a split aims at, over all KV heads: two a CU
 constexpr int kFewSlots = 512, kTileSlots = 512;
 
 // One workgroup's part of the attention, per KV head.
