@@ -285,7 +285,9 @@ PAGED = [
     ([60000, 0, 33000], [1, 1, 1], 128, 8, 1, 1),           # many parts
     ([9000, 200], [200, 2], 16, 12, 2, None),               # tiles in many parts
     ([0, 100, 0, 31], [48, 47, 49, 96], 64, 4, 1, None),    # tiles of 191 to 193 rows
-    ([3] * 300, [1, 2, 0] * 100, 2, 4, 4, 2)]
+    ([3] * 300, [1, 2, 0] * 100, 2, 4, 4, 2),
+    ([10, 300], [2, 1], 16, 1024, 1, None), ([1024, 1023, 2048], [1, 2, 40], 1024, 6, 2, None),
+    ([700, 40], [1, 60], 16, 300, 300, None), ([5] * 4096, [1] * 4096, 8, 2, 1, 1)]
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -342,7 +344,8 @@ RAGGED = [
     ([7] * 70, 12, 4), ([2, 900, 40], 40, 1), ([513], 5, 5),
     # in tiles: 49152 rows and heads on
     ([1600], 32, 8), ([700, 0, 1100, 3], 32, 8), ([47, 48, 49, 1000], 48, 12), ([130, 33], 320, 2),
-    ([200], 250, 250), ([20] * 140 + [300], 32, 4), ([1] * 600 + [950], 32, 32)]
+    ([200], 250, 250), ([20] * 140 + [300], 32, 4), ([1] * 600 + [950], 32, 32),
+    ([3, 60], 1024, 1), ([70], 1024, 1024)]
 
 
 @pytest.mark.parametrize("lens,Hq,Hkv", RAGGED)
