@@ -146,8 +146,10 @@ struct Operands {
 // T groups of 16 queries (rows) against 32 keys a step.  Scores are computed
 // transposed (S^T = K Q^T, v_mfma_f32_16x16x32_bf16), so a lane holds scores of
 // one query of each group, lane mod 16, and the probabilities are the second
-// product's B operand (O^T += V^T P^T) as they stand.
-template <int T>
+// product's B operand (O^T += V^T P^T) as they stand.  kFine: they enter in two
+// parts of bf16, where the matrix unit has nothing better to do; the error
+// against 64 bits is then the output's rounding, and else 1.4 times that.
+template <int T, bool kFine = false>
 struct Rows {
   // operands are read from LDS this many ahead of their products (and not all
   // at once, which would take registers that the other operands live in)
@@ -158,6 +160,9 @@ struct Rows {
   // product with ones (four times the same)
   float m[T];
   v4f l[T];
+  // kFine: what the last probabilities lost when they were cut off to bf16, in
+  // bf16: a second product adds it, and 2^-15 of them is lost
+  u32x4 low[kFine ? T : 1];
 
   __device__ __forceinline__ void init() {
 #pragma unroll
@@ -199,10 +204,14 @@ struct Rows {
       if (d + kAhead < 8) f[(d + kAhead) % (kAhead + 1)] = at.values(v, d + kAhead);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < T; ++t)
-        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(v8bf, f[d % (kAhead + 1)]), __builtin_bit_cast(v8bf, p[t]), o[t][d],
-            0, 0, 0);
+      for (int t = 0; t < T; ++t) {
+        const v8bf vd = __builtin_bit_cast(v8bf, f[d % (kAhead + 1)]);
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vd, __builtin_bit_cast(v8bf, p[t]),
+                                                          o[t][d], 0, 0, 0);
+        if constexpr (kFine)
+          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vd, __builtin_bit_cast(v8bf, low[t]),
+                                                            o[t][d], 0, 0, 0);
+      }
     }
   }
 
@@ -245,17 +254,35 @@ struct Rows {
         v4f e;
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[t][x][i], c, -m[t]));
-        p[t][2 * x] = pack_bf16(e[0], e[1]);
-        p[t][2 * x + 1] = pack_bf16(e[2], e[3]);
+        if constexpr (kFine) {
+          // cut off, not rounded; the rest is above zero unless all is zero, so
+          // that an infinite value stays what it is
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float e0 = e[2 * h], e1 = e[2 * h + 1];
+            const uint32_t u0 = __float_as_uint(e0), u1 = __float_as_uint(e1) & 0xffff0000u;
+            p[t][2 * x + h] = u1 | u0 >> 16;
+            low[t][2 * x + h] = pack_bf16(
+                fmaf(e0, 0x1p-24f, e0 - __uint_as_float(u0 & 0xffff0000u)),
+                fmaf(e1, 0x1p-24f, e1 - __uint_as_float(u1)));
+          }
+        } else {
+          p[t][2 * x] = pack_bf16(e[0], e[1]);
+          p[t][2 * x + 1] = pack_bf16(e[2], e[3]);
+        }
       }
   }
   __device__ __forceinline__ void sum(const u32x4 (&p)[T]) {
     constexpr uint32_t one = 0x3f803f80u;
     const v8bf ones = __builtin_bit_cast(v8bf, u32x4{one, one, one, one});
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+    for (int t = 0; t < T; ++t) {
       l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(v8bf, p[t]), l[t], 0,
                                                      0, 0);
+      if constexpr (kFine)
+        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(v8bf, low[t]), l[t],
+                                                       0, 0, 0);
+    }
   }
 
   // One step j of a run of steps without masked positions, as one stream: the
@@ -621,7 +648,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
     }
   };
 
-  Rows<T> w;
+  Rows<T, true> w;
   w.init();
   if (key0 < p.k1) {  // uniform
     load(at);
