@@ -555,7 +555,8 @@ __device__ __forceinline__ void lds_barrier() {
 //
 // Bound by the pages' bytes: 64 sequences of up to 8192 keys, 8 heads (1.11 GB),
 // 168 us, 6.6 TB/s; six of 100000 keys in e4m3, 4 heads (390 MB), 66 us, 5.9
-// TB/s.  Page loads bypass the caches, since a page is read once: 186 and 83 us
+// TB/s.  The matrix unit is busy for a tenth of that, so probabilities enter in
+// two parts (kFine) at no cost.  Page loads bypass the caches, since a page is read once: 186 and 83 us
 // when they did not, 205 and 97 us.
 template <Source kSrc, int T>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {

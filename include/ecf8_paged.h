@@ -110,7 +110,9 @@ int ecf8_paged_qk_norm_rope(const void *qkv, int64_t rows, const ecf8_paged_batc
  * t, reads positions [0, cached[s] + t].  q bf16, row i's heads at q + i *
  * q_stride elements; scores scaled by 1/sqrt(128); out bf16, row i's heads at
  * out + i * out_stride.  fp8 != 0: e4m3fn pools with scales as above.  fp32
- * scores, softmax statistics and sums; probabilities are rounded to bf16.
+ * scores, softmax statistics and sums; probabilities are rounded to bf16 (in two
+ * parts, to 2^-15, for sequences of up to 32 rows of new tokens and heads of a
+ * group).
  * rows: those of q and out; max_new: an upper bound of the step's new tokens
  * of any one sequence (the launches depend on both).  A step that exceeds
  * either sets `refused`, and its outputs are incomplete.  Rows past the last
