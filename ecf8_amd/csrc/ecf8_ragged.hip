@@ -101,8 +101,8 @@ struct Attn {
   const void *k, *v;                       // pools, or packed rows
   int64_t q_stride, out_stride, k_stride, v_stride;
   const float *ks, *vs;                    // scales of e4m3 pools
-  const int *starts, *lengths, *table;     // of the batch; packed rows: starts alone
-  const int *n_items, *others;             // other: items of a class that is not launched
+  const int *starts, *table;               // of the batch; packed rows: starts alone
+  const int *n_items, *others;             // others: items of a class that is not launched
   const Item *items;
   int *refused;
   float2 *stats;                           // partial maxima and sums
@@ -577,7 +577,6 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const int n_rows = min(p.n * a.group - p.row0, 16 * T);
   // (pages: an item is a whole sequence, of more tokens than the call was for)
   if (kSrc != kPacked && p.n * a.group > 16 * T && threadIdx.x == 0 && a.refused) *a.refused = 1;
-  if (n_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned step's lengths
   const int low = p.cached + p.row0 / a.group;  // the first query's limit
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
@@ -772,7 +771,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
   Place p;
   if (!get_item<kSrc>(a, kTileRows, (int)blockIdx.x / a.Hkv, p, lane)) return;
   const int all_rows = min(p.n * a.group - p.row0, kTileRows);
-  if (all_rows <= 0 || p.start < 0 || p.cached < 0) return;  // not the planned lengths
   const int first_row = 16 * kT * wave, n_rows = min(all_rows - first_row, 16 * kT);
   // the last position that all rows of the wave read, and of the workgroup
   const int low = p.cached + (p.row0 + min(first_row, all_rows - 1)) / a.group;
@@ -1127,7 +1125,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   a.k = k_pool, a.v = v_pool;
   a.q_stride = q_stride, a.out_stride = out_stride;
   a.ks = fp8 ? k_scale : nullptr, a.vs = fp8 ? v_scale : nullptr;
-  a.starts = b->starts, a.lengths = b->lengths, a.table = b->table, a.refused = b->refused;
+  a.starts = b->starts, a.table = b->table, a.refused = b->refused;
   a.Hkv = b->Hkv, a.group = G, a.rows = (int)rows, a.seqs = b->seqs, a.width = b->width;
   a.shift = __builtin_ctz((unsigned)b->page_size), a.pages = (uint32_t)b->pages;
   a.scale = kLog2e / sqrtf((float)kD);
