@@ -132,7 +132,9 @@ __device__ __forceinline__ void fill_row(const Plan &a, const int *first, int i)
 // One workgroup plans the step: prefix sums over the sequences (rows,
 // pages to take, pages to give back) say where everything goes, then pages,
 // items and rows are written element by element, each finding its sequence by
-// bisection in LDS.  All of it is latency: ~15 dependent rounds.
+// bisection in LDS.  All of it is latency, of three scans and some ten dependent
+// loads: 64 sequences 8.8 us, 512 that leave and 512 that come 18.8 us.  (Scans of
+// one value each, nine of them: 11.2 us.)
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   __shared__ int s_start[kMaxSeqs + 1], s_take[kMaxSeqs + 1], s_back[kMaxSeqs + 1];
   __shared__ int s_waves[2][3][kPlanWaves];  // (of two scans in a row)
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   // a workgroup's share is long: the long ones, laid end to end, are cut at
   // the multiples of the share.  Items are listed from the longest on: that
   // way a tile's last piece and the next one's first follow each other on a CU,
-  // and short tiles fill up what is left.  (1024 rows over 8700 keys: 135 us,
+  // and short tiles fill up what is left.  (1024 rows over 8700 keys: 150 us,
   // 254 us in equal parts, of which 33 met 32 CUs.)
   int t_items = 0, t_joins = 0;
   if (n_tiles > 0) {  // uniform
@@ -413,6 +415,8 @@ struct Write {
 // 16 lanes a head, 8 dims a lane (16-byte loads); dims d and d +- 64 lie 8
 // lanes apart, the norm's sum and the rotary partner are row rotations.
 // Workgroup: one row, 16 kU heads, all loads before the arithmetic.
+// HBM-bound: 8192 rows of 32 + 16 heads (202 MB) 31 us, 6.5 TB/s; a step of 16
+// rows 2.3 us, two memory round trips.
 template <int kU, bool kFp8>
 __global__ __launch_bounds__(256) void write_kernel(Write a) {
   const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x % a.parts;
@@ -533,7 +537,11 @@ extern "C" int ecf8_paged_qk_norm_rope(const void *qkv, int64_t rows, const ecf8
       !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return ECF8_ERR_MISALIGNED;
   const int H = b->Hq + 2 * b->Hkv;
-  const bool wide = rows * ((H + 15) / 16) > 2048;  // enough workgroups either way
+  // Three heads a lane once there are workgroups enough either way: 48 heads,
+  // 16 / 512 / 1024 / 8192 rows 2.3 / 4.1 / 6.0 / 32.8 us with one and 3.0 / 4.2 /
+  // 5.9 / 30.8 us with three; 12 heads, of which one does, 11.3 and 12.8 us for
+  // 8192 rows.
+  const bool wide = H > 32 && rows * ((H + 15) / 16) > 2048;
   const int per = wide ? 48 : 16, parts = (H + per - 1) / per;
   const Write a{static_cast<const uint16_t *>(qkv), static_cast<const uint16_t *>(q_norm),
                 static_cast<const uint16_t *>(k_norm), cos_t, sin_t, b->slots, b->positions,

@@ -408,7 +408,8 @@ struct Place {
 // The item-th tile of packed prompts, the ones that read the most keys first:
 // i-th tiles of all sequences before (i - 1)-th ones.  Up to kSorted sequences:
 // bisection for the level i, of which every lane counts kSorted / 64
-// sequences' tiles.  24 prompts of 8192 rows: 82 us, 104 us in packed order.
+// sequences' tiles.  24 prompts of 8192 rows: 78 us, 82 us in packed order; with
+// 512 sequences the search costs more than it gains (95 us, 83 us).
 constexpr int kSorted = 128;
 __device__ __forceinline__ bool sorted_tile(const Attn &a, int tile_rows, int item, Place &p,
                                             int lane) {
@@ -551,7 +552,7 @@ __device__ __forceinline__ void lds_barrier() {
 // KV head against positions [k0, k1), 128 a round, 32 a wave; the waves' sums
 // are joined in LDS.  A wave stages its keys and values through registers into
 // LDS of its own, a round ahead, so the loop has no barrier.  T = 1 where the
-// step's rows allow it: 174 registers instead of 238.
+// step's rows allow it: 176 us and 74 us in the cases below, 178 and 84 us with 2.
 //
 // Bound by the pages' bytes: 64 sequences of up to 8192 keys, 8 heads (1.11 GB),
 // 168 us, 6.6 TB/s; six of 100000 keys in e4m3, 4 heads (390 MB), 66 us, 5.9

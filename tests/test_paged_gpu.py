@@ -183,7 +183,8 @@ def _turned(x, w, cos, sin):
 @pytest.mark.parametrize("cached,new,page,Hq,Hkv,fp8,extra", [
     ([0], [1], 1, 1, 1, False, 0), ([5, 0, 31], [1, 0, 1], 16, 8, 2, False, 3),
     ([0, 7, 100], [33, 1, 65], 32, 32, 8, False, 2), ([0, 7, 100], [33, 1, 65], 32, 32, 4, True, 2),
-    ([3], [700], 64, 5, 5, True, 0), ([0, 0], [200, 900], 128, 7, 1, False, 1)])
+    ([3], [700], 64, 5, 5, True, 0), ([0, 0], [200, 900], 128, 7, 1, False, 1),
+    ([9, 0], [700, 400], 16, 30, 6, False, 1), ([9, 0], [700, 400], 16, 50, 10, True, 1)])
 def test_write_matches_fp64(cuda_device, cached, new, page, Hq, Hkv, fp8, extra):
     """q rounded to bf16 (2^-8 of it), pools to bf16 or e4m3 (2^-4 of it, or
     half the smallest step 2^-10 of a scale); before that fp32, within 2^-19
