@@ -298,16 +298,20 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       t.units = (t.end + kTileKeys - 1) / kTileKeys;
       return t;
     };
-    // (past kPlanThreads tiles, in 256 units, rounded up: the total fits)
-    const int scale = n_tiles > kPlanThreads ? 256 : 1;
+    // A share of all units, to the unit: rounded up a thread, 1036 tiles of which two
+    // have 1564 units were all one piece (2590 us of attention, now 720).  The
+    // total can pass 32 bits (a thread's cannot: at most 1370 tiles of 2^18), so low
+    // and high parts are summed apart.
     int mine = 0;
     for (int i = tid; i < n_tiles; i += kPlanThreads) mine += tile_at(i).units + kTileStart;
-    const int sum_units[1] = {(mine + scale - 1) / scale};
-    int skip[1], all_units[1];
-    block_scan(sum_units, s_waves[1], skip, all_units);
+    const int halves[2] = {mine & 0xffff, mine >> 16};
+    int skip[2], all[2];
+    block_scan(halves, s_waves[1], skip, all);
+    const int64_t all_units = ((int64_t)all[1] << 16) + all[0];
     // (more units than a tile can have are as good as any)
-    const int64_t exact = ((int64_t)all_units[0] * scale + a.tile_target - 1) / a.tile_target;
-    const int share = (int)min(max(exact, (int64_t)(2 * kTileMinUnits)), (int64_t)1 << 20);
+    const int64_t exact = (all_units + a.tile_target - 1) / a.tile_target;
+    const int share = __builtin_amdgcn_readfirstlane(
+        (int)min(max(exact, (int64_t)(2 * kTileMinUnits)), (int64_t)1 << 20));
     // Twice over the tiles: count the items of each length, then write them.
     for (int write = 0; write < 2; ++write) {
       int from0 = 0, t_parts = 0;
