@@ -1111,6 +1111,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
     return ECF8_ERR_INVALID_ARG;
   if (const int rc = check_batch(b)) return rc;
   if (rows > b->rows) return ECF8_ERR_CAPACITY;
+  if (max_new > rows) max_new = rows;  // (and its products fit)
   const int64_t wide = (int64_t)b->Hq * kD;
   if (q_stride % 8 || out_stride % 4 || (rows > 1 && (q_stride < wide || out_stride < wide)))
     return ECF8_ERR_UNSUPPORTED;

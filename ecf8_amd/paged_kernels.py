@@ -209,7 +209,7 @@ def paged_attention(q, k_pool, v_pool, batch: PagedBatch, out, max_new=None, k_s
     qs, os = _heads(q, batch.Hq, "q", dev), _heads(out, batch.Hq, "out", dev)
     if not 1 <= rows <= batch.max_rows or out.shape[0] < rows:
         raise ECF8Error(f"q must have 1..{batch.max_rows} rows, and out as many")
-    most = rows if max_new is None else int(max_new)
+    most = rows if max_new is None else min(int(max_new), rows)
     if most < 1:
         raise ECF8Error("max_new must be positive")
     fp8, ks, vs = _pools(batch, k_pool, v_pool, k_scale, v_scale)

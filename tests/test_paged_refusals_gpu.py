@@ -1,0 +1,54 @@
+"""Steps that the ragged-batch attention refuses on the device, and calls that
+it must not refuse."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from ecf8_amd._lib import ECF8Error
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+
+
+def _ints(v, dev):
+    return torch.tensor(v, dtype=torch.int32).to(dev)
+
+
+def _planned(dev, cached, new, Hq=4, Hkv=1):
+    """A planned batch, q of zeros, pools whose values are all 2, and out of 3."""
+    from ecf8_amd.paged_kernels import PagedBatch, paged_plan
+
+    b = PagedBatch(len(new), sum(new), 64, 16, 512, Hq, Hkv, dev)
+    paged_plan(b, _ints(cached, dev), _ints(new, dev))
+    q = torch.zeros(sum(new), Hq, D, dtype=torch.bfloat16, device=dev)
+    pools = [torch.full((64, Hkv, 16, D), 2.0, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    out = torch.full((sum(new), Hq * D), 3.0, dtype=torch.bfloat16, device=dev)
+    torch.cuda.synchronize()
+    b.raise_refused()
+    return b, q, pools, out
+
+
+@pytest.mark.parametrize("bound", [3, 2 ** 31, 2 ** 60, 2 ** 61, 2 ** 62, 2 ** 63 - 1, 2 ** 80])
+@pytest.mark.parametrize("new", [[3, 1], [1, 60]])
+def test_any_large_max_new_is_no_bound(cuda_device, new, bound):
+    """Also where its product with the heads of a group (4) passes 64 bits."""
+    from ecf8_amd._lib import lib
+    from ecf8_amd.paged_kernels import paged_attention
+
+    b, q, pools, out = _planned(cuda_device, [300, 7], new)
+    bound = max(bound, max(new))
+    paged_attention(q, *pools, b, out, max_new=bound)
+    torch.cuda.synchronize()
+    b.raise_refused()
+    assert bool((out == 2.0).all())
+    if bound < 2 ** 63:
+        out.fill_(3.0)
+        assert lib().ecf8_paged_attention(
+            q.data_ptr(), 4 * D, sum(new), b._ref, *(p.data_ptr() for p in pools), 0, None, None,
+            bound, out.data_ptr(), 4 * D, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        b.raise_refused()
+        assert bool((out == 2.0).all())
