@@ -110,6 +110,7 @@ struct Attn {
   int Hkv, group, rows, seqs, width, shift;
   uint32_t pages;
   int grid;                                // item slots launched per KV head
+  int max_new;                             // new tokens of a sequence
   float scale;                             // of the scores, times log2(e)
 };
 
@@ -516,6 +517,7 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
     if (item >= *a.n_items) return false;
     p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
     p.start = it.start, p.n = it.n, p.cached = it.cached;
+    if (p.n > a.max_new && threadIdx.x == 0 && a.refused) *a.refused = 1;
     return true;
   }
 }
@@ -576,8 +578,6 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   Place p;
   if (!get_item<kSrc>(a, 16 * T, (int)blockIdx.x / a.Hkv, p, lane)) return;
   const int n_rows = min(p.n * a.group - p.row0, 16 * T);
-  // (pages: an item is a whole sequence, of more tokens than the call was for)
-  if (kSrc != kPacked && p.n * a.group > 16 * T && threadIdx.x == 0 && a.refused) *a.refused = 1;
   const int low = p.cached + p.row0 / a.group;  // the first query's limit
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
@@ -1130,6 +1130,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   a.starts = b->starts, a.table = b->table, a.refused = b->refused;
   a.Hkv = b->Hkv, a.group = G, a.rows = (int)rows, a.seqs = b->seqs, a.width = b->width;
   a.shift = __builtin_ctz((unsigned)b->page_size), a.pages = (uint32_t)b->pages;
+  a.max_new = (int)max_new;
   a.scale = kLog2e / sqrtf((float)kD);
   const bool many = max_new * G > kFewRows;
   Joins few{}, tiles{};

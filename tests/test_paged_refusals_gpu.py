@@ -52,3 +52,20 @@ def test_any_large_max_new_is_no_bound(cuda_device, new, bound):
         torch.cuda.synchronize()
         b.raise_refused()
         assert bool((out == 2.0).all())
+
+
+@pytest.mark.parametrize("new,max_new", [
+    ([4], 1), ([2, 1], 1), ([8], 5), ([8, 1], 7), ([1, 40], 9), ([1, 40], 39), ([300, 2], 250)])
+def test_more_new_tokens_than_max_new_are_refused(cuda_device, new, max_new):
+    """Also where the kernels launched for max_new could do the step."""
+    from ecf8_amd.paged_kernels import paged_attention
+
+    b, q, pools, out = _planned(cuda_device, [0] * len(new), new)
+    paged_attention(q, *pools, b, out, max_new=max_new)
+    torch.cuda.synchronize()
+    with pytest.raises(ECF8Error):
+        b.raise_refused()
+    paged_attention(q, *pools, b, out, max_new=max(new))
+    torch.cuda.synchronize()
+    b.raise_refused()
+    assert bool((out == 2.0).all())
