@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import ECF8Error, check, lib
 from .head_kernels import refusal_flag
@@ -103,6 +104,24 @@ def _launch(name, dev, *args):
             check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
 
 
+def _unfollowed(names, *tensors):
+    """Refuses tensors that autograd follows, backward or forward."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ECF8Error(f"{_name(names, tensors, t)} is followed by autograd: these "
+                                "kernels have no backward")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ECF8Error(f"{_name(names, tensors, t)} is followed by autograd: these "
+                                "kernels have no tangent")
+
+
+def _name(names, tensors, t):
+    return next(n for n, u in zip(names.split(), tensors) if u is t)
+
+
 def _want(t, dtype, name, dev):
     """_need, at half of its price where all is well."""
     if t.dtype is not dtype or not t.is_cuda or t.device != dev or not t.is_contiguous():
@@ -120,8 +139,6 @@ def _heads(t, heads, name, dev):
     heads contiguous."""
     if not t.is_cuda or t.device != dev or t.dtype != torch.bfloat16:
         raise ECF8Error(f"{name} must be bfloat16 on {dev}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ECF8Error(f"{name} is followed by autograd: these kernels have no backward")
     shape, stride = t.shape, t.stride()
     if not ((len(shape) == 2 and shape[1] == heads * HEAD_DIM and stride[1] == 1)
             or (len(shape) == 3 and shape[1:] == (heads, HEAD_DIM) and stride[2] == 1
@@ -175,10 +192,10 @@ def paged_qk_norm_rope(qkv, batch: PagedBatch, q_norm, k_norm, eps, cos_t, sin_t
     the pools [pages, Hkv, page_size, 128], bf16 or e4m3fn (codes of x / scale,
     fp32 scales [Hkv]).  cos_t / sin_t fp32 [>= max_len, 64]."""
     dev, Hq, Hkv = batch.device, batch.Hq, batch.Hkv
+    _unfollowed("qkv q_norm k_norm cos sin q_out k_pool v_pool k_scale v_scale", qkv, q_norm,
+                k_norm, cos_t, sin_t, q_out, k_pool, v_pool, k_scale, v_scale)
     for t, n in ((qkv, "qkv"), (q_norm, "q_norm"), (k_norm, "k_norm"), (q_out, "q_out")):
         _want(t, torch.bfloat16, n, dev)
-    if qkv.requires_grad and torch.is_grad_enabled():
-        raise ECF8Error("qkv is followed by autograd: this kernel has no backward")
     _want(cos_t, torch.float32, "cos", dev)
     _want(sin_t, torch.float32, "sin", dev)
     rows = qkv.shape[0]
@@ -206,6 +223,7 @@ def paged_attention(q, k_pool, v_pool, batch: PagedBatch, out, max_new=None, k_s
     the new tokens of any sequence (default: any number); one token each runs
     one kernel less.  Returns ``out``."""
     dev, rows = batch.device, q.shape[0]
+    _unfollowed("q out k_pool v_pool k_scale v_scale", q, out, k_pool, v_pool, k_scale, v_scale)
     qs, os = _heads(q, batch.Hq, "q", dev), _heads(out, batch.Hq, "out", dev)
     if not 1 <= rows <= batch.max_rows or out.shape[0] < rows:
         raise ECF8Error(f"q must have 1..{batch.max_rows} rows, and out as many")
@@ -226,6 +244,7 @@ def ragged_attention(q, k, v, starts, out):
     rows 0..t of its sequence.  out: bf16 [N, Hq * 128] or [N, Hq, 128], rows
     outside every sequence left as they were.  Returns ``out``."""
     dev = q.device
+    _unfollowed("q k v out", q, k, v, out)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] < 1:
         raise ECF8Error("q, k, v must be [rows, heads, 128]")
     N, Hq, Hkv = q.shape[0], q.shape[1], k.shape[1]
