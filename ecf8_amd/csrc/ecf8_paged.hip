@@ -31,6 +31,7 @@ struct Plan {
   Join *few_joins, *tile_joins;
   int seqs, rows, pages, shift, width, group;  // page size 1 << shift
   int few_target, tile_target, fill_rows;
+  uint64_t stamp;
 };
 
 constexpr int kPlanThreads = 1024;
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
     }
     __syncthreads();
     if (tid == 0) {
-      *a.counts = Counts{0, 0, 0, 0};
+      *a.counts = Counts{0, 0, 0, 0, a.stamp};
       if (a.refused) *a.refused = 1;
     }
     if (a.fill_rows)
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       if (!write) t_items = start_buckets(s_bucket[1], s_waves[0]);
     }
   }
-  if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins};
+  if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins, a.stamp};
   if (a.fill_rows) {
     __threadfence_block();
     __syncthreads();
@@ -517,7 +518,7 @@ extern "C" int ecf8_paged_plan(const ecf8_paged_batch *b, const int *cached,
                reinterpret_cast<Join *>(base + w.few_joins_at),
                reinterpret_cast<Join *>(base + w.tile_joins_at), b->seqs, b->rows, b->pages,
                __builtin_ctz((unsigned)b->page_size), b->width, b->Hq / b->Hkv, w.few_parts / 2,
-               w.tile_parts / 2, one};
+               w.tile_parts / 2, one, ecf8::paged::schedule_stamp(b)};
   plan_kernel<<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
   if (!one)
     fill_kernel<<<(unsigned)((b->rows + kFillThreads - 1) / kFillThreads), kFillThreads, 0,

@@ -41,8 +41,12 @@ struct Join {
   int pad[3];
 };
 
+// At the start of the work buffer.  stamp: of the sizes that the plan wrote the
+// lists for (schedule_stamp), zero before the first plan.  The attention reads no
+// item under another: a list of anything else would send it out of its buffers.
 struct Counts {
   int few, tiles, few_joins, tile_joins;
+  uint64_t stamp;
 };
 
 // Byte offsets of the work buffer's parts.
@@ -78,6 +82,15 @@ inline Work work_layout(int64_t seqs, int64_t rows, int Hq, int Hkv) {
   w.tile_sums = take(w.tile_parts * (int64_t)Hkv * kTileRows * kD * 4);
   w.bytes = at;
   return w;
+}
+
+// FNV-1a over the sizes that items and the buffer's parts depend on; never zero.
+inline uint64_t schedule_stamp(const ecf8_paged_batch *b) {
+  uint64_t h = 0xcbf29ce484222325ull;
+  for (const int x : {b->seqs, b->rows, b->pages, b->page_size, b->width, b->Hq, b->Hkv})
+    for (int byte = 0; byte < 4; ++byte)
+      h = (h ^ (((uint32_t)x >> (8 * byte)) & 0xff)) * 0x100000001b3ull;
+  return h | 1;
 }
 
 inline bool sizes_ok(int64_t seqs, int64_t rows, int Hq, int Hkv) {

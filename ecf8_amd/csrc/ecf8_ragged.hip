@@ -104,6 +104,8 @@ struct Attn {
   const int *starts, *table;               // of the batch; packed rows: starts alone
   const int *n_items, *others;             // others: items of a class that is not launched
   const Item *items;
+  const uint64_t *stamp;                   // of the schedule, and what it has to be
+  uint64_t want_stamp;
   int *refused;
   float2 *stats;                           // partial maxima and sums
   float *sums;
@@ -510,11 +512,12 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
   } else {
     // (the last workgroup, which has no item or a short one)
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused &&
-        (a.starts[a.seqs] > a.rows || (a.others && *a.others > 0)))
+        (a.starts[a.seqs] > a.rows ||
+         (*a.stamp == a.want_stamp ? a.others && *a.others > 0 : *a.stamp != 0)))
       *a.refused = 1;
     const Item it = a.items[item];  // item < a.grid: in the list, filled or not
     asm volatile("" ::"s"(it.seq), "s"(it.start));  // not after the wait for n_items
-    if (item >= *a.n_items) return false;
+    if (*a.stamp != a.want_stamp || item >= *a.n_items) return false;
     p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
     p.start = it.start, p.n = it.n, p.cached = it.cached;
     if (p.n > a.max_new && threadIdx.x == 0 && a.refused) *a.refused = 1;
@@ -1021,7 +1024,7 @@ __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int gr
   const int j = group / o.rows_groups / a.Hkv;
   const Join jn = o.list[j];  // j: in the list, filled or not
   asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for the count
-  if (j >= *o.n) return;
+  if (*a.stamp != a.want_stamp || j >= *o.n) return;
   constexpr int part_rows = kPartRows;
   const int n_rows = min(jn.tokens * a.group - jn.row0, part_rows);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
@@ -1128,6 +1131,7 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   a.q_stride = q_stride, a.out_stride = out_stride;
   a.ks = fp8 ? k_scale : nullptr, a.vs = fp8 ? v_scale : nullptr;
   a.starts = b->starts, a.table = b->table, a.refused = b->refused;
+  a.stamp = &counts->stamp, a.want_stamp = schedule_stamp(b);
   a.Hkv = b->Hkv, a.group = G, a.rows = (int)rows, a.seqs = b->seqs, a.width = b->width;
   a.shift = __builtin_ctz((unsigned)b->page_size), a.pages = (uint32_t)b->pages;
   a.max_new = (int)max_new;

@@ -40,7 +40,8 @@ extern "C" {
  *   refused    [1] or NULL, memory that the device can write (e.g. pinned host
  *              memory): set when a kernel refuses a step's values
  *   work       ecf8_paged_work_bytes bytes, 16-byte aligned: the attention's
- *              schedule (written by ecf8_paged_plan) and partial sums
+ *              schedule (written by ecf8_paged_plan) and partial sums; its first
+ *              256 bytes are zeros before the first plan (an empty step)
  */
 typedef struct ecf8_paged_batch {
   int *table;
@@ -115,8 +116,9 @@ int ecf8_paged_qk_norm_rope(const void *qkv, int64_t rows, const ecf8_paged_batc
  * group).
  * rows: those of q and out; max_new: an upper bound of the step's new tokens
  * of any one sequence (the launches depend on both).  A step that exceeds
- * either sets `refused`, and its outputs are incomplete.  Rows past the last
- * sequence are left as they were.
+ * either sets `refused`, and its outputs are incomplete.  So does a `work` that was
+ * not planned for a batch of these sizes, of which nothing is read.  Rows past the
+ * last sequence are left as they were.
  */
 int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t rows,
                          const ecf8_paged_batch *batch,

@@ -69,3 +69,47 @@ def test_more_new_tokens_than_max_new_are_refused(cuda_device, new, max_new):
     torch.cuda.synchronize()
     b.raise_refused()
     assert bool((out == 2.0).all())
+
+
+@pytest.mark.parametrize("new", [[1, 1], [60, 3]])
+def test_a_schedule_of_other_sizes_is_not_read(cuda_device, new):
+    """A work buffer that was never planned, or planned for a batch of other
+    sizes: no row is written, and the step is refused; one of zeros is an
+    empty step."""
+    from ecf8_amd.paged_kernels import PagedBatch, paged_attention, paged_plan
+
+    dev, Hq, Hkv = cuda_device, 8, 2
+    b, q, pools, out = _planned(dev, [300, 5], new, Hq, Hkv)
+
+    def refused():
+        out.fill_(3.0)
+        paged_attention(q, *pools, b, out)
+        torch.cuda.synchronize()
+        bad, b.refused[0] = int(b.refused[0]), 0
+        return bad
+
+    assert refused() == 0 and bool((out == 2.0).all())
+    planned = b.work.clone()
+    for fill in (0x01, 0x5a, 0x7f, 0x80, 0xff):
+        b.work.fill_(fill)
+        assert refused() == 1 and bool((out == 3.0).all()), fill
+    b.work[:256].zero_()
+    assert refused() == 0 and bool((out == 3.0).all())
+    # a smaller batch's schedule, in the larger one's buffer, and the other way round
+    small = PagedBatch(2, sum(new), 32, 16, 512, Hq, Hkv, dev)
+    paged_plan(small, _ints([300, 5], dev), _ints(new, dev))
+    b.work[: small.work.numel()].copy_(small.work)
+    assert refused() == 1 and bool((out == 3.0).all())
+    for field, other in (("seqs", 1), ("rows", sum(new) - 1), ("width", b._c.width - 1)):
+        b.work.copy_(planned)
+        was = getattr(b._c, field)
+        setattr(b._c, field, other)
+        rows = min(sum(new), b._c.rows)
+        out.fill_(3.0)
+        paged_attention(q[:rows], *pools, b, out)
+        torch.cuda.synchronize()
+        bad, b.refused[0] = int(b.refused[0]), 0
+        setattr(b._c, field, was)
+        assert bad == 1 and bool((out == 3.0).all()), field
+    b.work.copy_(planned)
+    assert refused() == 0 and bool((out == 2.0).all())
