@@ -424,7 +424,7 @@ __device__ __forceinline__ bool sorted_tile(const Attn &a, int tile_rows, int it
     if (64 * i >= a.seqs) continue;  // uniform
     if (s < a.seqs) {
       here[i] = min(max(a.starts[s], 0), a.rows);
-      n[i] = max(min(a.starts[s + 1], a.rows) - here[i], 0);
+      n[i] = max(min(a.starts[s + 1], a.rows), here[i]) - here[i];
     }
     tiles[i] = (int)((uint32_t)(n[i] * a.group + tile_rows - 1) / (uint32_t)tile_rows);
     most = max(most, tiles[i]);
@@ -486,7 +486,7 @@ __device__ __forceinline__ bool packed_tile(const Attn &a, int tile_rows, int it
   }
   p.seq = lo;
   p.start = here;
-  p.n = max(next - here, 0);
+  p.n = max(next, here) - here;
   p.row0 = (vt - first(here, lo)) * tile_rows;
   return p.row0 >= 0 && p.row0 < p.n * a.group;
 }

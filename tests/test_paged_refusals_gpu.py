@@ -113,3 +113,23 @@ def test_a_schedule_of_other_sizes_is_not_read(cuda_device, new):
         assert bad == 1 and bool((out == 3.0).all()), field
     b.work.copy_(planned)
     assert refused() == 0 and bool((out == 2.0).all())
+
+
+@pytest.mark.parametrize("Hq", [4, 400])  # 32 rows a workgroup, and tiles
+@pytest.mark.parametrize("starts", [
+    [100, -2 ** 31], [200, -2 ** 31 + 5, 200], [3] * 150 + [-2 ** 31], [-2 ** 31, 2 ** 31 - 1]])
+def test_packed_starts_at_the_ends_of_int32_stay_in_range(cuda_device, starts, Hq):
+    """No difference of starts overflows: no row but those of [0, N) is touched."""
+    from ecf8_amd.paged_kernels import ragged_attention
+
+    dev, N = cuda_device, 200
+    x = torch.zeros(N, Hq + 2, D, dtype=torch.bfloat16, device=dev)
+    x[:, Hq + 1:] = 2.0
+    whole = torch.full((N + 20, Hq * D), 3.0, dtype=torch.bfloat16, device=dev)
+    out = whole[10: N + 10]
+    ragged_attention(x[:, :Hq], x[:, Hq: Hq + 1], x[:, Hq + 1:], _ints(starts, dev), out)
+    torch.cuda.synchronize()
+    assert bool((whole[:10] == 3.0).all()) and bool((whole[N + 10:] == 3.0).all())
+    assert bool(((out == 2.0) | (out == 3.0)).all())
+    if starts[0] < 0:  # one sequence, cut to the rows that there are
+        assert bool((out == 2.0).all())
