@@ -116,6 +116,8 @@ _SIGNATURES = {
                               _vp], _i32),
     "ecf8_ragged_attention": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _vp,
                                _i64, _vp], _i32),
+    "ecf8_ragged_attention_checked": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32,
+                                       _i32, _vp, _i64, _vp, _vp], _i32),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -508,6 +508,15 @@ template <Source kSrc>
 __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item, Place &p,
                                          int lane) {
   if constexpr (kSrc == kPacked) {
+    // (the last workgroup, which has no tile or one of the last)
+    if (a.refused && blockIdx.x == gridDim.x - 1) {
+      bool bad = false;
+      for (int s = threadIdx.x; s < a.seqs; s += 256) {
+        const int from = a.starts[s], to = a.starts[s + 1];
+        bad |= from < 0 || from > to || to > a.rows;
+      }
+      if (bad) *a.refused = 1;
+    }
     return find_tile(a, tile_rows, item, p, lane);
   } else {
     // (the last workgroup, which has no item or a short one)
@@ -1191,10 +1200,11 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   return launched();
 }
 
-extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void *k,
-                                     int64_t k_stride, const void *v, int64_t v_stride,
-                                     int64_t rows, const int *starts, int64_t seqs, int Hq,
-                                     int Hkv, void *out, int64_t out_stride, void *stream) {
+extern "C" int ecf8_ragged_attention_checked(const void *q, int64_t q_stride, const void *k,
+                                             int64_t k_stride, const void *v, int64_t v_stride,
+                                             int64_t rows, const int *starts, int64_t seqs, int Hq,
+                                             int Hkv, void *out, int64_t out_stride, int *refused,
+                                             void *stream) {
   if (!q || !k || !v || !starts || !out || rows <= 0 || seqs <= 0 || Hq <= 0 || Hkv <= 0)
     return ECF8_ERR_INVALID_ARG;
   const int64_t wide = (int64_t)Hq * kD, kv = (int64_t)Hkv * kD;
@@ -1204,13 +1214,13 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
                                       v_stride < kv)))
     return ECF8_ERR_UNSUPPORTED;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8) ||
-      !aligned(starts, 4))
+      !aligned(starts, 4) || !aligned(refused, 4))
     return ECF8_ERR_MISALIGNED;
   Attn a{};
   a.q = static_cast<const uint16_t *>(q), a.out = static_cast<uint16_t *>(out);
   a.k = k, a.v = v;
   a.q_stride = q_stride, a.out_stride = out_stride, a.k_stride = k_stride, a.v_stride = v_stride;
-  a.starts = starts;
+  a.starts = starts, a.refused = refused;
   a.Hkv = Hkv, a.group = Hq / Hkv, a.rows = (int)rows, a.seqs = (int)seqs;
   a.scale = kLog2e / sqrtf((float)kD);
   // Tiles once they make up a workgroup for every CU: 2048 rows of 32 heads take
@@ -1223,4 +1233,12 @@ extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void
 #undef ECF8_FEW
 #undef ECF8_TILES
   return launched();
+}
+
+extern "C" int ecf8_ragged_attention(const void *q, int64_t q_stride, const void *k,
+                                     int64_t k_stride, const void *v, int64_t v_stride,
+                                     int64_t rows, const int *starts, int64_t seqs, int Hq,
+                                     int Hkv, void *out, int64_t out_stride, void *stream) {
+  return ecf8_ragged_attention_checked(q, q_stride, k, k_stride, v, v_stride, rows, starts, seqs,
+                                       Hq, Hkv, out, out_stride, nullptr, stream);
 }

@@ -22,7 +22,7 @@ import torch
 from torch.autograd import forward_ad
 
 from ._lib import ECF8Error, check, lib
-from .head_kernels import refusal_flag
+from .head_kernels import _flag_ptr, refusal_flag
 from .llm_kernels import _need
 
 HEAD_DIM = 128
@@ -236,13 +236,15 @@ def paged_attention(q, k_pool, v_pool, batch: PagedBatch, out, max_new=None, k_s
     return out
 
 
-def ragged_attention(q, k, v, starts, out):
+def ragged_attention(q, k, v, starts, out, refused=None):
     """Causal attention of packed prompts of different lengths, without a
     cache: sequence s has rows [starts[s], starts[s + 1]) (int32, on the
     device, ascending) of q [N, Hq, 128] and k, v [N, Hkv, 128] (bf16, e.g.
     slices of a fused projection's output), Hq a multiple of Hkv; row t reads
     rows 0..t of its sequence.  out: bf16 [N, Hq * 128] or [N, Hq, 128], rows
-    outside every sequence left as they were.  Returns ``out``."""
+    outside every sequence left as they were.  ``refused`` (a refusal_flag()):
+    set by starts that are not ascending or outside [0, N], whose rows are
+    incomplete.  Returns ``out``."""
     dev = q.device
     _unfollowed("q k v out", q, k, v, out)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] < 1:
@@ -255,7 +257,7 @@ def ragged_attention(q, k, v, starts, out):
     _want(starts, torch.int32, "starts", dev)
     if starts.numel() < 2:
         raise ECF8Error("starts must hold the sequences' first rows and the end")
-    _launch("ecf8_ragged_attention", dev, q.data_ptr(), strides[0], k.data_ptr(), strides[1],
+    _launch("ecf8_ragged_attention_checked", dev, q.data_ptr(), strides[0], k.data_ptr(), strides[1],
             v.data_ptr(), strides[2], N, starts.data_ptr(), starts.numel() - 1, Hq, Hkv,
-            out.data_ptr(), os)
+            out.data_ptr(), os, _flag_ptr(refused))
     return out

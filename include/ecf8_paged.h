@@ -139,6 +139,15 @@ int ecf8_ragged_attention(const void *q, int64_t q_stride, const void *k, int64_
                           int64_t seqs, int Hq, int Hkv, void *out, int64_t out_stride,
                           void *stream);
 
+/* ecf8_ragged_attention; starts that are not ascending, or outside [0, rows],
+ * also set refused[0] (memory that the device can write, e.g. pinned host memory).
+ * Without it such starts are cut to the rows that there are, and the outputs are
+ * incomplete. */
+int ecf8_ragged_attention_checked(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                                  const void *v, int64_t v_stride, int64_t rows,
+                                  const int *starts, int64_t seqs, int Hq, int Hkv, void *out,
+                                  int64_t out_stride, int *refused, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

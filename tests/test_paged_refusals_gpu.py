@@ -133,3 +133,36 @@ def test_packed_starts_at_the_ends_of_int32_stay_in_range(cuda_device, starts, H
     assert bool(((out == 2.0) | (out == 3.0)).all())
     if starts[0] < 0:  # one sequence, cut to the rows that there are
         assert bool((out == 2.0).all())
+
+
+@pytest.mark.parametrize("Hq", [4, 400])  # 32 rows a workgroup, and tiles
+@pytest.mark.parametrize("starts,bad", [
+    ([0, 200], 0), ([7, 9, 9, 150], 0), ([0, 0, 0], 0), ([-1, 200], 1), ([0, 201], 1), ([150, 0], 1),
+    ([0, 90, 89, 200], 1), ([0, 500, 200], 1), ([-9, -5], 1), ([201, 201], 1), ([0, 2 ** 31 - 1], 1),
+    ([-2 ** 31, 10], 1), ([200, -2 ** 31], 1),
+    (list(range(201)), 0), (list(range(150)) + [100] + list(range(150, 200)), 1),
+    ([i // 5 for i in range(1001)], 0), ([i // 5 for i in range(1001)] + [0], 1),
+    ([5] + [i // 5 for i in range(1001)], 1)])
+def test_packed_starts_out_of_order_are_refused(cuda_device, starts, bad, Hq):
+    """Equal values, so a row is their mean or as it was; no row but those of
+    [0, N) is touched."""
+    from ecf8_amd.head_kernels import refusal_flag
+    from ecf8_amd.paged_kernels import ragged_attention
+
+    dev, N = cuda_device, 200
+    x = torch.zeros(N, Hq + 2, D, dtype=torch.bfloat16, device=dev)
+    x[:, Hq + 1:] = 2.0
+    whole = torch.full((N + 20, Hq * D), 3.0, dtype=torch.bfloat16, device=dev)
+    out = whole[10: N + 10]
+    flag = refusal_flag()
+    parts = x[:, :Hq], x[:, Hq: Hq + 1], x[:, Hq + 1:]
+    ragged_attention(*parts, _ints(starts, dev), out, flag)
+    torch.cuda.synchronize()
+    assert int(flag) == bad
+    assert bool((whole[:10] == 3.0).all()) and bool((whole[N + 10:] == 3.0).all())
+    assert bool(((out == 2.0) | (out == 3.0)).all())
+    if not bad:
+        assert bool((out[starts[0]: starts[-1]] == 2.0).all())
+        ragged_attention(*parts, _ints(starts, dev), out)  # without a flag
+        torch.cuda.synchronize()
+        assert int(flag) == 0
