@@ -542,11 +542,15 @@ extern "C" int ecf8_paged_qk_norm_rope(const void *qkv, int64_t rows, const ecf8
       !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return ECF8_ERR_MISALIGNED;
   const int H = b->Hq + 2 * b->Hkv;
-  // Three heads a lane once there are workgroups enough either way: 48 heads,
-  // 16 / 512 / 1024 / 8192 rows 2.3 / 4.1 / 6.0 / 32.8 us with one and 3.0 / 4.2 /
-  // 5.9 / 30.8 us with three; 12 heads, of which one does, 11.3 and 12.8 us for
-  // 8192 rows.
-  const bool wide = H > 32 && rows * ((H + 15) / 16) > 2048;
+  // Three heads a lane, 48 a workgroup, once there are workgroups enough either
+  // way (48 heads, 16 / 512 / 1024 / 8192 rows 2.3 / 4.0 / 5.9 / 32.7 us with one and
+  // 3.0 / 4.1 / 5.9 / 30.5 us with three), where that makes one workgroup of two or
+  // three, or fills two thirds of its lanes.  8192 rows of 12 / 20 / 24 / 32 / 52 /
+  // 60 / 64 / 72 / 144 heads: 11.3 / 21.1 / 21.9 / 23.8 / 39.3 / 42.0 / 48.6 / 62.2 / 124 us
+  // with one, 12.8 / 15.3 / 17.0 / 21.3 / 42.5 / 44.0 / 47.6 / 54.2 / 103 us with three.
+  // (The rule's worst: 64 heads, 1024 rows in e4m3, 10.1 us with three, 8.4 with one.)
+  const bool fills = H <= 48 ? H > 16 : 3 * H >= 2 * 48 * ((H + 47) / 48);
+  const bool wide = fills && rows * ((H + 15) / 16) > 2048;
   const int per = wide ? 48 : 16, parts = (H + per - 1) / per;
   const Write a{static_cast<const uint16_t *>(qkv), static_cast<const uint16_t *>(q_norm),
                 static_cast<const uint16_t *>(k_norm), cos_t, sin_t, b->slots, b->positions,
