@@ -565,14 +565,14 @@ __device__ __forceinline__ void lds_barrier() {
 // Workgroup of four waves: up to 16 T rows (token, head of the group) of one
 // KV head against positions [k0, k1), 128 a round, 32 a wave; the waves' sums
 // are joined in LDS.  A wave stages its keys and values through registers into
-// LDS of its own, a round ahead, so the loop has no barrier.  T = 1 where the
-// step's rows allow it: 176 us and 74 us in the cases below, 178 and 84 us with 2.
+// LDS of its own, a round ahead, so the loop has no barrier.
 //
 // Bound by the pages' bytes: 64 sequences of up to 8192 keys, 8 heads (1.11 GB),
-// 168 us, 6.6 TB/s; six of 100000 keys in e4m3, 4 heads (390 MB), 66 us, 5.9
+// 169 us, 6.6 TB/s; six of 100000 keys in e4m3, 4 heads (390 MB), 68 us, 5.7
 // TB/s.  The matrix unit is busy for a tenth of that, so probabilities enter in
-// two parts (kFine) at no cost.  Page loads bypass the caches, since a page is read once: 186 and 83 us
-// when they did not, 205 and 97 us.
+// two parts (kFine) at no cost.  With the join, these take 172 and 72 us; 195 and 82
+// if page loads go through the caches, which a page, read once, gains nothing from;
+// 173 and 78 with T = 2 where the step's rows allow 1.
 template <Source kSrc, int T>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
                                                  (int64_t)w * a.k_stride + kvh * kD + 8 * unit);
         vr[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) +
                                                  (int64_t)w * a.v_stride + kvh * kD + 8 * unit);
-      } else {  // (read once: of e4m3 pages 88 us instead of 97, of bf16 185 instead of 205)
+      } else {  // (read once)
         kr[i] = __builtin_nontemporal_load(static_cast<const u32x4 *>(a.k) +
                                             (size_t)w * kUnits + unit);
         vr[i] = __builtin_nontemporal_load(static_cast<const u32x4 *>(a.v) +
@@ -758,10 +758,11 @@ constexpr int kTileWaves = kTileRows / (16 * kT);
 // Bound by the products (51 MFMA of 16 cycles a wave and step) and the vector
 // instructions beside them (140): 1.25 PFLOP/s in the loop of unmasked steps,
 // where a large library product reaches 1.34.  One prompt of 8192 tokens, 32
-// heads: 485 us, of which the loop takes 440; 24 prompts of 8192 tokens together:
-// 80 us, mostly the first loads and the last steps of ~100 short tiles.  Tiles of
-// 384 rows and eight waves reach the same rate in the loop, but take 505 and 104
-// us: fewer tiles fill the card less evenly.
+// heads: 485 to 505 us by card, of which the loop takes 440; 24 prompts of 8192
+// tokens together: 80 us, mostly the first loads and the last steps of ~100 short
+// tiles.  Tiles of 384 rows and eight waves reach the same rate in the loop, but take
+// 1.04 and 1.3 times as long: fewer tiles fill the card less evenly.  Pages of fewer
+// than 8 positions (not kWhole): 6 registers spilled in bf16.
 template <Source kSrc, bool kWhole>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Attn a) {
   // Stages of a step's keys and values each: after the barrier before step j
@@ -1223,8 +1224,10 @@ extern "C" int ecf8_ragged_attention_checked(const void *q, int64_t q_stride, co
   a.starts = starts, a.refused = refused;
   a.Hkv = Hkv, a.group = Hq / Hkv, a.rows = (int)rows, a.seqs = (int)seqs;
   a.scale = kLog2e / sqrtf((float)kD);
-  // Tiles once they make up a workgroup for every CU: 2048 rows of 32 heads take
-  // 68 us in tiles and 79 us in 32 rows a workgroup, 1024 rows 37 and 30 us.
+  // Tiles once they make up a workgroup for every CU: one prompt of 512 / 1024 / 1536
+  // / 2048 rows of 32 heads takes 22 / 36 / 49 / 64 us in tiles and 16 / 34 / 57 / 87
+  // us in 32 rows a workgroup; 2048 rows in 16 / 64 prompts 17 / 13 and 33 / 29 us,
+  // 8192 in 512 73 and 108 us.
   const bool tiles = rows * Hq / kTileRows >= kTileSlots / 2;
   a.grid = (int)(rows * a.group / (tiles ? kTileRows : kFewRows) + seqs);
   const unsigned grid = (unsigned)((int64_t)a.grid * Hkv);

@@ -175,7 +175,8 @@ def paged_plan(batch: PagedBatch, cached, new, release=None):
     pages it owns (int32 [max_seqs] each).  Allocates pages, and fills
     ``starts``, ``lengths`` (cached + new), ``slots`` and ``positions``.  A
     step that does not fit sets ``refused``, changes no page and is planned
-    empty.  The inputs are read by the launch alone."""
+    empty.  The inputs are read by the launch alone.  To plan a step a second
+    time, leave ``release`` out: it would give the new pages back as well."""
     dev = batch.device
     _ints(cached, batch.max_seqs, "cached", dev)
     _ints(new, batch.max_seqs, "new", dev)
@@ -241,7 +242,8 @@ def ragged_attention(q, k, v, starts, out, refused=None):
     cache: sequence s has rows [starts[s], starts[s + 1]) (int32, on the
     device, ascending) of q [N, Hq, 128] and k, v [N, Hkv, 128] (bf16, e.g.
     slices of a fused projection's output), Hq a multiple of Hkv; row t reads
-    rows 0..t of its sequence.  out: bf16 [N, Hq * 128] or [N, Hq, 128], rows
+    rows 0..t of its sequence.  Probabilities are rounded to bf16 once from
+    49152 (N * Hq) on, and kept to 2^-15 below.  out: bf16 [N, Hq * 128] or [N, Hq, 128], rows
     outside every sequence left as they were.  ``refused`` (a refusal_flag()):
     set by starts that are not ascending or outside [0, N], whose rows are
     incomplete.  Returns ``out``."""

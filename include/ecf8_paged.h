@@ -81,7 +81,8 @@ int64_t ecf8_paged_work_bytes(int64_t seqs, int64_t rows, int Hq, int Hkv);
  * table row, more rows than `rows`, too few free pages) sets `refused`,
  * changes neither table, owned nor the stack, and plans an empty step: starts
  * and lengths zero, every slot -1.  A step planned again with the same lengths
- * takes no further pages.
+ * takes no further pages; with release set again, its sequences' pages go back and
+ * others come, and what was written to them since is lost.
  */
 int ecf8_paged_plan(const ecf8_paged_batch *batch, const int *cached, const int *new_tokens,
                     const int *release, void *stream);
@@ -131,8 +132,9 @@ int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t rows,
  * [starts[s], starts[s + 1]) (starts: device int32 [seqs + 1], ascending) of
  * q [rows, Hq, 128] and k, v [rows, Hkv, 128] (bf16, row strides in
  * elements, multiples of 8); query t reads rows 0..t of its own sequence.
- * Numerics and out as above.  Rows outside every sequence are left as they
- * were.
+ * Numerics and out as above, but for the probabilities: rounded to bf16 once in
+ * calls of 49152 (rows * Hq) and more, in two parts in smaller ones.  Rows outside
+ * every sequence are left as they were.
  */
 int ecf8_ragged_attention(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                           const void *v, int64_t v_stride, int64_t rows, const int *starts,
