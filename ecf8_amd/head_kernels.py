@@ -68,11 +68,14 @@ def refusal_flag() -> torch.Tensor:
     return torch.zeros(1, dtype=torch.int32, device="cpu", pin_memory=torch.cuda.is_available())
 
 
-def _flag_ptr(refused):
+def _flag_ptr(refused, dev):
     if refused is None:
         return None
-    if refused.dtype != torch.int32 or not (refused.is_cuda or refused.is_pinned()):
-        raise ECF8Error("refused must be int32 in pinned host or device memory")
+    if refused.dtype != torch.int32 or not (
+            refused.device == dev if refused.is_cuda else refused.is_pinned()):
+        raise ECF8Error(f"refused must be int32 in pinned host memory or on {dev}")
+    if refused.numel() < 1:
+        raise ECF8Error("refused must hold a value")
     return refused.data_ptr()
 
 
@@ -93,7 +96,7 @@ def greedy_emit(logits, work, tokens, next_token, step, pos=None, advance: int =
         check(lib().ecf8_greedy_emit_checked(
             logits.data_ptr(), logits.stride(0), B, V, work.data_ptr(), work.numel() * 8,
             tokens.data_ptr(), tokens.shape[1], next_token.data_ptr(), step.data_ptr(),
-            pos.data_ptr() if advance else None, advance, _flag_ptr(refused),
+            pos.data_ptr() if advance else None, advance, _flag_ptr(refused, dev),
             torch.cuda.current_stream(dev).cuda_stream), "ecf8_greedy_emit")
 
 
@@ -109,5 +112,5 @@ def embed_rows(token, table, out, refused=None):
         raise ECF8Error("out does not fit the embedded rows")
     with torch.cuda.device(dev):
         check(lib().ecf8_embed_rows_checked(
-            token.data_ptr(), B, table.data_ptr(), V, H, out.data_ptr(), _flag_ptr(refused),
+            token.data_ptr(), B, table.data_ptr(), V, H, out.data_ptr(), _flag_ptr(refused, dev),
             torch.cuda.current_stream(dev).cuda_stream), "ecf8_embed_rows")

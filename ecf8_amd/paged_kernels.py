@@ -261,5 +261,5 @@ def ragged_attention(q, k, v, starts, out, refused=None):
         raise ECF8Error("starts must hold the sequences' first rows and the end")
     _launch("ecf8_ragged_attention_checked", dev, q.data_ptr(), strides[0], k.data_ptr(), strides[1],
             v.data_ptr(), strides[2], N, starts.data_ptr(), starts.numel() - 1, Hq, Hkv,
-            out.data_ptr(), os, _flag_ptr(refused))
+            out.data_ptr(), os, _flag_ptr(refused, dev))
     return out

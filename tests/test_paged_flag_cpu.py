@@ -27,7 +27,8 @@ def test_flags_of_other_kinds_are_refused():
     from ecf8_amd._lib import ECF8Error
     from ecf8_amd.head_kernels import _flag_ptr
 
-    assert _flag_ptr(None) is None
+    dev = torch.device("cuda", 0)
+    assert _flag_ptr(None, dev) is None
     for flag in (torch.zeros(1, dtype=torch.int64), torch.zeros(1, dtype=torch.int32)):
         with pytest.raises(ECF8Error):
-            _flag_ptr(flag)
+            _flag_ptr(flag, dev)

@@ -166,3 +166,15 @@ def test_packed_starts_out_of_order_are_refused(cuda_device, starts, bad, Hq):
         ragged_attention(*parts, _ints(starts, dev), out)  # without a flag
         torch.cuda.synchronize()
         assert int(flag) == 0
+
+
+def test_flags_of_other_devices_and_empty_ones_are_refused(cuda_device):
+    from ecf8_amd.head_kernels import _flag_ptr, refusal_flag
+
+    flag = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    assert _flag_ptr(flag, flag.device) == flag.data_ptr()
+    assert _flag_ptr(refusal_flag(), flag.device)
+    for bad, dev in ((flag, torch.device("cuda", 1)), (flag[:0], flag.device),
+                     (refusal_flag()[:0], flag.device), (flag.cpu(), flag.device)):
+        with pytest.raises(ECF8Error):
+            _flag_ptr(bad, dev)
