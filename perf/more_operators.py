@@ -248,8 +248,11 @@ def prepare(case: dict, seed: int):
         s.kept = _ints([len(p) for p in paths])
         s.path = _ints([p + [-1] * (s.nodes - len(p)) for p in paths])
         if own:  # as draft_verify leaves them
+            from ecf8_amd.draft_kernels import KeepPlan
+
             s.trees.kept.copy_(s.kept)
             s.trees.path.copy_(s.path)
+            s.keep = KeepPlan(s.trees, s.layers)
         return s
     s.kp, s.vp = pools(2)
     s.ks = s.vs = None
@@ -423,7 +426,7 @@ def run(state):
         t = s.trees
         K.draft_verify(t, s.tokens, s.target, s.accept, s.sample, draft=s.draft)
         return {"kept": t.kept, "path": t.path, "emitted": t.emitted, "next": t.next_token}
-    K.draft_keep(s.trees, s.layers)
+    K.draft_keep(s.keep)
     return s.pools
 
 
