@@ -208,8 +208,9 @@ def prepare(case: dict, seed: int):
         return s
     if kind == "verify":
         N, V = s.rows, case["vocab"]
-        logits = _normal(N, V, gen=gen, scale=3.0, dtype=torch.float32)
-        guess = 0.95 * logits + _normal(N, V, gen=gen, scale=0.6, dtype=torch.float32)
+        # few tokens have most of the probability, and the drafter's are near them
+        logits = _normal(N, V, gen=gen, scale=6.0, dtype=torch.float32)
+        guess = 0.95 * logits + _normal(N, V, gen=gen, scale=0.8, dtype=torch.float32)
         s.target = torch.softmax(logits, -1)
         s.draft = torch.softmax(guess, -1)
         del logits
