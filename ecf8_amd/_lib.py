@@ -118,6 +118,16 @@ _SIGNATURES = {
                                _i64, _vp], _i32),
     "ecf8_ragged_attention_checked": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32,
                                        _i32, _vp, _i64, _vp, _vp], _i32),
+    # include/ecf8_draft.h: trees of drafted tokens
+    "ecf8_draft_work_bytes": ([_i64, _i64, _i32, _i32, _i32, _i32], _i64),
+    "ecf8_draft_plan": ([_vp, _vp, _vp, _i64, _vp], _i32),
+    "ecf8_draft_attention": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
+                             _i32),
+    "ecf8_probability_work_bytes": ([_i64], _i64),
+    "ecf8_token_probabilities": ([_vp, _i64, _i64, _i64, _vp, _f32, _vp, _i64, _vp, _i64, _vp],
+                                 _i32),
+    "ecf8_draft_verify": ([_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp], _i32),
+    "ecf8_draft_keep": ([_vp, _vp, _vp, _i32, _i32, _vp], _i32),
 }
 
 EXPORTED = tuple(_SIGNATURES)

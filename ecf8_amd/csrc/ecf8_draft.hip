@@ -1,0 +1,991 @@
+// Speculative decoding on gfx950, but for the trees' attention: the trees' masks,
+// positions and schedule, the target's probabilities, their verification and
+// the move of the accepted rows in the cache.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ecf8.h"
+#include "ecf8_dev.h"
+#include "ecf8_draft.h"
+#include "ecf8_draft_layout.h"
+
+namespace {
+
+using namespace ecf8::draft;
+using ecf8::paged::kMaxSeqs;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+// the same at any address of their elements
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef v4f v4f_any __attribute__((aligned(4)));
+
+__device__ __forceinline__ float bf16_f32(uint32_t h16) { return __uint_as_float(h16 << 16); }
+
+// --------------------------------------------------------------- the plan
+
+struct Plan {
+  const int *starts, *lengths, *parents;
+  uint64_t *masks;
+  int *out_parents, *positions, *refused;
+  Counts *counts;
+  Item *items;
+  Join *joins;
+  int seqs, rows, all_rows, group, max_nodes, max_children, tile, target, least;
+  uint64_t stamp;
+};
+
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kPer = kMaxSeqs / kPlanThreads;
+
+// The exclusive prefix sums of N values over the workgroup, and their totals.
+// Calls in a row alternate between two halves of `waves`.
+template <int N>
+__device__ __forceinline__ void block_scan(const int (&v)[N], int (*waves)[kPlanWaves],
+                                           int (&before)[N], int (&total)[N]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int inc[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    inc[x] = ecf8::dev::wave_inclusive_scan(v[x]);
+    if (lane == 63) waves[x][wave] = inc[x];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    before[x] = inc[x] - v[x], total[x] = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int t = waves[x][w];
+      if (w < wave) before[x] += t;
+      total[x] += t;
+    }
+  }
+}
+
+// A wave's tree: lane t is row t.  A row's mask is the union of the parents' on
+// the way up, in six doublings.
+__device__ __forceinline__ void plan_tree(const Plan &a, int s) {
+  const int lane = threadIdx.x & 63;
+  const int start = a.starts[s], n = a.starts[s + 1] - start;
+  if (n <= 0) return;
+  const int cached = a.lengths[s] - n;
+  if (n > a.max_nodes || start < 0 || start > a.rows - n || cached < 0) {
+    for (int t = lane; t < n; t += 64)
+      if (start >= 0 && start + t < a.all_rows) {
+        a.masks[start + t] = 0;
+        a.out_parents[start + t] = -1;
+      }
+    if (lane == 0 && a.refused) *a.refused = 1;
+    return;
+  }
+  int up = lane < n ? a.parents[start + lane] : -1;
+  bool bad = lane < n && (lane ? up < 0 || up >= lane : up != -1);
+  int before = 0;  // earlier rows of the same parent
+  for (int k = 0; k < n; ++k) before += k < lane && __builtin_amdgcn_readlane(up, k) == up;
+  bad |= lane > 0 && lane < n && before >= a.max_children;
+  if (__any(bad)) {
+    up = -1;
+    if (lane == 0 && a.refused) *a.refused = 1;
+  }
+  const int parent = up;
+  uint64_t bits = 1ull << lane;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    const uint64_t above = __shfl(bits, up & 63);
+    const int next = __shfl(up, up & 63);
+    if (up >= 0) bits |= above, up = next;
+  }
+  if (lane < n) {
+    a.masks[start + lane] = bits;
+    a.out_parents[start + lane] = parent;
+    a.positions[start + lane] = cached + __popcll(bits) - 1;
+  }
+}
+
+// Buckets of lengths, the longest first.
+constexpr int kBuckets = 64;
+__device__ __forceinline__ int bucket_of(int length, int share) {
+  return kBuckets - 1 - min(kBuckets - 1, (int)(48ll * length / share));
+}
+
+// The attention's schedule, by one workgroup.  Every (sequence, tile of rows)
+// has ceil(length / kUnitKeys) units; laid end to end they are cut at the
+// multiples of a workgroup's share (where `least` units are left on both
+// sides), and the pieces listed from the longest on.
+__device__ __forceinline__ void plan_schedule(const Plan &a) {
+  __shared__ int s_first[kMaxSeqs + 1];  // tiles before a sequence's
+  __shared__ int s_waves[2][2][kPlanWaves];
+  __shared__ int s_bucket[kBuckets];
+  const int tid = threadIdx.x, S = a.seqs;
+  const int step = (S + kPlanThreads - 1) / kPlanThreads;
+  if (tid < kBuckets) s_bucket[tid] = 0;
+  int tiles[kPer], sum = 0, units = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = step * tid + i;
+    tiles[i] = 0;
+    if (i >= step || s >= S) continue;
+    const int start = a.starts[s], n = a.starts[s + 1] - start, len = a.lengths[s];
+    if (n < 1 || n > a.max_nodes || start < 0 || start > a.rows - n || len < n) continue;
+    tiles[i] = (n * a.group + a.tile - 1) / a.tile;
+    sum += tiles[i];
+    units += tiles[i] * ((len + kUnitKeys - 1) / kUnitKeys);
+  }
+  // (the sum of all can pass 32 bits, a thread's cannot)
+  const int one[1] = {sum}, halves[2] = {units & 0xffff, units >> 16};
+  int at[1], n_tiles[1], skip[2], all[2];
+  block_scan(one, s_waves[0], at, n_tiles);
+  block_scan(halves, s_waves[1], skip, all);
+  const int64_t exact = (((int64_t)all[1] << 16) + all[0] + a.target - 1) / a.target;
+  const int share = (int)min(max(exact, (int64_t)(2 * a.least)), (int64_t)1 << 29);
+  {
+    int first = at[0];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int s = step * tid + i;
+      if (i < step && s < S) s_first[s] = first;
+      first += tiles[i];
+    }
+    if (tid == 0) s_first[S] = n_tiles[0];
+  }
+  __syncthreads();
+  int n_items = 0, n_joins = 0;
+  // Twice over the tiles: count the pieces of each length, then write them.
+  for (int write = 0; write < 2; ++write) {
+    int from0 = 0, parts = 0;  // from0: mod share
+    n_joins = 0;
+    for (int i0 = 0; i0 < n_tiles[0]; i0 += kPlanThreads) {  // uniform
+      const int i = i0 + tid;
+      Item it{};
+      int len = 0, mine[1] = {0};
+      if (i < n_tiles[0]) {
+        int lo = 0, hi = S;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_first[mid] <= i) lo = mid;
+          else hi = mid;
+        }
+        it.seq = lo, it.row0 = (i - s_first[lo]) * a.tile;
+        it.start = a.starts[lo], it.n = a.starts[lo + 1] - it.start;
+        len = a.lengths[lo], it.cached = len - it.n;
+        mine[0] = (len + kUnitKeys - 1) / kUnitKeys;
+      }
+      int from[1], total[1];
+      block_scan(mine, s_waves[0], from, total);
+      const int f = from0 + from[0];
+      const int c0 = (f + a.least + share - 1) / share, c1 = (f + mine[0] - a.least) / share;
+      const int k = mine[0] ? max(0, c1 - c0 + 1) + 1 : 0;
+      const int cut[2] = {k > 1 ? k : 0, k > 1};
+      int p[2], all_cut[2];
+      block_scan(cut, s_waves[1], p, all_cut);
+      p[0] += parts, p[1] += n_joins;
+      for (int j = 0; j < k; ++j) {
+        const int u0 = j ? (c0 + j - 1) * share - f : 0;
+        const int u1 = j + 1 < k ? (c0 + j) * share - f : mine[0];
+        const int to = atomicAdd(&s_bucket[bucket_of(u1 - u0, share)], 1);
+        if (write) {
+          it.k0 = u0 * kUnitKeys, it.k1 = min(u1 * kUnitKeys, len);
+          it.part = k > 1 ? p[0] + j : -1;
+          a.items[to] = it;
+        }
+      }
+      if (write && k > 1) a.joins[p[1]] = Join{it.row0, p[0], k, it.start, it.n, {it.seq, it.cached, 0}};
+      parts += all_cut[0], n_joins += all_cut[1];
+      from0 = (from0 + total[0]) % share;
+    }
+    __syncthreads();
+    if (!write) {
+      const int count[1] = {tid < kBuckets ? s_bucket[tid] : 0};
+      int first[1], total[1];
+      block_scan(count, s_waves[0], first, total);
+      if (tid < kBuckets) s_bucket[tid] = first[0];
+      n_items = total[0];
+      __syncthreads();
+    }
+  }
+  if (tid == 0) *a.counts = Counts{n_items, n_joins, a.stamp};
+}
+
+// The first workgroup schedules, the others take 16 sequences' trees each.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
+  if (blockIdx.x == 0) {
+    plan_schedule(a);
+  } else {
+    const int s = ((int)blockIdx.x - 1) * kPlanWaves + (int)(threadIdx.x >> 6);
+    if (s < a.seqs) plan_tree(a, s);
+  }
+}
+
+// -------------------------------------------------------- probabilities
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) less that
+constexpr float kLn2 = 0.69314718f;
+
+struct Probs {
+  const uint16_t *logits;
+  float *out;
+  const float *temperature;
+  int64_t ld, ldo;
+  uint2 *work;  // [rows, kChunks]
+  float common;
+  int V, chunks;
+};
+
+// 1 / temperature times log2(e), in two parts.
+struct Scale {
+  float hi, lo;
+  bool greedy;
+  __device__ __forceinline__ explicit Scale(float t) {
+    greedy = t <= 0.f;
+    hi = fminf(kLog2e / t, 0x1p100f);
+    if (t != t) hi = t;
+    lo = (fmaf(-hi, t, kLog2e) + kLog2eLow) / t;
+    if (!(fabsf(lo) < 0x1p80f)) lo = 0.f;
+  }
+  // exp(x / temperature), x <= 0; what the product's rounding lost is added
+  __device__ __forceinline__ float exp(float x) const {
+    const float e = x * hi;
+    const float rest = fmaf(x, lo, fmaf(x, hi, -e));
+    const float y = __builtin_amdgcn_exp2f(e);
+    // (rest is no number where x / temperature is infinite: y is 0)
+    return y > 0.f ? fmaf(y * kLn2, rest, y) : y;
+  }
+};
+
+// Sort key of a logit at index i as in ecf8_greedy_emit: larger is better, NaN
+// above everything, equal values to the lower index.
+__device__ __forceinline__ uint64_t logit_key(uint32_t h, uint32_t i) {
+  uint32_t k;
+  if ((h & 0x7fffu) > 0x7f80u) k = 0x1ffffu;
+  else if ((h & 0x7fffu) == 0) k = 0x8000u;
+  else k = h & 0x8000u ? 0x8000u - (h & 0x7fffu) : 0x8000u + h;
+  return ((uint64_t)k << 32) | (uint32_t)~i;
+}
+
+// Eight logits from element i on; past the row's end -inf.
+__device__ __forceinline__ u32x4 load_logits(const uint16_t *row, int i, int V) {
+  if (i + 8 <= V) return *reinterpret_cast<const u32x4_any *>(row + i);
+  u32x4 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t h = i + j < V ? row[i + j] : 0xff80u;
+    v[j >> 1] = j & 1 ? v[j >> 1] | h << 16 : h;
+  }
+  return v;
+}
+
+__device__ __forceinline__ float at8(u32x4 v, int j) {
+  return j & 1 ? __uint_as_float(v[j >> 1] & 0xffff0000u) : bf16_f32(v[j >> 1] & 0xffffu);
+}
+
+// The largest logit of a run of a row and the sum of the exponentials below it;
+// greedy rows: the best key.
+__global__ __launch_bounds__(256) void probability_stats_kernel(Probs a) {
+  __shared__ uint64_t s_k[4];
+  __shared__ float s_m[4], s_l[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.y, units = (a.V + 7) / 8, per = (units + a.chunks - 1) / a.chunks;
+  const uint16_t *x = a.logits + (int64_t)row * a.ld;
+  const Scale c(a.temperature ? a.temperature[row] : a.common);
+  const int u0 = blockIdx.x * per, u1 = min(u0 + per, units);
+  uint2 *out = a.work + (size_t)row * ECF8_PROBABILITY_CHUNKS + blockIdx.x;
+  if (c.greedy) {  // uniform
+    uint64_t best = 0;
+    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
+      const u32x4 v = load_logits(x, 8 * u, a.V);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint64_t k = logit_key((v[j >> 1] >> (16 * (j & 1))) & 0xffffu, 8 * u + j);
+        best = k > best ? k : best;
+      }
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t k = __shfl_xor(best, o);
+      best = k > best ? k : best;
+    }
+    if (lane == 0) s_k[wave] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 4; ++i) best = s_k[i] > best ? s_k[i] : best;
+      *out = make_uint2((uint32_t)best, (uint32_t)(best >> 32));
+    }
+    return;
+  }
+  float m = -INFINITY, l = 0.f;
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
+    const u32x4 v = load_logits(x, 8 * u, a.V);
+    float top = at8(v, 0);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, at8(v, j));
+    if (top > m) {
+      l *= m == -INFINITY ? 0.f : c.exp(m - top);
+      m = top;
+    }
+    const float from = m == -INFINITY ? 0.f : m;  // -inf from that: 0, NaN: NaN
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l += c.exp(at8(v, j) - from);
+  }
+  auto join = [&](float m2, float l2) {
+    const float top = fmaxf(m, m2);
+    if (top == -INFINITY) {
+      l += l2;
+    } else {
+      l = (m == -INFINITY ? l : l * c.exp(m - top)) + (m2 == -INFINITY ? l2 : l2 * c.exp(m2 - top));
+      m = top;
+    }
+  };
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o);
+    join(m2, l2);
+  }
+  if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 4; ++i) join(s_m[i], s_l[i]);
+    *out = make_uint2(__float_as_uint(m), __float_as_uint(l));
+  }
+}
+
+__global__ __launch_bounds__(256) void probability_kernel(Probs a) {
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.y, units = (a.V + 7) / 8, per = (units + a.chunks - 1) / a.chunks;
+  const uint16_t *x = a.logits + (int64_t)row * a.ld;
+  float *out = a.out + (int64_t)row * a.ldo;
+  const Scale c(a.temperature ? a.temperature[row] : a.common);
+  const int u0 = blockIdx.x * per, u1 = min(u0 + per, units);
+  const uint2 st = a.work[(size_t)row * ECF8_PROBABILITY_CHUNKS + min(lane, a.chunks - 1)];
+  if (c.greedy) {  // uniform
+    uint64_t best = ((uint64_t)st.y << 32) | st.x;
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t k = __shfl_xor(best, o);
+      best = k > best ? k : best;
+    }
+    const int at = (int)~(uint32_t)best;
+    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = 8 * u + 4 * h;
+        const v4f v = {i == at ? 1.f : 0.f, i + 1 == at ? 1.f : 0.f, i + 2 == at ? 1.f : 0.f,
+                       i + 3 == at ? 1.f : 0.f};
+        if (i + 4 <= a.V) *reinterpret_cast<v4f_any *>(out + i) = v;
+        else
+          for (int j = 0; j < 4; ++j)
+            if (i + j < a.V) out[i + j] = v[j];
+      }
+    return;
+  }
+  const float m0 = __uint_as_float(st.x);
+  float m = m0;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  // (lanes past the last run: nothing)
+  float l = lane >= a.chunks ? 0.f : __uint_as_float(st.y);
+  if (m0 != -INFINITY) l *= c.exp(m0 - m);
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  const float inv = 1.f / l;
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
+    const u32x4 v = load_logits(x, 8 * u, a.V);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 8 * u + 4 * h;
+      v4f p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = c.exp(at8(v, 4 * h + j) - m) * inv;
+      if (i + 4 <= a.V) *reinterpret_cast<v4f_any *>(out + i) = p;
+      else
+        for (int j = 0; j < 4; ++j)
+          if (i + j < a.V) out[i + j] = p[j];
+    }
+  }
+}
+
+// --------------------------------------------------------- verification
+
+struct Verify {
+  const int *starts, *parents;
+  const int64_t *tokens;
+  const float *target, *draft, *accept, *sample;
+  int64_t ld_target, ld_draft;
+  int *kept, *path, *refused;
+  int64_t *emitted, *next_token;
+  double *runs, *mass;  // [2, seqs, kRuns], [max_children - 1, nodes, kRuns]
+  int64_t nodes;
+  int seqs, rows, V, max_nodes, max_children, packed, per;
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// What a wave knows of a sequence's tree, lane t of row t.
+struct Tree {
+  int start, n, up, rank;  // rank: earlier rows of the same parent
+  int64_t token;
+  bool in;                 // the token is one of the vocabulary
+  double u, p, q;          // q, p: of the token, after the parent
+  uint64_t kids, above;    // children; ancestors and itself
+};
+
+// false: nothing to verify.
+template <bool kDrawn>
+__device__ __forceinline__ bool load_tree(const Verify &a, int s, Tree &t) {
+  const int lane = threadIdx.x & 63;
+  t.start = a.starts[s], t.n = a.starts[s + 1] - t.start;
+  if (t.n < 1 || t.n > a.max_nodes || t.start < 0 || t.start > a.rows - t.n) return false;
+  const int row = t.start + min(lane, t.n - 1);
+  t.up = lane < t.n ? a.parents[row] : -1;
+  if (t.up >= lane) t.up = -1;  // (of a plan that was never made)
+  t.token = a.tokens[row];
+  t.in = t.token >= 0 && t.token < a.V;
+  t.u = (double)a.accept[row];
+  const int64_t after = t.start + max(t.up, 0), c = t.in ? t.token : 0;
+  t.p = t.in ? (double)a.target[after * a.ld_target + c] : 0.0;
+  t.q = kDrawn && t.in ? (double)a.draft[after * a.ld_draft + c] : 0.0;
+  t.kids = 0, t.rank = 0;
+  for (int k = 1; k < t.n; ++k) {
+    const int up = __builtin_amdgcn_readlane(t.up, k);
+    if (up == lane) t.kids |= 1ull << k;
+    t.rank += k < lane && up == t.up;
+  }
+  t.above = 1ull << lane;
+  int up = t.up;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    const uint64_t more = __shfl(t.above, up & 63);
+    const int next = __shfl(up, up & 63);
+    if (up >= 0) t.above |= more, up = next;
+  }
+  return true;
+}
+
+// Where the walk ends: the last accepted row and its rejected children.
+struct End {
+  int last;
+  uint64_t gone;
+};
+
+// Drafts that are different tokens: what is left of w is Z less the rejected.
+__device__ __forceinline__ End walk_top(const Tree &t) {
+  End e{0, 0};
+  for (;;) {
+    uint64_t kids = __shfl(t.kids, e.last);
+    double mass = 1.0;
+    e.gone = 0;
+    int next = -1;
+    while (kids) {
+      const int j = __builtin_ctzll(kids);
+      kids &= kids - 1;
+      const int64_t c = __shfl(t.token, j);
+      // (a token that was rejected is not left)
+      const bool twice = __any(((e.gone >> (threadIdx.x & 63)) & 1) && t.token == c);
+      const double w = twice ? 0.0 : __shfl(t.p, j), u = __shfl(t.u, j);
+      if (u * mass < w) {
+        next = j;
+        break;
+      }
+      mass -= w;
+      e.gone |= 1ull << j;
+    }
+    if (next < 0) return e;
+    e.last = next;
+  }
+}
+
+// Drafts that were drawn.  Lane t tries row t's children as far as the sums Z of
+// `known` levels allow; s_inv[l][t]: 1 / Z after l rejections (l = 0: 1).  Sums
+// exist of rows that the walk could still reach when they were taken.  Returns
+// the rows that need the next level's, of those the walk can reach.
+struct Tried {
+  int next, gone;  // accepted child or -1; rejected children
+  bool open;       // children are left to be tried
+  bool reached;
+};
+__device__ __forceinline__ uint64_t try_drawn(const Verify &a, int s, const Tree &t, int known,
+                                              double (*s_inv)[64], Tried &r) {
+  const int lane = threadIdx.x & 63;
+  r = Tried{-1, 0, lane < t.n && t.kids != 0, false};
+  uint64_t left = t.kids;
+  double z = 1.0;
+  s_inv[0][lane] = 1.0;
+  for (int l = 0;; ++l) {
+    // child l of the rows that rejected all before it; all lanes take part in the
+    // exchange
+    const int j = left ? __builtin_ctzll(left) : 0;
+    const double u = __shfl(t.u, j), q = __shfl(t.q, j);
+    double w = __shfl(t.p, j);
+    if (r.open) {
+      for (int x = 0; x < l; ++x) w = fmax(fma(w, s_inv[x][lane], -q), 0.0);
+      if (u * q * z < w) {
+        r.next = j, r.open = false;
+      } else {
+        left &= left - 1, ++r.gone;
+        r.open = left != 0;
+      }
+    }
+    const bool up_open = __shfl((int)r.open, t.up & 63);
+    const int up_next = __shfl(r.next, t.up & 63), up_gone = __shfl(r.gone, t.up & 63);
+    const bool ok = lane == 0 || (lane < t.n && t.up >= 0 &&
+                                  (up_open ? t.rank >= up_gone : up_next == lane));
+    r.reached = lane < t.n && (t.above & ~__ballot(ok)) == 0;
+    const uint64_t need = __ballot(r.open && r.reached);
+    if (l == known || !need) return need;
+    for (uint64_t m = need; m; m &= m - 1) {
+      const int i = __builtin_ctzll(m);
+      const int64_t node = a.packed ? t.start + i : (int64_t)s * a.max_nodes + i;
+      const double sum = wave_sum(a.mass[(l * a.nodes + node) * kRuns + lane]);
+      if (lane == i) z = sum;
+    }
+    s_inv[l + 1][lane] = 1.0 / z;
+    if (r.open && !r.reached) r.open = false;  // nobody asks any more
+  }
+}
+
+__device__ __forceinline__ int run_length(int V) { return ((V + kRuns - 1) / kRuns + 3) / 4 * 4; }
+
+// w of four elements from v on (those at or past `end` are zero), for a row of
+// `gone` rejected children.
+__device__ __forceinline__ void left4(const float *p, const float *q, int v, int end, int gone,
+                                      const double *inv, double (&w)[4]) {
+  v4f pv = {}, qv = {};
+  if (v + 4 <= end) {
+    pv = *reinterpret_cast<const v4f_any *>(p + v);
+    if (gone) qv = *reinterpret_cast<const v4f_any *>(q + v);
+  } else {
+    for (int j = 0; j < 4; ++j)
+      if (v + j < end) {
+        pv[j] = p[v + j];
+        if (gone) qv[j] = q[v + j];
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = (double)pv[j];
+  for (int x = 0; x < gone; ++x) {
+    const double f = inv[x];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = fmax(fma(w[j], f, -(double)qv[j]), 0.0);
+  }
+}
+
+__device__ __forceinline__ double block_sum(double v, double *s) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// Level `level`: the sums of what `level` rejected children leave, by runs of
+// the vocabulary, of every row whose next child needs it.
+__global__ __launch_bounds__(256) void mass_kernel(Verify a, int level) {
+  extern __shared__ double s_dyn[];  // [level][64]
+  double(*s_inv)[64] = reinterpret_cast<double(*)[64]>(s_dyn);
+  __shared__ double s_sum[4], s_f[kMaxNodes];
+  __shared__ uint64_t s_need;
+  const int s = blockIdx.y;
+  Tree t;
+  if (!load_tree<true>(a, s, t)) return;
+  if (threadIdx.x < 64) {
+    Tried r;
+    const uint64_t need = try_drawn(a, s, t, level - 1, s_inv, r);
+    if (threadIdx.x == 0) s_need = need;
+  }
+  __syncthreads();
+  const int len = run_length(a.V);
+  for (uint64_t need = s_need; need; need &= need - 1) {
+    const int i = __builtin_ctzll(need);
+    __syncthreads();
+    if ((int)threadIdx.x < level) s_f[threadIdx.x] = s_inv[threadIdx.x][i];
+    __syncthreads();
+    const int64_t row = t.start + i;
+    const int64_t node = a.packed ? row : (int64_t)s * a.max_nodes + i;
+    for (int x = 0; x < a.per; ++x) {
+      const int run = blockIdx.x * a.per + x;
+      if (run >= kRuns) break;
+      const int64_t lo = (int64_t)run * len;
+      const int end = (int)min(lo + len, (int64_t)a.V);
+      double sum = 0.0;
+      for (int64_t v = lo + 4 * (int)threadIdx.x; v < end; v += 1024) {
+        double w[4];
+        left4(a.target + row * a.ld_target, a.draft + row * a.ld_draft, (int)v, end, level, s_f, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      sum = block_sum(sum, s_sum);
+      if (threadIdx.x == 0) a.mass[((level - 1) * a.nodes + node) * kRuns + run] = sum;
+    }
+  }
+}
+
+// The end of a sequence's walk, and what its last row's w is made of.
+struct Left {
+  int last, gone, n_tokens;  // gone: levels of drawn drafts; n_tokens: tokens that are gone
+  uint64_t path;
+};
+template <bool kDrawn>
+__device__ __forceinline__ bool find_end(const Verify &a, int s, Tree &t, double (*s_inv)[64],
+                                         double *s_f, int64_t *s_tokens, Left *s_left) {
+  if (!load_tree<kDrawn>(a, s, t)) return false;
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    Left e{0, 0, 0, 0};
+    if constexpr (kDrawn) {
+      Tried r;
+      try_drawn(a, s, t, a.max_children - 1, s_inv, r);
+      const uint64_t ends = __ballot(r.reached && r.next < 0);
+      e.last = ends ? __builtin_ctzll(ends) : 0;
+      e.gone = __shfl(r.gone, e.last);
+      if (lane < e.gone) s_f[lane] = s_inv[lane][e.last];
+    } else {
+      const End w = walk_top(t);
+      e.last = w.last;
+      e.n_tokens = __popcll(w.gone);
+      if ((w.gone >> lane) & 1) s_tokens[__popcll(w.gone & ((1ull << lane) - 1))] = t.token;
+    }
+    e.path = __shfl(t.above, e.last);
+    if (lane == 0) *s_left = e;
+  }
+  __syncthreads();
+  return true;
+}
+
+template <bool kDrawn>
+__device__ __forceinline__ void last4(const Verify &a, const Left &e, int64_t row, int v, int end,
+                                      const double *s_f, const int64_t *s_tokens, bool some,
+                                      double (&w)[4]) {
+  left4(a.target + row * a.ld_target, kDrawn ? a.draft + row * a.ld_draft : nullptr, v, end,
+        kDrawn ? e.gone : 0, s_f, w);
+  if (!kDrawn && some)
+    for (int x = 0; x < e.n_tokens; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (s_tokens[x] == v + j) w[j] = 0.0;
+}
+
+// The last row's w, and its target probabilities, summed by runs.
+template <bool kDrawn>
+__global__ __launch_bounds__(256) void last_kernel(Verify a) {
+  extern __shared__ double s_dyn[];  // [max_children][64]
+  __shared__ double s_sum[4], s_f[kMaxNodes];
+  __shared__ int64_t s_tokens[kMaxNodes];
+  __shared__ Left s_left;
+  const int s = blockIdx.y;
+  Tree t;
+  if (!find_end<kDrawn>(a, s, t, reinterpret_cast<double(*)[64]>(s_dyn), s_f, s_tokens, &s_left))
+    return;
+  const Left e = s_left;
+  const int64_t row = t.start + e.last;
+  const int len = run_length(a.V);
+  for (int x = 0; x < a.per; ++x) {
+    const int run = blockIdx.x * a.per + x;
+    if (run >= kRuns) break;
+    const int64_t lo = (int64_t)run * len;
+    const int end = (int)min(lo + len, (int64_t)a.V);
+    bool some = false;
+    for (int i = 0; i < e.n_tokens; ++i) some |= s_tokens[i] >= lo && s_tokens[i] < end;
+    double sum = 0.0, whole = 0.0;
+    for (int64_t v = lo + 4 * (int)threadIdx.x; v < end; v += 1024) {
+      double w[4], p[4];
+      left4(a.target + row * a.ld_target, nullptr, (int)v, end, 0, nullptr, p);
+      last4<kDrawn>(a, e, row, (int)v, end, s_f, s_tokens, some, w);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+      whole += (p[0] + p[1]) + (p[2] + p[3]);
+    }
+    sum = block_sum(sum, s_sum);
+    whole = block_sum(whole, s_sum);
+    if (threadIdx.x == 0) {
+      a.runs[(size_t)s * kRuns + run] = sum;
+      a.runs[(size_t)(a.seqs + s) * kRuns + run] = whole;
+    }
+  }
+}
+
+__device__ __forceinline__ double wave_scan(double v) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// The next token: the run that holds it, then the lane's elements, then the
+// element.  Then the outputs.
+template <bool kDrawn>
+__global__ __launch_bounds__(256) void pick_kernel(Verify a) {
+  extern __shared__ double s_dyn[];
+  __shared__ double s_sum[4], s_f[kMaxNodes], s_before, s_goal;
+  __shared__ int64_t s_tokens[kMaxNodes];
+  __shared__ Left s_left;
+  __shared__ int s_run, s_whole, s_at;
+  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int *path = a.path + (size_t)s * a.max_nodes;
+  int64_t *emitted = a.emitted + (size_t)s * a.max_nodes;
+  Tree t;
+  if (s == 0 && threadIdx.x == 0 && a.refused && a.starts[a.seqs] > a.rows) *a.refused = 1;
+  if (!find_end<kDrawn>(a, s, t, reinterpret_cast<double(*)[64]>(s_dyn), s_f, s_tokens, &s_left)) {
+    if ((int)threadIdx.x < a.max_nodes) path[threadIdx.x] = -1, emitted[threadIdx.x] = -1;
+    if (threadIdx.x == 0) {
+      a.kept[s] = 0, a.next_token[s] = -1;
+      if (t.n != 0 && a.refused) *a.refused = 1;
+    }
+    return;
+  }
+  const Left e = s_left;
+  if (threadIdx.x < 64) {
+    const double w = a.runs[(size_t)s * kRuns + lane];
+    const double p = a.runs[(size_t)(a.seqs + s) * kRuns + lane];
+    double upto = wave_scan(w);
+    double total = __shfl(upto, 63);
+    const bool whole = !(total > 0.0);
+    double mine = w;
+    if (whole) upto = wave_scan(p), total = __shfl(upto, 63), mine = p;
+    const double goal = fmax((double)a.sample[s], 0.0) * total;
+    const uint64_t over = __ballot(upto > goal), some = __ballot(mine > 0.0);
+    // (a sample of one or more: the last that there is)
+    const int run = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+    const double before = __shfl(upto, max(run - 1, 0));
+    if (lane == 0) {
+      s_run = total > 0.0 && total < INFINITY ? run : -1;
+      s_whole = whole, s_goal = goal, s_before = run > 0 ? before : 0.0, s_at = -1;
+    }
+  }
+  __syncthreads();
+  const int run = s_run;
+  if (run >= 0) {  // uniform
+    const int64_t row = t.start + e.last;
+    const int len = run_length(a.V), lo = run * len;  // (run has elements)
+    const int end = min(lo + len, a.V);
+    const int each = ((end - lo + 255) / 256 + 3) / 4 * 4;
+    const int v0 = min(lo + each * (int)threadIdx.x, end), v1 = min(v0 + each, end);
+    Left way = e;
+    if (s_whole) way.gone = way.n_tokens = 0;
+    double sum = 0.0;
+    for (int v = v0; v < v1; v += 4) {
+      double w[4];
+      last4<kDrawn>(a, way, row, v, v1, s_f, s_tokens, true, w);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    const double upto = wave_scan(sum);
+    if (lane == 63) s_sum[wave] = upto;
+    __syncthreads();
+    double before = s_before + (upto - sum);
+    for (int x = 0; x < wave; ++x) before += s_sum[x];
+    // The first element that passes the goal; where rounding leaves none, the last
+    // above zero.
+    int first = 0x7fffffff, last = -1;
+    for (int v = v0; v < v1; v += 4) {
+      double w[4];
+      last4<kDrawn>(a, way, row, v, v1, s_f, s_tokens, true, w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        before += w[j];
+        if (w[j] > 0.0) {
+          if (before > s_goal) first = min(first, v + j);
+          last = v + j;
+        }
+      }
+    }
+    __shared__ int s_first, s_last;
+    if (threadIdx.x == 0) s_first = 0x7fffffff, s_last = -1;
+    __syncthreads();
+    if (first != 0x7fffffff) atomicMin(&s_first, first);
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    if (threadIdx.x == 0) s_at = s_first != 0x7fffffff ? s_first : s_last;
+    __syncthreads();
+  }
+  if (threadIdx.x >= 64) return;
+  const int kept = __popcll(e.path);
+  const bool on = (e.path >> lane) & 1;
+  const int place = __popcll(e.path & ((1ull << lane) - 1));
+  if (on) {
+    path[place] = lane;
+    if (place > 0) emitted[place - 1] = t.token;
+  }
+  if (lane >= kept && lane < a.max_nodes) path[lane] = -1, emitted[lane] = -1;
+  const bool strange = __any(lane > 0 && lane < t.n && !t.in);
+  if (lane == 0) {
+    emitted[kept - 1] = s_at;
+    a.kept[s] = kept, a.next_token[s] = s_at;
+    if ((s_at < 0 || strange) && a.refused) *a.refused = 1;
+  }
+}
+
+// ------------------------------------------------------- the cache's rows
+
+constexpr int kKeepPools = 128;
+struct Keep {
+  const int *starts, *lengths, *table, *kept, *path;
+  int *refused;
+  int width, shift, Hkv, max_nodes, units, n, per;  // units: of 16 bytes a row
+  uint32_t pages;
+  uint8_t *pool[kKeepPools];
+};
+
+// Workgroup: one sequence, `per` (pool, head) pairs, a wave each in turn.  Rows
+// move to earlier places and no further than the row before them, so a wave that
+// takes them in order, 64 / units at a time, never reads what it has written.
+__global__ __launch_bounds__(256) void keep_kernel(Keep a) {
+  __shared__ uint32_t s_from[kMaxNodes], s_to[kMaxNodes];
+  const int s = blockIdx.y, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int start = a.starts[s], n = a.starts[s + 1] - start, cached = a.lengths[s] - n;
+  int kept = a.kept[s];
+  if (kept < 1) return;
+  const int row = lane < a.max_nodes ? a.path[(size_t)s * a.max_nodes + lane] : -1;
+  const int before = __shfl_up(row, 1);
+  const bool bad = lane < kept && (lane == 0 ? row != 0 : row <= before || row >= n);
+  const uint64_t wrong = __ballot(bad) | (kept > a.max_nodes ? 1ull << (a.max_nodes - 1) : 0) |
+                         (cached < 0 || n < 1 ? 1ull : 0);
+  if (wrong) {
+    kept = min(kept, (int)__builtin_ctzll(wrong));
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused) *a.refused = 1;
+  }
+  const uint64_t moves = __ballot(lane < kept && row != lane);
+  if (!moves) return;
+  const int first = __builtin_ctzll(moves), moved = kept - first;  // (and all after it)
+  if (threadIdx.x < 64 && lane >= first && lane < kept) {
+    auto slot = [&](int pos) {
+      const uint32_t page =
+          min((uint32_t)a.table[(size_t)s * a.width + min(pos >> a.shift, a.width - 1)], a.pages - 1);
+      return ((page * a.Hkv) << a.shift) + (uint32_t)(pos & ((1 << a.shift) - 1));
+    };
+    s_from[lane - first] = slot(cached + row);
+    s_to[lane - first] = slot(cached + lane);
+  }
+  __syncthreads();
+  const int unit = lane % a.units, sub = lane / a.units, step = 64 / a.units;
+  const int end = min((int)(blockIdx.x + 1) * a.per, a.n * a.Hkv);
+  for (int i = blockIdx.x * a.per + wave; i < end; i += 4) {
+    const uint32_t head = (uint32_t)(i % a.Hkv) << a.shift;
+    u32x4 *pool = reinterpret_cast<u32x4 *>(a.pool[i / a.Hkv]);
+    for (int r = sub; r < moved; r += step) {
+      const u32x4 v = pool[(size_t)(s_from[r] + head) * a.units + unit];
+      pool[(size_t)(s_to[r] + head) * a.units + unit] = v;
+    }
+  }
+}
+
+inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
+inline bool aligned(const void *p, uintptr_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+inline int launched() { return hipGetLastError() == hipSuccess ? ECF8_OK : ECF8_ERR_HIP; }
+
+Work layout_of(const ecf8_paged_batch *b, const ecf8_draft_trees *t) {
+  return work_layout(b->seqs, b->rows, b->Hq, b->Hkv, t->max_nodes, t->max_children);
+}
+
+}  // namespace
+
+extern "C" int64_t ecf8_draft_work_bytes(int64_t seqs, int64_t rows, int Hq, int Hkv,
+                                         int max_nodes, int max_children) {
+  return sizes_ok(seqs, rows, Hq, Hkv, max_nodes, max_children)
+             ? work_layout(seqs, rows, Hq, Hkv, max_nodes, max_children).bytes
+             : -1;
+}
+
+extern "C" int ecf8_draft_plan(const ecf8_paged_batch *b, const ecf8_draft_trees *t,
+                               const int *parents, int64_t rows, void *stream) {
+  if (!parents || rows <= 0) return ECF8_ERR_INVALID_ARG;
+  if (const int rc = check_trees(b, t)) return rc;
+  if (rows > b->rows) return ECF8_ERR_CAPACITY;
+  if (!aligned(parents, 4)) return ECF8_ERR_MISALIGNED;
+  const Work w = layout_of(b, t);
+  auto *base = static_cast<uint8_t *>(t->work);
+  const Plan a{b->starts, b->lengths, parents, t->masks, t->parents, b->positions, b->refused,
+               reinterpret_cast<Counts *>(base), reinterpret_cast<Item *>(base + w.items_at),
+               reinterpret_cast<Join *>(base + w.joins_at), b->seqs, (int)rows, b->rows, b->Hq / b->Hkv,
+               t->max_nodes, t->max_children, w.tile, w.target, 1, schedule_stamp(b, t)};
+  const unsigned grid = 1 + (unsigned)((b->seqs + kPlanWaves - 1) / kPlanWaves);
+  plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
+  return launched();
+}
+
+extern "C" int64_t ecf8_probability_work_bytes(int64_t rows) {
+  return rows <= 0 || rows > 65535 ? -1 : rows * ECF8_PROBABILITY_CHUNKS * 8;
+}
+
+extern "C" int ecf8_token_probabilities(const void *logits, int64_t ld, int64_t rows, int64_t V,
+                                        const float *temperature, float common, float *out,
+                                        int64_t ldo, void *work, int64_t work_bytes,
+                                        void *stream) {
+  if (!logits || !out || !work || rows <= 0 || V <= 0) return ECF8_ERR_INVALID_ARG;
+  if (rows > 65535 || V > (1 << 30) || (rows > 1 && ld < V)) return ECF8_ERR_UNSUPPORTED;
+  if ((rows > 1 && ldo < V) || work_bytes < ecf8_probability_work_bytes(rows))
+    return ECF8_ERR_CAPACITY;
+  if (!aligned(logits, 2) || !aligned(out, 4) || !aligned(temperature, 4) || !aligned(work, 8))
+    return ECF8_ERR_MISALIGNED;
+  const int64_t units = (V + 7) / 8;
+  int64_t chunks = 2048 / rows < 8 ? 8 : 2048 / rows;
+  if (chunks > ECF8_PROBABILITY_CHUNKS) chunks = ECF8_PROBABILITY_CHUNKS;
+  if (chunks > (units + 255) / 256) chunks = (units + 255) / 256;
+  const Probs a{static_cast<const uint16_t *>(logits), out, temperature, ld, ldo,
+                static_cast<uint2 *>(work), common, (int)V, (int)chunks};
+  const dim3 grid((unsigned)chunks, (unsigned)rows);
+  probability_stats_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
+  probability_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
+  return launched();
+}
+
+extern "C" int ecf8_draft_verify(const ecf8_paged_batch *b, const ecf8_draft_trees *t,
+                                 const int64_t *tokens, int64_t rows, const float *target,
+                                 int64_t ld_target, const float *draft, int64_t ld_draft,
+                                 int64_t V, const float *accept, const float *sample,
+                                 void *stream) {
+  if (!tokens || !target || !accept || !sample || rows <= 0 || V <= 0) return ECF8_ERR_INVALID_ARG;
+  if (const int rc = check_trees(b, t)) return rc;
+  if (rows > b->rows) return ECF8_ERR_CAPACITY;
+  if (V > (1 << 30) || (rows > 1 && (ld_target < V || (draft && ld_draft < V))))
+    return ECF8_ERR_UNSUPPORTED;
+  if (!aligned(tokens, 8) || !aligned(target, 4) || !aligned(draft, 4) || !aligned(accept, 4) ||
+      !aligned(sample, 4))
+    return ECF8_ERR_MISALIGNED;
+  const Work w = layout_of(b, t);
+  auto *base = static_cast<uint8_t *>(t->work);
+  Verify a{b->starts, t->parents, tokens, target, draft, accept, sample, ld_target, ld_draft,
+           t->kept, t->path, b->refused, t->emitted, t->next_token,
+           reinterpret_cast<double *>(base + w.runs), reinterpret_cast<double *>(base + w.mass),
+           w.nodes, b->seqs, (int)rows, (int)V, t->max_nodes, t->max_children, w.packed, 1};
+  const int64_t per = (int64_t)b->seqs * kRuns / 2048;
+  a.per = per < 1 ? 1 : per > 8 ? 8 : (int)per;
+  const dim3 grid((unsigned)((kRuns + a.per - 1) / a.per), (unsigned)b->seqs);
+  const unsigned lds = draft ? (unsigned)(t->max_children * 64 * sizeof(double)) : 0;
+  if (draft) {
+    for (int level = 1; level < t->max_children; ++level)
+      mass_kernel<<<grid, 256, lds, as_stream(stream)>>>(a, level);
+    last_kernel<true><<<grid, 256, lds, as_stream(stream)>>>(a);
+    pick_kernel<true><<<(unsigned)b->seqs, 256, lds, as_stream(stream)>>>(a);
+  } else {
+    last_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(a);
+    pick_kernel<false><<<(unsigned)b->seqs, 256, 0, as_stream(stream)>>>(a);
+  }
+  return launched();
+}
+
+extern "C" int ecf8_draft_keep(const ecf8_paged_batch *b, const ecf8_draft_trees *t,
+                               void *const *pools, int n_pools, int fp8, void *stream) {
+  if (!pools || n_pools <= 0) return ECF8_ERR_INVALID_ARG;
+  if (const int rc = check_trees(b, t)) return rc;
+  for (int i = 0; i < n_pools; ++i) {
+    if (!pools[i]) return ECF8_ERR_INVALID_ARG;
+    if (!aligned(pools[i], 16)) return ECF8_ERR_MISALIGNED;
+  }
+  Keep a{};
+  a.starts = b->starts, a.lengths = b->lengths, a.table = b->table;
+  a.kept = t->kept, a.path = t->path, a.refused = b->refused;
+  a.width = b->width, a.shift = __builtin_ctz((unsigned)b->page_size), a.Hkv = b->Hkv;
+  a.max_nodes = t->max_nodes, a.units = fp8 ? kD / 16 : kD / 8, a.pages = (uint32_t)b->pages;
+  for (int i0 = 0; i0 < n_pools; i0 += kKeepPools) {
+    a.n = n_pools - i0 < kKeepPools ? n_pools - i0 : kKeepPools;
+    for (int i = 0; i < a.n; ++i) a.pool[i] = static_cast<uint8_t *>(pools[i0 + i]);
+    const int64_t pairs = (int64_t)a.n * a.Hkv, each = pairs * b->seqs / 1024;
+    a.per = each < 4 ? 4 : (int)each;
+    const dim3 grid((unsigned)((pairs + a.per - 1) / a.per), (unsigned)b->seqs);
+    keep_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
+  }
+  return launched();
+}

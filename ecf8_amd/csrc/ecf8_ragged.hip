@@ -11,6 +11,7 @@
 
 #include "ecf8.h"
 #include "ecf8_dev.h"
+#include "ecf8_draft_layout.h"
 #include "ecf8_paged.h"
 #include "ecf8_paged_layout.h"
 
@@ -114,6 +115,8 @@ struct Attn {
   int grid;                                // item slots launched per KV head
   int max_new;                             // new tokens of a sequence
   float scale;                             // of the scores, times log2(e)
+  const uint64_t *masks;                   // trees: of the packed rows
+  const int *lengths;
 };
 
 enum Source { kPages, kPagesFp8, kPacked };
@@ -355,6 +358,20 @@ struct Rows {
           if (key0 + 16 * x + 4 * (lane >> 4) + i > limit[t]) s[t][x][i] = -INFINITY;
   }
 
+  // The lane's query of group t reads the keys of the set bits of word[t] only.
+  static __device__ __forceinline__ void mask_words(v4f (&s)[T][2], const uint32_t (&word)[T],
+                                                    int lane) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const uint32_t w = word[t] >> (4 * (lane >> 4));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(w >> (16 * x + i) & 1)) s[t][x][i] = -INFINITY;
+    }
+  }
+
   // Adds the infinities and NaNs of keys [first, end), whose values were
   // staged without them: each reaches the queries that read its position.
   // value(key, dim): four values of a key from dim on.  Rare.
@@ -374,6 +391,26 @@ struct Rows {
 #pragma unroll
           for (int t = 0; t < T; ++t)
             if (odd && key <= limit[t]) o[t][d][i] += x;
+        }
+      }
+  }
+  // The same of trees: reads(t, key) says which queries do.
+  template <class Value, class Reads>
+  __device__ __forceinline__ void add_odd_if(int first, int end, int lane, Value value,
+                                             Reads reads) {
+#pragma unroll 1
+    for (int key = first; key < end; ++key)
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const u32x2 v = value(key, 16 * d + 4 * (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x =
+              __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+          const bool odd = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+            if (odd && reads(t, key)) o[t][d][i] += x;
         }
       }
   }
@@ -534,6 +571,46 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
   }
 }
 
+// The item of slot `item` of a step's trees; false past the last, and where the
+// plan is another step's.
+__device__ __forceinline__ bool get_tree_item(const Attn &a, int item, Place &p) {
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused &&
+      (a.starts[a.seqs] > a.rows || *a.stamp != a.want_stamp))
+    *a.refused = 1;
+  const Item it = a.items[item];  // item < a.grid: in the list, filled or not
+  asm volatile("" ::"s"(it.seq), "s"(it.start));  // not after the wait for n_items
+  if (*a.stamp != a.want_stamp || item >= *a.n_items) return false;
+  if (a.starts[it.seq] != it.start || a.starts[it.seq + 1] != it.start + it.n ||
+      a.lengths[it.seq] != it.cached + it.n) {
+    if (threadIdx.x == 0 && a.refused) *a.refused = 1;
+    return false;
+  }
+  p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
+  p.start = it.start, p.n = it.n, p.cached = it.cached;
+  return true;
+}
+
+// The masks of the lane's queries, as load_queries has them.
+template <int T>
+__device__ __forceinline__ void load_masks(const Attn &a, int start, int row0, int end, int lane,
+                                           uint64_t (&bits)[T]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+    bits[t] = a.masks[min(start + min(row0 + 16 * t + (lane & 15), end - 1) / a.group, a.rows - 1)];
+}
+
+// Which of the 32 keys from key0 < end on a query of mask `bits` reads: the cached
+// ones, and the mask's of the rows after them.
+__device__ __forceinline__ uint32_t tree_word(uint64_t bits, int key0, int cached, int end) {
+  const int off = key0 - cached;
+  uint64_t w;
+  if (off <= -32) w = ~0ull;
+  else if (off <= 0) w = bits << -off | ((1ull << -off) - 1);
+  else w = off < 64 ? bits >> off : 0;
+  if (end - key0 < 32) w &= (1ull << (end - key0)) - 1;
+  return (uint32_t)w;
+}
+
 // Four bf16 of a sequence's value rows at (key, dim), as they lie in memory.
 template <Source kSrc>
 __device__ __forceinline__ u32x2 value4(const Attn &a, const Place &p, int kvh, int key, int dim) {
@@ -573,7 +650,9 @@ __device__ __forceinline__ void lds_barrier() {
 // two parts (kFine) at no cost.  With the join, these take 172 and 72 us; 195 and 82
 // if page loads go through the caches, which a page, read once, gains nothing from;
 // 173 and 78 with T = 2 where the step's rows allow 1.
-template <Source kSrc, int T>
+//
+// kTree: the step's trees (rows read the cached positions and their masks').
+template <Source kSrc, int T, bool kTree = false>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
   __shared__ float s_m[4][16 * T], s_l[4][16 * T];
@@ -588,9 +667,14 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const Operands ops(lane);
 
   Place p;
-  if (!get_item<kSrc>(a, 16 * T, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  if constexpr (kTree) {
+    if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
+  } else {
+    if (!get_item<kSrc>(a, 16 * T, (int)blockIdx.x / a.Hkv, p, lane)) return;
+  }
   const int n_rows = min(p.n * a.group - p.row0, 16 * T);
-  const int low = p.cached + p.row0 / a.group;  // the first query's limit
+  // the first query's limit, or what all read
+  const int low = kTree ? p.cached - 1 : p.cached + p.row0 / a.group;
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
@@ -607,8 +691,10 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   uint32_t at = locate(key0), next = locate(key0 + 128);
   v8bf q[T][4];
   int limit[T];
+  uint64_t bits[T];
   load_queries<T>(a, kvh, p.start, p.row0, p.row0 + n_rows, lane, q);
-  query_limits<T>(a, p.cached, p.row0, p.row0 + n_rows, lane, limit);
+  if constexpr (kTree) load_masks<T>(a, p.start, p.row0, p.row0 + n_rows, lane, bits);
+  else query_limits<T>(a, p.cached, p.row0, p.row0 + n_rows, lane, limit);
   u32x4 kr[kLoads], vr[kLoads];
   bool odd = false;
   auto load = [&](uint32_t at) {
@@ -679,15 +765,33 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
       v4f s[T][2];
       u32x4 pr[T];
       w.scores(ops, k, q, s);
-      if (masked) w.mask(s, key0, limit, lane);
+      if (masked) {
+        if constexpr (kTree) {
+          uint32_t word[T];
+#pragma unroll
+          for (int t = 0; t < T; ++t) word[t] = tree_word(bits[t], key0, p.cached, p.k1);
+          w.mask_words(s, word, lane);
+        } else {
+          w.mask(s, key0, limit, lane);
+        }
+      }
       w.weigh(s, c, pr, key0 == p.k0 + 32 * wave);
       w.second(ops, v, pr);
     }
     if (__any(odd))
       for (key0 = p.k0 + 32 * wave; key0 < p.k1; key0 += 128)
-        if (key0 + 31 > low)
-          w.add_odd(key0, min(key0 + 32, p.k1), limit, lane,
-                    [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
+        if (key0 + 31 > low) {
+          if constexpr (kTree)
+            w.add_odd_if(
+                key0, min(key0 + 32, p.k1), lane,
+                [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); },
+                [&](int t, int key) {
+                  return (tree_word(bits[t], key, p.cached, p.k1) & 1) != 0;
+                });
+          else
+            w.add_odd(key0, min(key0 + 32, p.k1), limit, lane,
+                      [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); });
+        }
   }
 
   // join the waves
@@ -733,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
     } else {
       const int g = p.row0 + row;
       const int tk = p.start + g / a.group;
-      const float inv = vscale / sum;
+      const float inv = kTree && sum == 0.f ? 0.f : vscale / sum;  // (a mask can be empty)
       if (tk < a.rows)
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
                                    (kvh * a.group + g % a.group) * kD + 4 * u) =
@@ -1025,7 +1129,7 @@ struct Joins {
 
 // The parts of split rows, joined: four dims a lane, kSplit halves of a wave a
 // row (each every kSplit-th part), four parts' loads at a time.
-template <int kSplit, int kPartRows>
+template <int kSplit, int kPartRows, bool kTree = false>
 __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int group) {
   __shared__ float s_top[8], s_l[8];
   __shared__ v4f s_sum[8][32];
@@ -1035,6 +1139,12 @@ __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int gr
   const Join jn = o.list[j];  // j: in the list, filled or not
   asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for the count
   if (*a.stamp != a.want_stamp || j >= *o.n) return;
+  if constexpr (kTree) {  // (pad: the sequence and its cached tokens)
+    const int seq = jn.pad[0];
+    if (a.starts[seq] != jn.start || a.starts[seq + 1] != jn.start + jn.tokens ||
+        a.lengths[seq] != jn.pad[1] + jn.tokens)
+      return;
+  }
   constexpr int part_rows = kPartRows;
   const int n_rows = min(jn.tokens * a.group - jn.row0, part_rows);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
@@ -1089,7 +1199,7 @@ __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int gr
       }
     }
     const int g = jn.row0 + row, tk = jn.start + g / a.group;
-    const float inv = vscale / l;
+    const float inv = kTree && l == 0.f ? 0.f : vscale / l;
     if ((kSplit == 1 ? row0 + half < n_rows : half == 0) && tk < a.rows)
       *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
                                  (kvh * a.group + g % a.group) * kD + 4 * lane) =
@@ -1104,6 +1214,221 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
   const int i = (int)blockIdx.x;
   if (i < few.groups) join_parts<8, kFewRows>(a, few, i);
   else join_parts<1, kTileRows>(a, tiles, i - few.groups);
+}
+
+// ------------------------------------------------------------ drafted trees
+
+// Workgroup of eight waves: up to 32 kWr rows (token, head of the group) of one
+// KV head against positions [k0, k1).  Waves of the same wave / kWr share a
+// slice of 32 keys, those of the same wave % kWr share 32 rows; all stage kSlices
+// slices a round through registers, kDepth rounds ahead, into LDS.
+template <Source kSrc, int kWr, int kSlices, int kDepth>
+__global__ __launch_bounds__(512) void tree_kernel(Attn a) {
+  constexpr int T = 2, kWk = 8 / kWr, kSteps = kSlices / kWk, kRows = 32 * kWr;
+  constexpr bool kFp8 = kSrc == kPagesFp8, kFine = kWr < 8;
+  constexpr int kUnits = kFp8 ? 8 : 16;  // 16-byte units of a row in memory
+  __shared__ u32x4 s_kv[2][kSlices][32 * (kKeyRow + kValueRow)];
+  __shared__ float s_m[4][16 * T], s_l[4][16 * T];
+  __shared__ int s_odd;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % kWr, wk = wave / kWr;
+  const int kvh = (int)blockIdx.x % a.Hkv;
+  const Operands ops(lane);
+
+  Place p;
+  if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
+  const int all_rows = min(p.n * a.group - p.row0, kRows);
+  const int n_rows = min(all_rows - 32 * wr, 32);
+  float c = a.scale, vscale = 1.f;
+  if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
+
+  // A thread stages a 16-byte unit of a row of every slice: of the keys and of the
+  // values, in e4m3 of one of them.
+  const int unit = (int)threadIdx.x % kUnits, sub = (int)(threadIdx.x / kUnits) & 31;
+  const bool keys = threadIdx.x < 256;
+  const int *table = a.table + (size_t)p.seq * a.width;
+  const int rounds = (p.k1 - p.k0 + 32 * kSlices - 1) / (32 * kSlices);
+  auto key_of = [&](int j, int i) { return min(p.k0 + 32 * (kSlices * j + i) + sub, p.k1 - 1); };
+  auto look = [&](int j, int (&entry)[kSlices]) {
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) entry[i] = table[key_of(j, i) >> a.shift];
+  };
+  constexpr int kLoads = kFp8 ? 1 : 2;
+  u32x4 r[kDepth][kSlices][kLoads];
+  auto load = [&](int j, const int (&entry)[kSlices], u32x4 (&r)[kSlices][kLoads]) {
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) {
+      const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
+      const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) +
+                                 (key_of(j, i) & ((1 << a.shift) - 1))) * kUnits + unit;
+      if constexpr (kFp8) {
+        r[i][0] = static_cast<const u32x4 *>(keys ? a.k : a.v)[at];
+      } else {
+        r[i][0] = static_cast<const u32x4 *>(a.k)[at];
+        r[i][1] = static_cast<const u32x4 *>(a.v)[at];
+      }
+    }
+  };
+  auto store = [&](int j, u32x4 (&r)[kSlices][kLoads]) {
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) {
+      u32x4 *s_k = s_kv[j & 1][i], *s_v = s_k + 32 * kKeyRow;
+      const bool masked = p.k0 + 32 * (kSlices * j + i) + 31 >= p.cached;  // uniform
+      auto finite = [&](u32x4 v) {
+        if (!masked) return v;
+        const u32x4 f = finite_or_zero(v);
+        if (differ(f, v)) s_odd = 1;
+        return f;
+      };
+      if constexpr (kFp8) {
+        u32x4 w[2];
+        widen16(r[i][0], w);
+        if (keys) {
+          s_k[sub * kKeyRow + 2 * unit] = w[0];
+          s_k[sub * kKeyRow + 2 * unit + 1] = w[1];
+        } else {
+          s_v[sub * kValueRow + 2 * unit] = finite(w[0]);
+          s_v[sub * kValueRow + 2 * unit + 1] = finite(w[1]);
+        }
+      } else {
+        s_k[sub * kKeyRow + unit] = r[i][0];
+        s_v[sub * kValueRow + unit] = finite(r[i][1]);
+      }
+    }
+  };
+
+  int first[kDepth + 1][kSlices], entry[kSlices];
+#pragma unroll
+  for (int x = 0; x <= kDepth; ++x) look(x, first[x]);
+  v8bf q[T][4];
+  uint64_t bits[T];
+  const int row0 = p.row0 + min(32 * wr, all_rows - 1), row_end = p.row0 + all_rows;
+  load_queries<T>(a, kvh, p.start, row0, row_end, lane, q);
+  load_masks<T>(a, p.start, row0, row_end, lane, bits);
+  if (threadIdx.x == 0) s_odd = 0;
+#pragma unroll
+  for (int x = 0; x < kDepth; ++x) load(x, first[x], r[x]);
+#pragma unroll
+  for (int i = 0; i < kSlices; ++i) entry[i] = first[kDepth][i];
+  __syncthreads();  // s_odd
+
+  Rows<T, kFine> w;
+  w.init();
+  auto round = [&](int j, u32x4 (&r)[kSlices][kLoads]) {
+    store(j, r);
+    if (j + kDepth < rounds) {  // uniform
+      int next[kSlices];
+      look(j + kDepth + 1, next);
+      load(j + kDepth, entry, r);
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) entry[i] = next[i];
+    }
+    // (the stage of round j + 1 was read in round j - 1, before this barrier)
+    lds_barrier();
+    if (n_rows <= 0) return;  // uniform
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int slice = st * kWk + wk, key0 = p.k0 + 32 * (kSlices * j + slice);
+      if (key0 >= p.k1) break;  // uniform
+      lds_u8 *k = (lds_u8 *)s_kv[j & 1][slice], *v = k + 32 * 16 * kKeyRow;
+      v4f s[T][2];
+      u32x4 pr[T];
+      w.scores(ops, k, q, s);
+      if (key0 + 31 >= p.cached) {
+        uint32_t word[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t) word[t] = tree_word(bits[t], key0, p.cached, p.k1);
+        w.mask_words(s, word, lane);
+      }
+      w.weigh(s, c, pr, j == 0 && st == 0);
+      w.second(ops, v, pr);
+    }
+  };
+#pragma unroll 1
+  for (int j = 0; j < rounds; j += kDepth) {
+#pragma unroll
+    for (int x = 0; x < kDepth; ++x)
+      if (j + x < rounds) round(j + x, r[x]);
+  }
+  __syncthreads();
+  if (s_odd && n_rows > 0)
+    for (int i = wk; p.k0 + 32 * i < p.k1; i += kWk) {
+      const int key0 = p.k0 + 32 * i;
+      if (key0 + 31 < p.cached) continue;
+      w.add_odd_if(
+          key0, min(key0 + 32, p.k1), lane,
+          [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); },
+          [&](int t, int key) { return (tree_word(bits[t], key, p.cached, p.k1) & 1) != 0; });
+    }
+  float l[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    l[t] = w.l[t][0];
+    if (l[t] == 0.f) w.m[t] = kLowest;
+  }
+  // join the slices' waves, half of them at a time; over the stages, which have been
+  // read
+  v4f *s_o = reinterpret_cast<v4f *>(&s_kv[0][0][0]);
+#pragma unroll
+  for (int half = kWk / 2; half > 0; half /= 2) {
+    const int at = (wk % half) * kWr + wr;  // below 4
+    if (half < kWk / 2) __syncthreads();
+    if (wk >= half && wk < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        if (lane < 16) s_m[at][16 * t + lane] = w.m[t], s_l[at][16 * t + lane] = l[t];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) s_o[(at * 16 + 8 * t + d) * 64 + lane] = w.o[t][d];
+      }
+    }
+    __syncthreads();
+    if (wk < half) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const float m = s_m[at][16 * t + (lane & 15)], top = fmaxf(m, w.m[t]);
+        const float f0 = __builtin_amdgcn_exp2f(w.m[t] - top), f1 = __builtin_amdgcn_exp2f(m - top);
+        l[t] = l[t] * f0 + s_l[at][16 * t + (lane & 15)] * f1;
+        w.m[t] = top;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const v4f o = s_o[(at * 16 + 8 * t + d) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[t][d][i] = w.o[t][d][i] * f0 + o[i] * f1;
+        }
+      }
+    }
+  }
+  if (wk != 0) return;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int row = 32 * wr + 16 * t + (lane & 15), g = lane >> 4;
+    if (row >= all_rows) continue;
+    if (p.part >= 0) {
+      const size_t at = ((size_t)p.part * a.Hkv + kvh) * kRows + row;
+      v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
+      if (g == 0) a.stats[at] = make_float2(w.m[t], l[t]);
+    } else {
+      const int at = p.row0 + row, tk = p.start + at / a.group;
+      const float inv = l[t] == 0.f ? 0.f : vscale / l[t];  // (a mask can be empty)
+      if (tk < a.rows) {
+        uint16_t *op = a.out + (int64_t)tk * a.out_stride +
+                       (kvh * a.group + at % a.group) * kD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          *reinterpret_cast<u32x2 *>(op + 16 * d) =
+              u32x2{pack_bf16(w.o[t][d][0] * inv, w.o[t][d][1] * inv),
+                    pack_bf16(w.o[t][d][2] * inv, w.o[t][d][3] * inv)};
+      }
+    }
+  }
+}
+
+template <int kRows>
+__global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o) {
+  join_parts<kRows <= 32 ? 8 : 1, kRows, true>(a, o, (int)blockIdx.x);
 }
 
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
@@ -1198,6 +1523,93 @@ extern "C" int ecf8_paged_attention(const void *q, int64_t q_stride, int64_t row
   }
   if (const int groups = few.groups + tiles.groups)
     join_kernel<<<(unsigned)groups, 256, 0, as_stream(stream)>>>(a, few, tiles);
+  return launched();
+}
+
+extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t rows,
+                                    const ecf8_paged_batch *b, const ecf8_draft_trees *trees,
+                                    const void *k_pool, const void *v_pool, int fp8,
+                                    const float *k_scale, const float *v_scale, void *out,
+                                    int64_t out_stride, void *stream) {
+  if (!q || !k_pool || !v_pool || !out || rows <= 0 || (fp8 && (!k_scale || !v_scale)))
+    return ECF8_ERR_INVALID_ARG;
+  if (const int rc = ecf8::draft::check_trees(b, trees)) return rc;
+  if (rows > b->rows) return ECF8_ERR_CAPACITY;
+  const int64_t wide = (int64_t)b->Hq * kD;
+  if (q_stride % 8 || out_stride % 4 || (rows > 1 && (q_stride < wide || out_stride < wide)))
+    return ECF8_ERR_UNSUPPORTED;
+  if (!aligned(q, 16) || !aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(out, 8) ||
+      !aligned(k_scale, 4) || !aligned(v_scale, 4))
+    return ECF8_ERR_MISALIGNED;
+  const ecf8::draft::Work w = ecf8::draft::work_layout(b->seqs, b->rows, b->Hq, b->Hkv,
+                                                       trees->max_nodes, trees->max_children);
+  auto *base = static_cast<uint8_t *>(trees->work);
+  auto *counts = reinterpret_cast<ecf8::draft::Counts *>(base);
+  Attn a{};
+  a.q = static_cast<const uint16_t *>(q), a.out = static_cast<uint16_t *>(out);
+  a.k = k_pool, a.v = v_pool;
+  a.q_stride = q_stride, a.out_stride = out_stride;
+  a.ks = fp8 ? k_scale : nullptr, a.vs = fp8 ? v_scale : nullptr;
+  a.starts = b->starts, a.table = b->table, a.refused = b->refused;
+  a.masks = trees->masks, a.lengths = b->lengths;
+  a.stamp = &counts->stamp, a.want_stamp = ecf8::draft::schedule_stamp(b, trees);
+  a.Hkv = b->Hkv, a.group = b->Hq / b->Hkv, a.rows = (int)rows, a.seqs = b->seqs;
+  a.width = b->width;
+  a.shift = __builtin_ctz((unsigned)b->page_size), a.pages = (uint32_t)b->pages;
+  a.scale = kLog2e / sqrtf((float)kD);
+  a.n_items = &counts->items;
+  a.items = reinterpret_cast<const Item *>(base + w.items_at);
+  a.stats = reinterpret_cast<float2 *>(base + w.stats);
+  a.sums = reinterpret_cast<float *>(base + w.sums);
+  // tiles of the step, and the pieces that their cuts add
+  const int64_t seqs = rows < b->seqs ? rows : b->seqs;
+  const int64_t tiles = (rows < w.nodes ? rows : w.nodes) * a.group / w.tile + seqs;
+  const int64_t units =
+      ((int64_t)b->width * b->page_size + ecf8::draft::kUnitKeys - 1) / ecf8::draft::kUnitKeys;
+  const int64_t cuts = w.target < tiles * (units - 1) ? w.target : tiles * (units - 1);
+  a.grid = (int)(tiles + cuts);
+  const unsigned grid = (unsigned)(a.grid * a.Hkv);
+  Joins j{};
+  j.n = &counts->joins, j.list = reinterpret_cast<const Join *>(base + w.joins_at);
+  j.stats = a.stats, j.sums = a.sums;
+  j.rows_groups = w.tile / 8;
+  j.groups = (int)(tiles < cuts ? tiles : cuts) * a.Hkv * j.rows_groups;
+#define ECF8_TREE_FEW(T)                                                                  \
+  do {                                                                                    \
+    if (fp8) few_kernel<kPagesFp8, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);      \
+    else few_kernel<kPages, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);             \
+  } while (0)
+#define ECF8_TREE(R, S, D)                                                                \
+  do {                                                                                    \
+    if (fp8) tree_kernel<kPagesFp8, R / 32, S, D><<<grid, 512, 0, as_stream(stream)>>>(a); \
+    else tree_kernel<kPages, R / 32, S, D><<<grid, 512, 0, as_stream(stream)>>>(a);       \
+  } while (0)
+#define ECF8_TREE_JOIN(R) \
+  if (j.groups) tree_join_kernel<R><<<(unsigned)j.groups, 256, 0, as_stream(stream)>>>(a, j)
+  switch (w.tile) {
+    case 16:
+      ECF8_TREE_FEW(1);
+      ECF8_TREE_JOIN(32);
+      break;
+    case 32:
+      ECF8_TREE_FEW(2);
+      ECF8_TREE_JOIN(32);
+      break;
+    case 64:
+      ECF8_TREE(64, 4, 1);
+      ECF8_TREE_JOIN(64);
+      break;
+    case 128:
+      ECF8_TREE(128, 2, 2);
+      ECF8_TREE_JOIN(128);
+      break;
+    default:
+      ECF8_TREE(256, 2, 2);
+      ECF8_TREE_JOIN(256);
+  }
+#undef ECF8_TREE_FEW
+#undef ECF8_TREE
+#undef ECF8_TREE_JOIN
   return launched();
 }
 
