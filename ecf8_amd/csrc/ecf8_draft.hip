@@ -33,12 +33,13 @@ struct Plan {
   Counts *counts;
   Item *items;
   Join *joins;
-  int seqs, rows, all_rows, group, max_nodes, max_children, tile, target, least;
+  int seqs, rows, all_rows, group, max_nodes, max_children, tile, target, begin;
   uint64_t stamp;
 };
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPer = kMaxSeqs / kPlanThreads;
+constexpr int kLeast = 1;  // units on both sides of a cut
 
 // The exclusive prefix sums of N values over the workgroup, and their totals.
 // Calls in a row alternate between two halves of `waves`.
@@ -112,9 +113,9 @@ __device__ __forceinline__ int bucket_of(int length, int share) {
 }
 
 // The attention's schedule, by one workgroup.  Every (sequence, tile of rows)
-// has ceil(length / kUnitKeys) units; laid end to end they are cut at the
-// multiples of a workgroup's share (where `least` units are left on both
-// sides), and the pieces listed from the longest on.
+// has ceil(length / kUnitKeys) units, and begin for its first loads and last
+// sums; laid end to end they are cut at the multiples of a workgroup's share, and
+// the pieces listed from the longest on.
 __device__ __forceinline__ void plan_schedule(const Plan &a) {
   __shared__ int s_first[kMaxSeqs + 1];  // tiles before a sequence's
   __shared__ int s_waves[2][2][kPlanWaves];
@@ -132,7 +133,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
     if (n < 1 || n > a.max_nodes || start < 0 || start > a.rows - n || len < n) continue;
     tiles[i] = (n * a.group + a.tile - 1) / a.tile;
     sum += tiles[i];
-    units += tiles[i] * ((len + kUnitKeys - 1) / kUnitKeys);
+    units += tiles[i] * ((len + kUnitKeys - 1) / kUnitKeys + a.begin);
   }
   // (the sum of all can pass 32 bits, a thread's cannot)
   const int one[1] = {sum}, halves[2] = {units & 0xffff, units >> 16};
@@ -140,7 +141,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
   block_scan(one, s_waves[0], at, n_tiles);
   block_scan(halves, s_waves[1], skip, all);
   const int64_t exact = (((int64_t)all[1] << 16) + all[0] + a.target - 1) / a.target;
-  const int share = (int)min(max(exact, (int64_t)(2 * a.least)), (int64_t)1 << 29);
+  const int share = (int)min(max(exact, (int64_t)2 * kLeast), (int64_t)1 << 29);
   {
     int first = at[0];
 #pragma unroll
@@ -160,7 +161,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
     for (int i0 = 0; i0 < n_tiles[0]; i0 += kPlanThreads) {  // uniform
       const int i = i0 + tid;
       Item it{};
-      int len = 0, mine[1] = {0};
+      int len = 0, units = 0, mine[1] = {0};
       if (i < n_tiles[0]) {
         int lo = 0, hi = S;
         while (hi - lo > 1) {
@@ -171,20 +172,21 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
         it.seq = lo, it.row0 = (i - s_first[lo]) * a.tile;
         it.start = a.starts[lo], it.n = a.starts[lo + 1] - it.start;
         len = a.lengths[lo], it.cached = len - it.n;
-        mine[0] = (len + kUnitKeys - 1) / kUnitKeys;
+        units = (len + kUnitKeys - 1) / kUnitKeys;
+        mine[0] = units + a.begin;
       }
       int from[1], total[1];
       block_scan(mine, s_waves[0], from, total);
-      const int f = from0 + from[0];
-      const int c0 = (f + a.least + share - 1) / share, c1 = (f + mine[0] - a.least) / share;
-      const int k = mine[0] ? max(0, c1 - c0 + 1) + 1 : 0;
+      const int f = from0 + from[0] + a.begin;
+      const int c0 = (f + kLeast + share - 1) / share, c1 = (f + units - kLeast) / share;
+      const int k = units ? max(0, c1 - c0 + 1) + 1 : 0;
       const int cut[2] = {k > 1 ? k : 0, k > 1};
       int p[2], all_cut[2];
       block_scan(cut, s_waves[1], p, all_cut);
       p[0] += parts, p[1] += n_joins;
       for (int j = 0; j < k; ++j) {
         const int u0 = j ? (c0 + j - 1) * share - f : 0;
-        const int u1 = j + 1 < k ? (c0 + j) * share - f : mine[0];
+        const int u1 = j + 1 < k ? (c0 + j) * share - f : units;
         const int to = atomicAdd(&s_bucket[bucket_of(u1 - u0, share)], 1);
         if (write) {
           it.k0 = u0 * kUnitKeys, it.k1 = min(u1 * kUnitKeys, len);
@@ -899,7 +901,7 @@ extern "C" int ecf8_draft_plan(const ecf8_paged_batch *b, const ecf8_draft_trees
   const Plan a{b->starts, b->lengths, parents, t->masks, t->parents, b->positions, b->refused,
                reinterpret_cast<Counts *>(base), reinterpret_cast<Item *>(base + w.items_at),
                reinterpret_cast<Join *>(base + w.joins_at), b->seqs, (int)rows, b->rows, b->Hq / b->Hkv,
-               t->max_nodes, t->max_children, w.tile, w.target, 1, schedule_stamp(b, t)};
+               t->max_nodes, t->max_children, w.tile, w.target, w.tile <= 32 ? 1 : 5, schedule_stamp(b, t)};
   const unsigned grid = 1 + (unsigned)((b->seqs + kPlanWaves - 1) / kPlanWaves);
   plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
   return launched();

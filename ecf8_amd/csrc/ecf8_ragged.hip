@@ -77,6 +77,17 @@ __device__ __forceinline__ void widen16(u32x4 c, u32x4 (&out)[2]) {
   }
 }
 
+// The same by the conversion that gives bf16 at once: half of the instructions.
+__device__ __forceinline__ void widen16_pairs(u32x4 c, u32x4 (&out)[2]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    out[j >> 1][2 * (j & 1)] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[j], 1.f, false));
+    out[j >> 1][2 * (j & 1) + 1] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[j], 1.f, true));
+  }
+}
+
 // Keys and values lie in LDS as rows of 128 bf16, 272 and 288 bytes apart: the
 // key operand reads 16 bytes of 16 rows, the transposing value read 32 bytes
 // of eight rows each half wave, and both find all 64 banks, at addresses that
@@ -155,11 +166,10 @@ struct Operands {
 // product's B operand (O^T += V^T P^T) as they stand.  kFine: they enter in two
 // parts of bf16, where the matrix unit has nothing better to do; the error
 // against 64 bits is then the output's rounding, and else 1.4 times that.
-template <int T, bool kFine = false>
+// kAhead: operands are read from LDS this many ahead of their products (and not all
+// at once, which would take registers that the other operands live in).
+template <int T, bool kFine = false, int kAhead = 1>
 struct Rows {
-  // operands are read from LDS this many ahead of their products (and not all
-  // at once, which would take registers that the other operands live in)
-  static constexpr int kAhead = 1;
   v4f o[T][8];
   // of the lane's query (alike in its four lanes): the whole number that its
   // base-2 exponents are taken from, and the sum of its probabilities, as a
@@ -278,6 +288,13 @@ struct Rows {
         }
       }
   }
+  // Two probabilities: cut off to bf16, and what they lost (see powers).
+  static __device__ __forceinline__ u32x2 cut(float e0, float e1) {
+    const uint32_t u0 = __float_as_uint(e0), u1 = __float_as_uint(e1) & 0xffff0000u;
+    return u32x2{u1 | u0 >> 16,
+                 pack_bf16(fmaf(e0, 0x1p-24f, e0 - __uint_as_float(u0 & 0xffff0000u)),
+                           fmaf(e1, 0x1p-24f, e1 - __uint_as_float(u1)))};
+  }
   __device__ __forceinline__ void sum(const u32x4 (&p)[T]) {
     constexpr uint32_t one = 0x3f803f80u;
     const v8bf ones = __builtin_bit_cast(v8bf, u32x4{one, one, one, one});
@@ -306,7 +323,11 @@ struct Rows {
   __device__ __forceinline__ void stream(lds_u8 *v, lds_u8 *k, u32x4 (&was)[T],
                                          const v8bf (&q)[T][4], v4f (&s)[T][2], float c,
                                          Between between) {
-    u32x4 f[kAhead + 1], p[T];
+    u32x4 f[kAhead + 1], p[T], rest[kFine ? T : 1];
+    if constexpr (kFine) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) rest[t] = low[t];
+    }
     float e[T][2];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f[i] = operand(v, k, i);
@@ -318,13 +339,25 @@ struct Rows {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         e[t][i & 1] = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], c, -m[t]));
-        if (i & 1) p[t][i >> 1] = pack_bf16(e[t][0], e[t][1]);
+        if (i & 1) {
+          if constexpr (kFine) {
+            const u32x2 two = cut(e[t][0], e[t][1]);
+            p[t][i >> 1] = two[0], low[t][i >> 1] = two[1];
+          } else {
+            p[t][i >> 1] = pack_bf16(e[t][0], e[t][1]);
+          }
+        }
       }
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+      for (int t = 0; t < T; ++t) {
         o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
             __builtin_bit_cast(v8bf, f[i % (kAhead + 1)]), __builtin_bit_cast(v8bf, was[t]),
             o[t][i], 0, 0, 0);
+        if constexpr (kFine)
+          o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(v8bf, f[i % (kAhead + 1)]), __builtin_bit_cast(v8bf, rest[t]),
+              o[t][i], 0, 0, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     uint32_t bits = 0;
@@ -571,23 +604,36 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
   }
 }
 
-// The item of slot `item` of a step's trees; false past the last, and where the
-// plan is another step's.
-__device__ __forceinline__ bool get_tree_item(const Attn &a, int item, Place &p) {
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused &&
-      (a.starts[a.seqs] > a.rows || *a.stamp != a.want_stamp))
-    *a.refused = 1;
+// The item of slot `item` of a step's trees; false past the last.  A plan of these
+// sizes may be of another step (stale): its items lead to no place out of range,
+// so what was loaded for the check is looked at only where outputs are written.
+struct TreePlace : Place {
+  bool stale, report;
+};
+__device__ __forceinline__ bool get_tree_item(const Attn &a, int item, TreePlace &p) {
   const Item it = a.items[item];  // item < a.grid: in the list, filled or not
-  asm volatile("" ::"s"(it.seq), "s"(it.start));  // not after the wait for n_items
-  if (*a.stamp != a.want_stamp || item >= *a.n_items) return false;
-  if (a.starts[it.seq] != it.start || a.starts[it.seq + 1] != it.start + it.n ||
-      a.lengths[it.seq] != it.cached + it.n) {
-    if (threadIdx.x == 0 && a.refused) *a.refused = 1;
+  const uint64_t stamp = *a.stamp;
+  const int n_items = *a.n_items, step_rows = a.starts[a.seqs];
+  // (all before the first wait)
+  asm volatile("" ::"s"(it.seq), "s"(it.start), "s"(n_items), "s"((int)stamp), "s"(step_rows));
+  p.report = blockIdx.x == gridDim.x - 1 && (step_rows > a.rows || stamp != a.want_stamp);
+  if (stamp != a.want_stamp || item >= n_items) {
+    if (p.report && threadIdx.x == 0 && a.refused) *a.refused = 1;
     return false;
   }
   p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
   p.start = it.start, p.n = it.n, p.cached = it.cached;
+  // (scalar loads: the wait for vector ones would be here)
+  typedef const __attribute__((address_space(4))) int constant_int;
+  auto *starts = (constant_int *)a.starts, *lengths = (constant_int *)a.lengths;
+  const int start = starts[it.seq], next = starts[it.seq + 1], length = lengths[it.seq];
+  p.stale = ((start ^ it.start) | (next ^ (it.start + it.n)) |
+             (length ^ (it.cached + it.n))) != 0;
   return true;
+}
+__device__ __forceinline__ bool may_write(const Attn &a, const TreePlace &p) {
+  if ((p.report || p.stale) && threadIdx.x == 0 && a.refused) *a.refused = 1;
+  return !p.stale;
 }
 
 // The masks of the lane's queries, as load_queries has them.
@@ -666,7 +712,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const int unit = lane % kUnits;
   const Operands ops(lane);
 
-  Place p;
+  std::conditional_t<kTree, TreePlace, Place> p;
   if constexpr (kTree) {
     if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
   } else {
@@ -794,6 +840,9 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
         }
   }
 
+  if constexpr (kTree) {
+    if (!may_write(a, p)) return;
+  }
   // join the waves
   float l[T];
 #pragma unroll
@@ -1129,7 +1178,7 @@ struct Joins {
 
 // The parts of split rows, joined: four dims a lane, kSplit halves of a wave a
 // row (each every kSplit-th part), four parts' loads at a time.
-template <int kSplit, int kPartRows, bool kTree = false>
+template <int kSplit, int kPartRows>
 __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int group) {
   __shared__ float s_top[8], s_l[8];
   __shared__ v4f s_sum[8][32];
@@ -1139,12 +1188,6 @@ __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int gr
   const Join jn = o.list[j];  // j: in the list, filled or not
   asm volatile("" ::"s"(jn.row0), "s"(jn.start));  // not after the wait for the count
   if (*a.stamp != a.want_stamp || j >= *o.n) return;
-  if constexpr (kTree) {  // (pad: the sequence and its cached tokens)
-    const int seq = jn.pad[0];
-    if (a.starts[seq] != jn.start || a.starts[seq + 1] != jn.start + jn.tokens ||
-        a.lengths[seq] != jn.pad[1] + jn.tokens)
-      return;
-  }
   constexpr int part_rows = kPartRows;
   const int n_rows = min(jn.tokens * a.group - jn.row0, part_rows);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
@@ -1199,7 +1242,7 @@ __device__ __forceinline__ void join_parts(const Attn &a, const Joins &o, int gr
       }
     }
     const int g = jn.row0 + row, tk = jn.start + g / a.group;
-    const float inv = kTree && l == 0.f ? 0.f : vscale / l;
+    const float inv = vscale / l;
     if ((kSplit == 1 ? row0 + half < n_rows : half == 0) && tk < a.rows)
       *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
                                  (kvh * a.group + g % a.group) * kD + 4 * lane) =
@@ -1218,201 +1261,234 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 
 // ------------------------------------------------------------ drafted trees
 
-// Workgroup of eight waves: up to 32 kWr rows (token, head of the group) of one
-// KV head against positions [k0, k1).  Waves of the same wave / kWr share a
-// slice of 32 keys, those of the same wave % kWr share 32 rows; all stage kSlices
-// slices a round through registers, kDepth rounds ahead, into LDS.
-template <Source kSrc, int kWr, int kSlices, int kDepth>
-__global__ __launch_bounds__(512) void tree_kernel(Attn a) {
-  constexpr int T = 2, kWk = 8 / kWr, kSteps = kSlices / kWk, kRows = 32 * kWr;
-  constexpr bool kFp8 = kSrc == kPagesFp8, kFine = kWr < 8;
-  constexpr int kUnits = kFp8 ? 8 : 16;  // 16-byte units of a row in memory
-  __shared__ u32x4 s_kv[2][kSlices][32 * (kKeyRow + kValueRow)];
-  __shared__ float s_m[4][16 * T], s_l[4][16 * T];
+// Workgroup of four waves, two a CU: 64 T rows (token, head of the group) of one KV
+// head, 16 T a wave, against positions [k0, k1), 32 a step.  As in tile_kernel a
+// wave's softmax of a step runs beside the second product of the step before
+// (two waves of a SIMD that each do one after the other fall into step, and
+// neither hides the other: 2100 cycles a step of both instead of 1220, T = 2).
+// Keys and values go through registers, kDepth steps ahead, to a ring of LDS
+// stages.
+template <Source kSrc, int T, bool kFine, bool kOnce>
+__global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
+  constexpr int kDepth = 2;
+  constexpr int kRows = 64 * T;
+  constexpr bool kFp8 = kSrc == kPagesFp8;
+  constexpr int kUnits = kFp8 ? 8 : 16;               // 16-byte units of a row in memory
+  constexpr int kPass = 256 / kUnits, kLoads = 32 / kPass;
+  // after the barrier before step j the waves read steps j - 1 to j + 1 and write j + 2
+  constexpr int kRing = 4;
+  __shared__ u32x4 s_kv[kRing][32 * (kKeyRow + kValueRow)];
   __shared__ int s_odd;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = wave % kWr, wk = wave / kWr;
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
 
-  Place p;
+  TreePlace p;
   if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
   const int all_rows = min(p.n * a.group - p.row0, kRows);
-  const int n_rows = min(all_rows - 32 * wr, 32);
+  const int first_row = 16 * T * wave, n_rows = min(all_rows - first_row, 16 * T);
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
-  // A thread stages a 16-byte unit of a row of every slice: of the keys and of the
-  // values, in e4m3 of one of them.
-  const int unit = (int)threadIdx.x % kUnits, sub = (int)(threadIdx.x / kUnits) & 31;
-  const bool keys = threadIdx.x < 256;
+  // load i of a step: row kPass i + sub of its keys and values.  kTail: past the
+  // end the last row again.
+  const int unit = (int)threadIdx.x % kUnits, sub = (int)threadIdx.x / kUnits;
   const int *table = a.table + (size_t)p.seq * a.width;
-  const int rounds = (p.k1 - p.k0 + 32 * kSlices - 1) / (32 * kSlices);
-  auto key_of = [&](int j, int i) { return min(p.k0 + 32 * (kSlices * j + i) + sub, p.k1 - 1); };
-  auto look = [&](int j, int (&entry)[kSlices]) {
-#pragma unroll
-    for (int i = 0; i < kSlices; ++i) entry[i] = table[key_of(j, i) >> a.shift];
+  const int steps = (p.k1 - p.k0 + 31) / 32;
+  auto key_of = [&](auto tail, int j, int i) {
+    const int key = p.k0 + 32 * j + kPass * i + sub;
+    return decltype(tail)::value ? min(key, p.k1 - 1) : key;
   };
-  constexpr int kLoads = kFp8 ? 1 : 2;
-  u32x4 r[kDepth][kSlices][kLoads];
-  auto load = [&](int j, const int (&entry)[kSlices], u32x4 (&r)[kSlices][kLoads]) {
+  struct Staged {
+    u32x4 k[kLoads], v[kLoads];
+    int entry[kLoads];  // pages of the step kDepth later
+  };
+  auto look = [&](auto tail, int j, Staged &r) {
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) {
-      const uint32_t page = min((uint32_t)entry[i], a.pages - 1);
-      const size_t at = (size_t)(((page * a.Hkv + kvh) << a.shift) +
-                                 (key_of(j, i) & ((1 << a.shift) - 1))) * kUnits + unit;
-      if constexpr (kFp8) {
-        r[i][0] = static_cast<const u32x4 *>(keys ? a.k : a.v)[at];
-      } else {
-        r[i][0] = static_cast<const u32x4 *>(a.k)[at];
-        r[i][1] = static_cast<const u32x4 *>(a.v)[at];
-      }
+    for (int i = 0; i < kLoads; ++i) r.entry[i] = table[key_of(tail, j, i) >> a.shift];
+  };
+  auto place = [&](auto tail, int j, const Staged &r, size_t (&at)[kLoads]) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t page = min((uint32_t)r.entry[i], a.pages - 1);
+      at[i] = (size_t)(((page * a.Hkv + kvh) << a.shift) +
+                       (key_of(tail, j, i) & ((1 << a.shift) - 1))) * kUnits + unit;
     }
   };
-  auto store = [&](int j, u32x4 (&r)[kSlices][kLoads]) {
+  auto load = [&](const size_t (&at)[kLoads], Staged &r) {
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) {
-      u32x4 *s_k = s_kv[j & 1][i], *s_v = s_k + 32 * kKeyRow;
-      const bool masked = p.k0 + 32 * (kSlices * j + i) + 31 >= p.cached;  // uniform
-      auto finite = [&](u32x4 v) {
-        if (!masked) return v;
-        const u32x4 f = finite_or_zero(v);
-        if (differ(f, v)) s_odd = 1;
-        return f;
+    for (int i = 0; i < kLoads; ++i) {
+      auto get = [&](const void *pool) {
+        const u32x4 *x = static_cast<const u32x4 *>(pool) + at[i];
+        return kOnce ? __builtin_nontemporal_load(x) : *x;
       };
+      r.k[i] = get(a.k), r.v[i] = get(a.v);
+    }
+  };
+  auto store = [&](auto tail, int j, const Staged &r) {
+    u32x4 *s_k = s_kv[j % kRing], *s_v = s_k + 32 * kKeyRow;
+    const bool masked = decltype(tail)::value && p.k0 + 32 * j + 31 >= p.cached;  // uniform
+    auto finite = [&](u32x4 v) {
+      if (!masked) return v;
+      const u32x4 f = finite_or_zero(v);
+      if (differ(f, v)) s_odd = 1;
+      return f;
+    };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = kPass * i + sub;
       if constexpr (kFp8) {
         u32x4 w[2];
-        widen16(r[i][0], w);
-        if (keys) {
-          s_k[sub * kKeyRow + 2 * unit] = w[0];
-          s_k[sub * kKeyRow + 2 * unit + 1] = w[1];
-        } else {
-          s_v[sub * kValueRow + 2 * unit] = finite(w[0]);
-          s_v[sub * kValueRow + 2 * unit + 1] = finite(w[1]);
-        }
+        widen16_pairs(r.k[i], w);
+        s_k[row * kKeyRow + 2 * unit] = w[0];
+        s_k[row * kKeyRow + 2 * unit + 1] = w[1];
+        widen16_pairs(r.v[i], w);
+        s_v[row * kValueRow + 2 * unit] = finite(w[0]);
+        s_v[row * kValueRow + 2 * unit + 1] = finite(w[1]);
       } else {
-        s_k[sub * kKeyRow + unit] = r[i][0];
-        s_v[sub * kValueRow + unit] = finite(r[i][1]);
+        s_k[row * kKeyRow + unit] = r.k[i];
+        s_v[row * kValueRow + unit] = finite(r.v[i]);
       }
     }
   };
-
-  int first[kDepth + 1][kSlices], entry[kSlices];
-#pragma unroll
-  for (int x = 0; x <= kDepth; ++x) look(x, first[x]);
-  v8bf q[T][4];
-  uint64_t bits[T];
-  const int row0 = p.row0 + min(32 * wr, all_rows - 1), row_end = p.row0 + all_rows;
-  load_queries<T>(a, kvh, p.start, row0, row_end, lane, q);
-  load_masks<T>(a, p.start, row0, row_end, lane, bits);
-  if (threadIdx.x == 0) s_odd = 0;
-#pragma unroll
-  for (int x = 0; x < kDepth; ++x) load(x, first[x], r[x]);
-#pragma unroll
-  for (int i = 0; i < kSlices; ++i) entry[i] = first[kDepth][i];
-  __syncthreads();  // s_odd
-
-  Rows<T, kFine> w;
-  w.init();
-  auto round = [&](int j, u32x4 (&r)[kSlices][kLoads]) {
-    store(j, r);
-    if (j + kDepth < rounds) {  // uniform
-      int next[kSlices];
-      look(j + kDepth + 1, next);
-      load(j + kDepth, entry, r);
-#pragma unroll
-      for (int i = 0; i < kSlices; ++i) entry[i] = next[i];
-    }
-    // (the stage of round j + 1 was read in round j - 1, before this barrier)
+  auto barrier = [] {
+    __builtin_amdgcn_sched_barrier(0);
     lds_barrier();
-    if (n_rows <= 0) return;  // uniform
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto keys = [&](int j) { return (lds_u8 *)s_kv[j % kRing]; };
+  auto values = [&](int j) { return (lds_u8 *)(s_kv[j % kRing] + 32 * kKeyRow); };
+
+  // r[x]: the next steps j of j mod kDepth = (x + 2) mod kDepth; the first two are
+  // staged before the loop
+  constexpr std::true_type kTail;
+  Staged r[kDepth], lead[2];
+  look(kTail, 0, lead[0]), look(kTail, 1, lead[1]);
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const int slice = st * kWk + wk, key0 = p.k0 + 32 * (kSlices * j + slice);
-      if (key0 >= p.k1) break;  // uniform
-      lds_u8 *k = (lds_u8 *)s_kv[j & 1][slice], *v = k + 32 * 16 * kKeyRow;
-      v4f s[T][2];
-      u32x4 pr[T];
-      w.scores(ops, k, q, s);
-      if (key0 + 31 >= p.cached) {
-        uint32_t word[T];
+  for (int x = 0; x < kDepth; ++x) look(kTail, 2 + x, r[x]);
+  v8bf q[T][4];
+  const int row0 = p.row0 + min(first_row, all_rows - 1), row_end = p.row0 + all_rows;
+  load_queries<T>(a, kvh, p.start, row0, row_end, lane, q);
+  if (threadIdx.x == 0) s_odd = 0;
+  size_t at[kLoads];
 #pragma unroll
-        for (int t = 0; t < T; ++t) word[t] = tree_word(bits[t], key0, p.cached, p.k1);
-        w.mask_words(s, word, lane);
-      }
-      w.weigh(s, c, pr, j == 0 && st == 0);
-      w.second(ops, v, pr);
+  for (int x = 0; x < 2; ++x) place(kTail, x, lead[x], at), load(at, lead[x]);
+#pragma unroll
+  for (int x = 0; x < kDepth; ++x) {
+    place(kTail, 2 + x, r[x], at);
+    look(kTail, 2 + kDepth + x, r[x]);
+    load(at, r[x]);
+  }
+  __syncthreads();  // s_odd
+  store(kTail, 0, lead[0]), store(kTail, 1, lead[1]);
+  lds_barrier();
+
+  // Beside the scores of step j + 1: step j + 2 to its stage, and the loads of the
+  // step kDepth later.  Loads past the end are the last row again, never read: a
+  // load that may not be there makes every wait one for all loads.
+  auto between = [&](auto tail, int j, int i, Staged &r) {
+    if (i == 0) {
+      // (in the end the stage of the last step's values is read once more)
+      if (!decltype(tail)::value || j + 2 < steps) store(tail, j + 2, r);
+    } else if (i == 2) {
+      // (pages before the rows: what waits for them must not wait for these rows)
+      place(tail, j + 2 + kDepth, r, at);
+      look(tail, j + 2 + 2 * kDepth, r);
+    } else if (i == 4) {
+      load(at, r);
     }
   };
-#pragma unroll 1
-  for (int j = 0; j < rounds; j += kDepth) {
+  // all waves pass as many barriers: one for step 0, kDepth a turn
+  const int turns = (steps - 1 + kDepth - 1) / kDepth;
+  if (n_rows <= 0) {  // uniform: a wave without rows stages its share
+    barrier();
 #pragma unroll
-    for (int x = 0; x < kDepth; ++x)
-      if (j + x < rounds) round(j + x, r[x]);
+    for (int i = 0; i < 8; ++i) between(kTail, 0, i, r[0]);
+#pragma unroll 1
+    for (int turn = 0; turn < turns; ++turn)
+#pragma unroll
+      for (int x = 1; x <= kDepth; ++x) {
+        barrier();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) between(kTail, turn * kDepth + x, i, r[x % kDepth]);
+      }
+    return;
   }
-  __syncthreads();
-  if (s_odd && n_rows > 0)
-    for (int i = wk; p.k0 + 32 * i < p.k1; i += kWk) {
-      const int key0 = p.k0 + 32 * i;
-      if (key0 + 31 < p.cached) continue;
+  Rows<T, kFine, 2> w;
+  w.init();
+  v4f s[T][2];
+  u32x4 pr[T];
+  auto mask = [&](int j) {
+    const int key0 = p.k0 + 32 * j;
+    if (key0 + 31 < p.cached) return;  // uniform
+    uint64_t bits[T];  // (not kept in registers through the loops)
+    load_masks<T>(a, p.start, row0, row_end, lane, bits);
+    uint32_t word[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) word[t] = tree_word(bits[t], key0, p.cached, p.k1);
+    w.mask_words(s, word, lane);
+  };
+  w.scores(ops, keys(0), q, s);
+  barrier();
+  mask(0);
+  w.weigh(s, c, pr, true);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) between(kTail, 0, i, r[0]);
+  w.scores(ops, keys(1), q, s);
+  // Turns whose steps, and those that they load, have no masks and no end: a loop of
+  // their own, without a branch.
+  const int full = max(0, (min(p.cached, p.k1) - p.k0) / 32);
+  const int clear = min(turns, max(0, full - 3 - 2 * kDepth) / kDepth);
+  int turn = 0;
+#pragma unroll 1
+  for (; turn < clear; ++turn) {
+#pragma unroll
+    for (int x = 1; x <= kDepth; ++x) {
+      const int j = turn * kDepth + x;
+      barrier();
+      w.stream(values(j - 1) + ops.v, keys(j + 1) + ops.k, pr, q, s, c,
+               [&](int i) { between(std::false_type(), j, i, r[x % kDepth]); });
+    }
+  }
+#pragma unroll 1
+  for (; turn < turns; ++turn) {
+#pragma unroll
+    for (int x = 1; x <= kDepth; ++x) {
+      const int j = turn * kDepth + x;
+      barrier();
+      if (j < steps) {  // uniform
+        mask(j);
+        w.stream(values(j - 1) + ops.v, keys(j + 1) + ops.k, pr, q, s, c,
+                 [&](int i) { between(kTail, j, i, r[x % kDepth]); });
+      }
+    }
+  }
+  if (!may_write(a, p)) return;
+  w.second(ops, values(steps - 1), pr);
+  if (s_odd) {  // (written before the last barrier)
+    uint64_t bits[T];
+    load_masks<T>(a, p.start, row0, row_end, lane, bits);
+    for (int key0 = p.k0 + 32 * max(0, (p.cached - p.k0) / 32); key0 < p.k1; key0 += 32)
       w.add_odd_if(
           key0, min(key0 + 32, p.k1), lane,
           [&](int key, int dim) { return value4<kSrc>(a, p, kvh, key, dim); },
           [&](int t, int key) { return (tree_word(bits[t], key, p.cached, p.k1) & 1) != 0; });
-    }
-  float l[T];
+  }
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    l[t] = w.l[t][0];
-    if (l[t] == 0.f) w.m[t] = kLowest;
-  }
-  // join the slices' waves, half of them at a time; over the stages, which have been
-  // read
-  v4f *s_o = reinterpret_cast<v4f *>(&s_kv[0][0][0]);
-#pragma unroll
-  for (int half = kWk / 2; half > 0; half /= 2) {
-    const int at = (wk % half) * kWr + wr;  // below 4
-    if (half < kWk / 2) __syncthreads();
-    if (wk >= half && wk < 2 * half) {
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        if (lane < 16) s_m[at][16 * t + lane] = w.m[t], s_l[at][16 * t + lane] = l[t];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) s_o[(at * 16 + 8 * t + d) * 64 + lane] = w.o[t][d];
-      }
-    }
-    __syncthreads();
-    if (wk < half) {
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const float m = s_m[at][16 * t + (lane & 15)], top = fmaxf(m, w.m[t]);
-        const float f0 = __builtin_amdgcn_exp2f(w.m[t] - top), f1 = __builtin_amdgcn_exp2f(m - top);
-        l[t] = l[t] * f0 + s_l[at][16 * t + (lane & 15)] * f1;
-        w.m[t] = top;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const v4f o = s_o[(at * 16 + 8 * t + d) * 64 + lane];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w.o[t][d][i] = w.o[t][d][i] * f0 + o[i] * f1;
-        }
-      }
-    }
-  }
-  if (wk != 0) return;
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int row = 32 * wr + 16 * t + (lane & 15), g = lane >> 4;
+    const float l = w.l[t][0];
+    const int row = first_row + 16 * t + (lane & 15), g = lane >> 4;
     if (row >= all_rows) continue;
     if (p.part >= 0) {
       const size_t at = ((size_t)p.part * a.Hkv + kvh) * kRows + row;
       v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
-      if (g == 0) a.stats[at] = make_float2(w.m[t], l[t]);
+      if (g == 0) a.stats[at] = make_float2(l == 0.f ? kLowest : w.m[t], l);
     } else {
       const int at = p.row0 + row, tk = p.start + at / a.group;
-      const float inv = l[t] == 0.f ? 0.f : vscale / l[t];  // (a mask can be empty)
+      const float inv = l == 0.f ? 0.f : vscale / l;  // (a mask can be empty)
       if (tk < a.rows) {
         uint16_t *op = a.out + (int64_t)tk * a.out_stride +
                        (kvh * a.group + at % a.group) * kD + 4 * g;
@@ -1426,9 +1502,94 @@ __global__ __launch_bounds__(512) void tree_kernel(Attn a) {
   }
 }
 
-template <int kRows>
-__global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o) {
-  join_parts<kRows <= 32 ? 8 : 1, kRows, true>(a, o, (int)blockIdx.x);
+// Joins the parts of split rows: workgroup of `per` rows of a tile and KV head, four
+// dims a lane, eight parts' loads at a time.  Half a wave a row, or, for many parts
+// of few rows, a row at a time, its parts dealt to the eight half waves.
+__global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o, int part_rows, int per) {
+  __shared__ float s_top[8], s_l[8];
+  __shared__ v4f s_sum[8][32];
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5;
+  const int kvh = (int)blockIdx.x % a.Hkv, group = (int)blockIdx.x / a.Hkv;
+  const int y = group % o.rows_groups, j = group / o.rows_groups;
+  const Join jn = o.list[j];  // j: in the list, filled or not
+  const uint64_t stamp = *a.stamp;
+  const int n_joins = *o.n;
+  asm volatile("" ::"s"(jn.row0), "s"(jn.start), "s"((int)stamp), "s"(n_joins));
+  if (stamp != a.want_stamp || j >= n_joins) return;
+  // (pad: the sequence and its cached tokens; as in get_tree_item)
+  typedef const __attribute__((address_space(4))) int constant_int;
+  auto *starts = (constant_int *)a.starts, *lengths = (constant_int *)a.lengths;
+  const int seq = jn.pad[0];
+  const bool stale = ((starts[seq] ^ jn.start) | (starts[seq + 1] ^ (jn.start + jn.tokens)) |
+                      (lengths[seq] ^ (jn.pad[1] + jn.tokens))) != 0;
+  const int end = min(min(jn.tokens * a.group - jn.row0, part_rows), (y + 1) * per);
+  const float vscale = a.vs ? a.vs[kvh] : 1.f;
+  const size_t step = (size_t)a.Hkv * part_rows;
+  const size_t at0 = ((size_t)jn.part * a.Hkv + kvh) * part_rows;
+  float top, l;
+  v4f sum;
+  // parts x0, x0 + every, ... of a row (maxima of parts without a key are below
+  // every other's)
+  auto gather = [&](int row, int x0, int every) {
+    top = kLowest, l = 0.f, sum = v4f{};
+    for (; x0 < jn.n; x0 += 8 * every) {
+      v4f v[8];
+      float2 st[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const size_t p = at0 + row + min(x0 + u * every, jn.n - 1) * step;
+        v[u] = reinterpret_cast<const v4f *>(o.sums)[p * 32 + lane];
+        st[u] = o.stats[p];
+      }
+      float to = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) to = fmaxf(to, st[u].x);  // (past the last: that again)
+      const float f0 = __builtin_amdgcn_exp2f(top - to);
+      l *= f0, sum *= f0;
+      top = to;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (x0 + u * every >= jn.n) break;
+        const float f = __builtin_amdgcn_exp2f(st[u].x - top);
+        l = fmaf(f, st[u].y, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = fmaf(f, v[u][i], sum[i]);
+      }
+    }
+  };
+  auto put = [&](int row) {
+    const int g = jn.row0 + row, tk = jn.start + g / a.group;
+    const float inv = l == 0.f ? 0.f : vscale / l;  // (a mask can be empty)
+    if (tk < a.rows && !stale)
+      *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
+                                 (kvh * a.group + g % a.group) * kD + 4 * lane) =
+          u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
+  };
+  if ((jn.n + 7) / 8 <= per * ((jn.n + 63) / 64)) {  // whichever takes fewer batches
+    for (int row = y * per + half; row < end; row += 8) gather(row, 0, 1), put(row);
+    return;
+  }
+  for (int row = y * per; row < end; ++row) {
+    gather(row, half, 8);
+    if (lane == 0) s_top[half] = top, s_l[half] = l;
+    s_sum[half][lane] = sum;
+    __syncthreads();
+    if (half == 0) {
+      float to = s_top[0];
+#pragma unroll
+      for (int x = 1; x < 8; ++x) to = fmaxf(to, s_top[x]);
+      l = 0.f, sum = v4f{};
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float f = __builtin_amdgcn_exp2f(s_top[x] - to);
+        l = fmaf(f, s_l[x], l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = fmaf(f, s_sum[x][lane][i], sum[i]);
+      }
+      put(row);
+    }
+    __syncthreads();
+  }
 }
 
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
@@ -1572,44 +1733,42 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
   Joins j{};
   j.n = &counts->joins, j.list = reinterpret_cast<const Join *>(base + w.joins_at);
   j.stats = a.stats, j.sums = a.sums;
-  j.rows_groups = w.tile / 8;
-  j.groups = (int)(tiles < cuts ? tiles : cuts) * a.Hkv * j.rows_groups;
+  // rows a workgroup: eight, fewer while there are not a thousand workgroups
+  const int most_rows = trees->max_nodes * a.group < w.tile ? trees->max_nodes * a.group : w.tile;
+  const int64_t splits = (tiles < cuts ? tiles : cuts) * a.Hkv;
+  int per = 8;
+  while (per > 1 && splits * ((most_rows + per - 1) / per) < 1024) per /= 2;
+  j.rows_groups = (most_rows + per - 1) / per;
+  j.groups = (int)(splits * j.rows_groups);
 #define ECF8_TREE_FEW(T)                                                                  \
   do {                                                                                    \
     if (fp8) few_kernel<kPagesFp8, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);      \
     else few_kernel<kPages, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);             \
   } while (0)
-#define ECF8_TREE(R, S, D)                                                                \
+#define ECF8_TREE(T, F, O)                                                             \
   do {                                                                                    \
-    if (fp8) tree_kernel<kPagesFp8, R / 32, S, D><<<grid, 512, 0, as_stream(stream)>>>(a); \
-    else tree_kernel<kPages, R / 32, S, D><<<grid, 512, 0, as_stream(stream)>>>(a);       \
+    if (fp8) tree_kernel<kPagesFp8, T, F, O><<<grid, 256, 0, as_stream(stream)>>>(a);  \
+    else tree_kernel<kPages, T, F, O><<<grid, 256, 0, as_stream(stream)>>>(a);         \
   } while (0)
-#define ECF8_TREE_JOIN(R) \
-  if (j.groups) tree_join_kernel<R><<<(unsigned)j.groups, 256, 0, as_stream(stream)>>>(a, j)
   switch (w.tile) {
     case 16:
       ECF8_TREE_FEW(1);
-      ECF8_TREE_JOIN(32);
       break;
     case 32:
       ECF8_TREE_FEW(2);
-      ECF8_TREE_JOIN(32);
       break;
     case 64:
-      ECF8_TREE(64, 4, 1);
-      ECF8_TREE_JOIN(64);
-      break;
-    case 128:
-      ECF8_TREE(128, 2, 2);
-      ECF8_TREE_JOIN(128);
+      ECF8_TREE(1, true, true);
       break;
     default:
-      ECF8_TREE(256, 2, 2);
-      ECF8_TREE_JOIN(256);
+      if (trees->max_nodes * a.group <= 128) ECF8_TREE(2, false, true);
+      else ECF8_TREE(2, false, false);  // tiles of a sequence share its pages in L2
   }
 #undef ECF8_TREE_FEW
 #undef ECF8_TREE
-#undef ECF8_TREE_JOIN
+  if (j.groups)
+    tree_join_kernel<<<(unsigned)j.groups, 256, 0, as_stream(stream)>>>(
+        a, j, w.tile < kFewRows ? kFewRows : w.tile, per);
   return launched();
 }
 
