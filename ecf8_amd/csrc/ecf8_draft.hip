@@ -17,9 +17,11 @@ using namespace ecf8::draft;
 using ecf8::paged::kMaxSeqs;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 // the same at any address of their elements
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
 typedef v4f v4f_any __attribute__((aligned(4)));
 
 __device__ __forceinline__ float bf16_f32(uint32_t h16) { return __uint_as_float(h16 << 16); }
@@ -223,9 +225,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
 
 // -------------------------------------------------------- probabilities
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) less that
-constexpr float kLn2 = 0.69314718f;
+constexpr double kLog2e = 1.4426950408889634;
 
 struct Probs {
   const uint16_t *logits;
@@ -237,24 +237,25 @@ struct Probs {
   int V, chunks;
 };
 
-// 1 / temperature times log2(e), in two parts.
+// log2(e) / temperature in two parts, each rounded once.
 struct Scale {
   float hi, lo;
   bool greedy;
   __device__ __forceinline__ explicit Scale(float t) {
     greedy = t <= 0.f;
-    hi = fminf(kLog2e / t, 0x1p100f);
-    if (t != t) hi = t;
-    lo = (fmaf(-hi, t, kLog2e) + kLog2eLow) / t;
-    if (!(fabsf(lo) < 0x1p80f)) lo = 0.f;
+    // (finite and above zero, so that -inf times it is -inf)
+    const double c = fmin(fmax(kLog2e / (double)t, 0x1p-100), 0x1p100);
+    hi = t != t ? t : (float)c;
+    lo = (float)(c - (double)hi);
   }
-  // exp(x / temperature), x <= 0; what the product's rounding lost is added
+  // exp(x / temperature), x <= 0
   __device__ __forceinline__ float exp(float x) const {
-    const float e = x * hi;
-    const float rest = fmaf(x, lo, fmaf(x, hi, -e));
-    const float y = __builtin_amdgcn_exp2f(e);
-    // (rest is no number where x / temperature is infinite: y is 0)
-    return y > 0.f ? fmaf(y * kLn2, rest, y) : y;
+    return __builtin_amdgcn_exp2f(x * hi);
+  }
+  // the same without hi's rounding
+  __device__ __forceinline__ float fine_exp(float x) const {
+    const float y = fmaxf(x, -0x1p20f / hi);  // 0 from there on; (NaN becomes that)
+    return __builtin_amdgcn_exp2f(fmaf(y, hi, y * lo));
   }
 };
 
@@ -268,43 +269,60 @@ __device__ __forceinline__ uint64_t logit_key(uint32_t h, uint32_t i) {
   return ((uint64_t)k << 32) | (uint32_t)~i;
 }
 
-// Eight logits from element i on; past the row's end -inf.
-__device__ __forceinline__ u32x4 load_logits(const uint16_t *row, int i, int V) {
-  if (i + 8 <= V) return *reinterpret_cast<const u32x4_any *>(row + i);
-  u32x4 v;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t h = i + j < V ? row[i + j] : 0xff80u;
-    v[j >> 1] = j & 1 ? v[j >> 1] | h << 16 : h;
-  }
-  return v;
-}
-
-__device__ __forceinline__ float at8(u32x4 v, int j) {
+template <class Vec>
+__device__ __forceinline__ float logit(Vec v, int j) {
   return j & 1 ? __uint_as_float(v[j >> 1] & 0xffff0000u) : bf16_f32(v[j >> 1] & 0xffffu);
 }
 
+// A thread's part of a run of a row: units of kUnit logits, kAtOnce of them in
+// flight; units(u, n, v): n units from u on, 256 apart.  The row's last V mod
+// kUnit come one each to the first threads of the last run: single(i, logit).
+constexpr int kAtOnce = 4;
+template <int kUnit, class VecAny, class Vec, class Units, class Single>
+__device__ __forceinline__ void for_run(const Probs &a, int row, Vec, Units units,
+                                        Single single) {
+  const uint16_t *x = a.logits + (int64_t)row * a.ld;
+  const int whole = a.V / kUnit, per = (whole + a.chunks - 1) / a.chunks;
+  const int u0 = blockIdx.x * per, u1 = min(u0 + per, whole);
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += 256 * kAtOnce) {
+    Vec v[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      v[i] = *reinterpret_cast<const VecAny *>(x + kUnit * (int64_t)min(u + 256 * i, u1 - 1));
+    units(u, min(kAtOnce, (u1 - u + 255) / 256), v);
+  }
+  if (blockIdx.x == a.chunks - 1 && (int)threadIdx.x < a.V % kUnit) {
+    const int i = kUnit * whole + (int)threadIdx.x;
+    single(i, x[i]);
+  }
+}
+
 // The largest logit of a run of a row and the sum of the exponentials below it;
-// greedy rows: the best key.
+// greedy rows: the best key.  Bound by HBM: 416 rows of 151936 (126 MB) 28 us, 4.5
+// TB/s; the second kernel (253 MB written) 46 us, 5.5 TB/s.
 __global__ __launch_bounds__(256) void probability_stats_kernel(Probs a) {
   __shared__ uint64_t s_k[4];
   __shared__ float s_m[4], s_l[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.y, units = (a.V + 7) / 8, per = (units + a.chunks - 1) / a.chunks;
-  const uint16_t *x = a.logits + (int64_t)row * a.ld;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y;
   const Scale c(a.temperature ? a.temperature[row] : a.common);
-  const int u0 = blockIdx.x * per, u1 = min(u0 + per, units);
   uint2 *out = a.work + (size_t)row * ECF8_PROBABILITY_CHUNKS + blockIdx.x;
   if (c.greedy) {  // uniform
     uint64_t best = 0;
-    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
-      const u32x4 v = load_logits(x, 8 * u, a.V);
+    auto take = [&](uint32_t h, int i) {
+      const uint64_t k = logit_key(h, i);
+      best = k > best ? k : best;
+    };
+    for_run<8, u32x4_any>(
+        a, row, u32x4{},
+        [&](int u, int n, const u32x4(&v)[kAtOnce]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint64_t k = logit_key((v[j >> 1] >> (16 * (j & 1))) & 0xffffu, 8 * u + j);
-        best = k > best ? k : best;
-      }
-    }
+          for (int i = 0; i < kAtOnce; ++i)
+            if (i < n)
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                take((v[i][j >> 1] >> (16 * (j & 1))) & 0xffffu, 8 * (u + 256 * i) + j);
+        },
+        [&](int i, uint32_t h) { take(h, i); });
     for (int o = 32; o > 0; o >>= 1) {
       const uint64_t k = __shfl_xor(best, o);
       best = k > best ? k : best;
@@ -317,28 +335,38 @@ __global__ __launch_bounds__(256) void probability_stats_kernel(Probs a) {
     }
     return;
   }
+  // m: -inf while nothing else was there; sums from it count from 0 then, which
+  // -inf leaves at 0 and NaN makes NaN
   float m = -INFINITY, l = 0.f;
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
-    const u32x4 v = load_logits(x, 8 * u, a.V);
-    float top = at8(v, 0);
+  auto raise = [&](float top) {
+    if (top > m) l *= m == -INFINITY ? 1.f : c.exp(m - top), m = top;
+    return m == -INFINITY ? 0.f : m;
+  };
+  for_run<8, u32x4_any>(
+      a, row, u32x4{},
+      [&](int u, int n, const u32x4(&v)[kAtOnce]) {
+        float top = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, at8(v, j));
-    if (top > m) {
-      l *= m == -INFINITY ? 0.f : c.exp(m - top);
-      m = top;
-    }
-    const float from = m == -INFINITY ? 0.f : m;  // -inf from that: 0, NaN: NaN
+        for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l += c.exp(at8(v, j) - from);
-  }
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, logit(v[i], j));
+        const float from = raise(top);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+          if (i < n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j & 1] += c.exp(logit(v[i], j) - from);
+        l += sum[0] + sum[1];
+      },
+      [&](int i, uint32_t h) {
+        const float y = bf16_f32(h);
+        l += c.exp(y - raise(y));
+      });
   auto join = [&](float m2, float l2) {
     const float top = fmaxf(m, m2);
-    if (top == -INFINITY) {
-      l += l2;
-    } else {
-      l = (m == -INFINITY ? l : l * c.exp(m - top)) + (m2 == -INFINITY ? l2 : l2 * c.exp(m2 - top));
-      m = top;
-    }
+    l = (m == -INFINITY ? l : l * c.exp(m - top)) + (m2 == -INFINITY ? l2 : l2 * c.exp(m2 - top));
+    m = top;
   };
   for (int o = 32; o > 0; o >>= 1) {
     const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o);
@@ -352,14 +380,18 @@ __global__ __launch_bounds__(256) void probability_stats_kernel(Probs a) {
   }
 }
 
+// kPast: stores go past the caches, so that the logits, read twice, stay there.
+template <bool kPast>
 __global__ __launch_bounds__(256) void probability_kernel(Probs a) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.y, units = (a.V + 7) / 8, per = (units + a.chunks - 1) / a.chunks;
-  const uint16_t *x = a.logits + (int64_t)row * a.ld;
+  const int lane = threadIdx.x & 63, row = blockIdx.y;
   float *out = a.out + (int64_t)row * a.ldo;
   const Scale c(a.temperature ? a.temperature[row] : a.common);
-  const int u0 = blockIdx.x * per, u1 = min(u0 + per, units);
   const uint2 st = a.work[(size_t)row * ECF8_PROBABILITY_CHUNKS + min(lane, a.chunks - 1)];
+  auto put = [&](int i, v4f p) {
+    v4f_any *to = reinterpret_cast<v4f_any *>(out + i);
+    if constexpr (kPast) __builtin_nontemporal_store(p, to);
+    else *to = p;
+  };
   if (c.greedy) {  // uniform
     uint64_t best = ((uint64_t)st.y << 32) | st.x;
     for (int o = 32; o > 0; o >>= 1) {
@@ -367,17 +399,17 @@ __global__ __launch_bounds__(256) void probability_kernel(Probs a) {
       best = k > best ? k : best;
     }
     const int at = (int)~(uint32_t)best;
-    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = 8 * u + 4 * h;
-        const v4f v = {i == at ? 1.f : 0.f, i + 1 == at ? 1.f : 0.f, i + 2 == at ? 1.f : 0.f,
-                       i + 3 == at ? 1.f : 0.f};
-        if (i + 4 <= a.V) *reinterpret_cast<v4f_any *>(out + i) = v;
-        else
-          for (int j = 0; j < 4; ++j)
-            if (i + j < a.V) out[i + j] = v[j];
-      }
+    const int whole = a.V / 4, per = (whole + a.chunks - 1) / a.chunks;
+    const int u1 = min((int)(blockIdx.x + 1) * per, whole);
+    for (int u = blockIdx.x * per + (int)threadIdx.x; u < u1; u += 256) {
+      const int i = at - 4 * u;
+      put(4 * u, v4f{i == 0 ? 1.f : 0.f, i == 1 ? 1.f : 0.f, i == 2 ? 1.f : 0.f,
+                     i == 3 ? 1.f : 0.f});
+    }
+    if (blockIdx.x == a.chunks - 1 && (int)threadIdx.x < a.V % 4) {
+      const int i = 4 * whole + (int)threadIdx.x;
+      out[i] = i == at ? 1.f : 0.f;
+    }
     return;
   }
   const float m0 = __uint_as_float(st.x);
@@ -387,21 +419,21 @@ __global__ __launch_bounds__(256) void probability_kernel(Probs a) {
   float l = lane >= a.chunks ? 0.f : __uint_as_float(st.y);
   if (m0 != -INFINITY) l *= c.exp(m0 - m);
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-  const float inv = 1.f / l;
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
-    const u32x4 v = load_logits(x, 8 * u, a.V);
+  // a row with a NaN, an infinity or nothing but -inf is NaN throughout
+  const float inv = l > 0.f && l < INFINITY ? 1.f / l : NAN;
+  for_run<4, u32x2_any>(
+      a, row, u32x2{},
+      [&](int u, int n, const u32x2(&v)[kAtOnce]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = 8 * u + 4 * h;
-      v4f p;
+        for (int i = 0; i < kAtOnce; ++i)
+          if (i < n) {
+            v4f p;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = c.exp(at8(v, 4 * h + j) - m) * inv;
-      if (i + 4 <= a.V) *reinterpret_cast<v4f_any *>(out + i) = p;
-      else
-        for (int j = 0; j < 4; ++j)
-          if (i + j < a.V) out[i + j] = p[j];
-    }
-  }
+            for (int j = 0; j < 4; ++j) p[j] = c.fine_exp(logit(v[i], j) - m) * inv;
+            put(4 * (u + 256 * i), p);
+          }
+      },
+      [&](int i, uint32_t h) { out[i] = c.fine_exp(bf16_f32(h) - m) * inv; });
 }
 
 // --------------------------------------------------------- verification
@@ -921,15 +953,19 @@ extern "C" int ecf8_token_probabilities(const void *logits, int64_t ld, int64_t 
     return ECF8_ERR_CAPACITY;
   if (!aligned(logits, 2) || !aligned(out, 4) || !aligned(temperature, 4) || !aligned(work, 8))
     return ECF8_ERR_MISALIGNED;
+  // A run is what a workgroup has in flight at once, 1024 units of eight, or, while
+  // the workgroups are few, less.  416 rows of 151936 in 8 / 19 runs: 78 / 75 us.
   const int64_t units = (V + 7) / 8;
-  int64_t chunks = 2048 / rows < 8 ? 8 : 2048 / rows;
+  int64_t chunks = 2048 / rows < (units + 255) / 256 ? 2048 / rows : (units + 255) / 256;
+  if (chunks < (units + 1023) / 1024) chunks = (units + 1023) / 1024;
   if (chunks > ECF8_PROBABILITY_CHUNKS) chunks = ECF8_PROBABILITY_CHUNKS;
-  if (chunks > (units + 255) / 256) chunks = (units + 255) / 256;
   const Probs a{static_cast<const uint16_t *>(logits), out, temperature, ld, ldo,
                 static_cast<uint2 *>(work), common, (int)V, (int)chunks};
   const dim3 grid((unsigned)chunks, (unsigned)rows);
   probability_stats_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
-  probability_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
+  // (64 rows of 151936, 39 MB: 17.4 us, 18.5 past the caches; 416, 253 MB: 108 and 78)
+  if (rows * V >= 1 << 24) probability_kernel<true><<<grid, 256, 0, as_stream(stream)>>>(a);
+  else probability_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(a);
   return launched();
 }
 
