@@ -155,50 +155,61 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
     if (tid == 0) s_first[S] = n_tiles[0];
   }
   __syncthreads();
-  int n_items = 0, n_joins = 0;
+  int n_items = 0, n_joins = 0, parts = 0, from0 = 0;  // from0: mod share
+  // This thread's tile of a thousand, its units before it, pieces and their places.
+  struct Tile {
+    Item it;
+    int len, units, f, c0, k, part, join;
+  } mine{};
+  auto take = [&](int i0) {
+    const int i = i0 + tid;
+    Tile t{};
+    if (i < n_tiles[0]) {
+      int lo = 0, hi = S;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      t.it.seq = lo, t.it.row0 = (i - s_first[lo]) * a.tile;
+      t.it.start = a.starts[lo], t.it.n = a.starts[lo + 1] - t.it.start;
+      t.len = a.lengths[lo], t.it.cached = t.len - t.it.n;
+      t.units = (t.len + kUnitKeys - 1) / kUnitKeys;
+    }
+    const int all_units[1] = {t.units ? t.units + a.begin : 0};
+    int from[1], total[1];
+    block_scan(all_units, s_waves[0], from, total);
+    t.f = from0 + from[0] + a.begin;
+    t.c0 = (t.f + kLeast + share - 1) / share;
+    const int c1 = (t.f + t.units - kLeast) / share;
+    t.k = t.units ? max(0, c1 - t.c0 + 1) + 1 : 0;
+    const int cut[2] = {t.k > 1 ? t.k : 0, t.k > 1};
+    int before[2], all_cut[2];
+    block_scan(cut, s_waves[1], before, all_cut);
+    t.part = parts + before[0], t.join = n_joins + before[1];
+    parts += all_cut[0], n_joins += all_cut[1];
+    from0 = (from0 + total[0]) % share;
+    mine = t;
+  };
   // Twice over the tiles: count the pieces of each length, then write them.
   for (int write = 0; write < 2; ++write) {
-    int from0 = 0, parts = 0;  // from0: mod share
-    n_joins = 0;
+    if (n_tiles[0] > kPlanThreads) from0 = parts = n_joins = 0;
     for (int i0 = 0; i0 < n_tiles[0]; i0 += kPlanThreads) {  // uniform
-      const int i = i0 + tid;
-      Item it{};
-      int len = 0, units = 0, mine[1] = {0};
-      if (i < n_tiles[0]) {
-        int lo = 0, hi = S;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (s_first[mid] <= i) lo = mid;
-          else hi = mid;
-        }
-        it.seq = lo, it.row0 = (i - s_first[lo]) * a.tile;
-        it.start = a.starts[lo], it.n = a.starts[lo + 1] - it.start;
-        len = a.lengths[lo], it.cached = len - it.n;
-        units = (len + kUnitKeys - 1) / kUnitKeys;
-        mine[0] = units + a.begin;
-      }
-      int from[1], total[1];
-      block_scan(mine, s_waves[0], from, total);
-      const int f = from0 + from[0] + a.begin;
-      const int c0 = (f + kLeast + share - 1) / share, c1 = (f + units - kLeast) / share;
-      const int k = units ? max(0, c1 - c0 + 1) + 1 : 0;
-      const int cut[2] = {k > 1 ? k : 0, k > 1};
-      int p[2], all_cut[2];
-      block_scan(cut, s_waves[1], p, all_cut);
-      p[0] += parts, p[1] += n_joins;
-      for (int j = 0; j < k; ++j) {
-        const int u0 = j ? (c0 + j - 1) * share - f : 0;
-        const int u1 = j + 1 < k ? (c0 + j) * share - f : units;
+      if (!write || n_tiles[0] > kPlanThreads) take(i0);  // (a thousand are kept)
+      for (int j = 0; j < mine.k; ++j) {
+        const int u0 = j ? (mine.c0 + j - 1) * share - mine.f : 0;
+        const int u1 = j + 1 < mine.k ? (mine.c0 + j) * share - mine.f : mine.units;
         const int to = atomicAdd(&s_bucket[bucket_of(u1 - u0, share)], 1);
         if (write) {
-          it.k0 = u0 * kUnitKeys, it.k1 = min(u1 * kUnitKeys, len);
-          it.part = k > 1 ? p[0] + j : -1;
+          Item it = mine.it;
+          it.k0 = u0 * kUnitKeys, it.k1 = min(u1 * kUnitKeys, mine.len);
+          it.part = mine.k > 1 ? mine.part + j : -1;
           a.items[to] = it;
         }
       }
-      if (write && k > 1) a.joins[p[1]] = Join{it.row0, p[0], k, it.start, it.n, {it.seq, it.cached, 0}};
-      parts += all_cut[0], n_joins += all_cut[1];
-      from0 = (from0 + total[0]) % share;
+      if (write && mine.k > 1)
+        a.joins[mine.join] = Join{mine.it.row0, mine.part, mine.k, mine.it.start, mine.it.n,
+                                  {mine.it.seq, mine.it.cached, 0}};
     }
     __syncthreads();
     if (!write) {
@@ -438,6 +449,15 @@ __global__ __launch_bounds__(256) void probability_kernel(Probs a) {
 
 // --------------------------------------------------------- verification
 
+// Where a sequence's walk ended, for the kernel that draws its next token.
+struct Ended {
+  int64_t row;                // packed row whose w is drawn from, -1: none
+  int kept, gone, n_tokens, pad;
+  int64_t tokens[kMaxNodes];  // that are gone from w
+  double inv[kMaxNodes];      // 1 / Z of the levels that are gone
+};
+static_assert(sizeof(Ended) <= kEndedBytes, "the layout has room for it");
+
 struct Verify {
   const int *starts, *parents;
   const int64_t *tokens;
@@ -446,14 +466,46 @@ struct Verify {
   int *kept, *path, *refused;
   int64_t *emitted, *next_token;
   double *runs, *mass;  // [2, seqs, kRuns], [max_children - 1, nodes, kRuns]
+  Ended *ended;         // [seqs]
   int64_t nodes;
-  int seqs, rows, V, max_nodes, max_children, packed, per;
+  int seqs, rows, V, max_nodes, max_children, packed;
+  int per, lanes;  // runs a workgroup, threads a run
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Lane i's value, for an i that is the same in all lanes (a read of a scalar
+// register's worth, where a shuffle goes through LDS).
+__device__ __forceinline__ int lane_of(int v, int i) {
+  return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(i));
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int i) {
+  return (uint64_t)(uint32_t)lane_of((int)(v >> 32), i) << 32 | (uint32_t)lane_of((int)v, i);
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int i) {
+  return (int64_t)lane_of((uint64_t)v, i);
+}
+__device__ __forceinline__ double lane_of(double v, int i) {
+  return __longlong_as_double((long long)lane_of((uint64_t)__double_as_longlong(v), i));
+}
+
+// The inclusive prefix sum over the wave (see ecf8::dev::wave_inclusive_scan), and
+// the sum.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)u, kCtrl, kRows, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), kCtrl, kRows, 0xF, false);
+  return __longlong_as_double((long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo));
+}
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp_or_zero<0x111, 0xF>(v);  // row_shr:1
+  v += dpp_or_zero<0x112, 0xF>(v);  // row_shr:2
+  v += dpp_or_zero<0x114, 0xF>(v);  // row_shr:4
+  v += dpp_or_zero<0x118, 0xF>(v);  // row_shr:8
+  v += dpp_or_zero<0x142, 0xA>(v);  // row_bcast:15
+  v += dpp_or_zero<0x143, 0xC>(v);  // row_bcast:31
   return v;
 }
+__device__ __forceinline__ double wave_sum(double v) { return lane_of(wave_scan(v), 63); }
 
 // What a wave knows of a sequence's tree, lane t of row t.
 struct Tree {
@@ -479,12 +531,10 @@ __device__ __forceinline__ bool load_tree(const Verify &a, int s, Tree &t) {
   const int64_t after = t.start + max(t.up, 0), c = t.in ? t.token : 0;
   t.p = t.in ? (double)a.target[after * a.ld_target + c] : 0.0;
   t.q = kDrawn && t.in ? (double)a.draft[after * a.ld_draft + c] : 0.0;
-  t.kids = 0, t.rank = 0;
-  for (int k = 1; k < t.n; ++k) {
-    const int up = __builtin_amdgcn_readlane(t.up, k);
-    if (up == lane) t.kids |= 1ull << k;
-    t.rank += k < lane && up == t.up;
-  }
+  t.kids = 0;
+  for (int k = 1; k < t.n; ++k)
+    if (__builtin_amdgcn_readlane(t.up, k) == lane) t.kids |= 1ull << k;
+  t.rank = __popcll(__shfl(t.kids, t.up & 63) & ((1ull << lane) - 1));
   t.above = 1ull << lane;
   int up = t.up;
 #pragma unroll
@@ -506,17 +556,17 @@ struct End {
 __device__ __forceinline__ End walk_top(const Tree &t) {
   End e{0, 0};
   for (;;) {
-    uint64_t kids = __shfl(t.kids, e.last);
+    uint64_t kids = lane_of(t.kids, e.last);
     double mass = 1.0;
     e.gone = 0;
     int next = -1;
     while (kids) {
       const int j = __builtin_ctzll(kids);
       kids &= kids - 1;
-      const int64_t c = __shfl(t.token, j);
+      const int64_t c = lane_of(t.token, j);
       // (a token that was rejected is not left)
       const bool twice = __any(((e.gone >> (threadIdx.x & 63)) & 1) && t.token == c);
-      const double w = twice ? 0.0 : __shfl(t.p, j), u = __shfl(t.u, j);
+      const double w = twice ? 0.0 : lane_of(t.p, j), u = lane_of(t.u, j);
       if (u * mass < w) {
         next = j;
         break;
@@ -580,36 +630,90 @@ __device__ __forceinline__ uint64_t try_drawn(const Verify &a, int s, const Tree
 
 __device__ __forceinline__ int run_length(int V) { return ((V + kRuns - 1) / kRuns + 3) / 4 * 4; }
 
-// w of four elements from v on (those at or past `end` are zero), for a row of
-// `gone` rejected children.
-__device__ __forceinline__ void left4(const float *p, const float *q, int v, int end, int gone,
-                                      const double *inv, double (&w)[4]) {
-  v4f pv = {}, qv = {};
-  if (v + 4 <= end) {
-    pv = *reinterpret_cast<const v4f_any *>(p + v);
-    if (gone) qv = *reinterpret_cast<const v4f_any *>(q + v);
-  } else {
-    for (int j = 0; j < 4; ++j)
-      if (v + j < end) {
-        pv[j] = p[v + j];
-        if (gone) qv[j] = q[v + j];
-      }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = (double)pv[j];
-  for (int x = 0; x < gone; ++x) {
-    const double f = inv[x];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = fmax(fma(w[j], f, -(double)qv[j]), 0.0);
-  }
-}
+// What is left of the target's row p after `gone` drawn drafts of row q, or without
+// some tokens.
+struct Row {
+  const float *p, *q;
+  int gone, n_tokens;
+  const double *inv;
+  const int64_t *tokens;
 
-__device__ __forceinline__ double block_sum(double v, double *s) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  // four elements from v on; those at or past `end` are zero
+  __device__ __forceinline__ void load(int v, int end, v4f &pv, v4f &qv) const {
+    pv = qv = v4f{};
+    if (v + 4 <= end) {
+      pv = *reinterpret_cast<const v4f_any *>(p + v);
+      if (gone) qv = *reinterpret_cast<const v4f_any *>(q + v);
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (v + j < end) {
+          pv[j] = p[v + j];
+          if (gone) qv[j] = q[v + j];
+        }
+    }
+  }
+  __device__ __forceinline__ void left(int v, v4f pv, v4f qv, bool some, double (&w)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (double)pv[j];
+    for (int x = 0; x < gone; ++x) {
+      const double f = inv[x];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = fmax(fma(w[j], f, -(double)qv[j]), 0.0);
+    }
+    if (some)
+      for (int x = 0; x < n_tokens; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tokens[x] == v + j) w[j] = 0.0;
+  }
+  // is a token of [lo, end) gone?
+  __device__ __forceinline__ bool any_token(int64_t lo, int64_t end) const {
+    bool some = false;
+    for (int x = 0; x < n_tokens; ++x) some |= tokens[x] >= lo && tokens[x] < end;
+    return some;
+  }
+};
+
+// The sums over a workgroup's runs of w and, kWhole, of p: done(run, w, p) is called
+// by the first of a run's threads.  One or all four waves take a run, kUnits units of
+// four elements in flight.
+constexpr int kUnits = 2;
+template <bool kWhole, class Done>
+__device__ __forceinline__ void sum_runs(const Verify &a, const Row &r, Done done) {
+  __shared__ double s_sum[2][4];
+  const int len = run_length(a.V), l = (int)threadIdx.x % a.lanes;
+  for (int x = (int)threadIdx.x / a.lanes; x < a.per; x += 256 / a.lanes) {
+    const int run = blockIdx.x * a.per + x;
+    const int64_t lo = min((int64_t)run * len, (int64_t)a.V);
+    const int end = (int)min(lo + len, (int64_t)a.V);
+    const bool some = r.any_token(lo, end);
+    double sum = 0.0, whole = 0.0;
+    const int step = 4 * a.lanes;
+    for (int64_t v = lo + 4 * l; v < end; v += kUnits * step) {
+      v4f pv[kUnits], qv[kUnits];
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        r.load((int)min(v + i * step, (int64_t)end), end, pv[i], qv[i]);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        double w[4];
+        r.left((int)v + i * step, pv[i], qv[i], some, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+        if constexpr (kWhole)
+          whole += ((double)pv[i][0] + (double)pv[i][1]) + ((double)pv[i][2] + (double)pv[i][3]);
+      }
+    }
+    sum = wave_sum(sum);
+    if constexpr (kWhole) whole = wave_sum(whole);
+    if (a.lanes > 64) {  // uniform
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) s_sum[0][threadIdx.x >> 6] = sum, s_sum[1][threadIdx.x >> 6] = whole;
+      __syncthreads();
+      sum = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]);
+      whole = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
+    }
+    if (l == 0 && run < kRuns) done(run, sum, whole);
+  }
 }
 
 // Level `level`: the sums of what `level` rejected children leave, by runs of
@@ -617,7 +721,7 @@ __device__ __forceinline__ double block_sum(double v, double *s) {
 __global__ __launch_bounds__(256) void mass_kernel(Verify a, int level) {
   extern __shared__ double s_dyn[];  // [level][64]
   double(*s_inv)[64] = reinterpret_cast<double(*)[64]>(s_dyn);
-  __shared__ double s_sum[4], s_f[kMaxNodes];
+  __shared__ double s_f[kMaxNodes];
   __shared__ uint64_t s_need;
   const int s = blockIdx.y;
   Tree t;
@@ -628,7 +732,6 @@ __global__ __launch_bounds__(256) void mass_kernel(Verify a, int level) {
     if (threadIdx.x == 0) s_need = need;
   }
   __syncthreads();
-  const int len = run_length(a.V);
   for (uint64_t need = s_need; need; need &= need - 1) {
     const int i = __builtin_ctzll(need);
     __syncthreads();
@@ -636,221 +739,187 @@ __global__ __launch_bounds__(256) void mass_kernel(Verify a, int level) {
     __syncthreads();
     const int64_t row = t.start + i;
     const int64_t node = a.packed ? row : (int64_t)s * a.max_nodes + i;
-    for (int x = 0; x < a.per; ++x) {
-      const int run = blockIdx.x * a.per + x;
-      if (run >= kRuns) break;
-      const int64_t lo = (int64_t)run * len;
-      const int end = (int)min(lo + len, (int64_t)a.V);
-      double sum = 0.0;
-      for (int64_t v = lo + 4 * (int)threadIdx.x; v < end; v += 1024) {
-        double w[4];
-        left4(a.target + row * a.ld_target, a.draft + row * a.ld_draft, (int)v, end, level, s_f, w);
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
-      }
-      sum = block_sum(sum, s_sum);
-      if (threadIdx.x == 0) a.mass[((level - 1) * a.nodes + node) * kRuns + run] = sum;
-    }
+    const Row r{a.target + row * a.ld_target, a.draft + row * a.ld_draft, level, 0, s_f, nullptr};
+    sum_runs<false>(a, r, [&](int run, double sum, double) {
+      a.mass[((level - 1) * a.nodes + node) * kRuns + run] = sum;
+    });
   }
 }
 
-// The end of a sequence's walk, and what its last row's w is made of.
-struct Left {
-  int last, gone, n_tokens;  // gone: levels of drawn drafts; n_tokens: tokens that are gone
-  uint64_t path;
-};
-template <bool kDrawn>
-__device__ __forceinline__ bool find_end(const Verify &a, int s, Tree &t, double (*s_inv)[64],
-                                         double *s_f, int64_t *s_tokens, Left *s_left) {
-  if (!load_tree<kDrawn>(a, s, t)) return false;
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    Left e{0, 0, 0, 0};
-    if constexpr (kDrawn) {
-      Tried r;
-      try_drawn(a, s, t, a.max_children - 1, s_inv, r);
-      const uint64_t ends = __ballot(r.reached && r.next < 0);
-      e.last = ends ? __builtin_ctzll(ends) : 0;
-      e.gone = __shfl(r.gone, e.last);
-      if (lane < e.gone) s_f[lane] = s_inv[lane][e.last];
-    } else {
-      const End w = walk_top(t);
-      e.last = w.last;
-      e.n_tokens = __popcll(w.gone);
-      if ((w.gone >> lane) & 1) s_tokens[__popcll(w.gone & ((1ull << lane) - 1))] = t.token;
-    }
-    e.path = __shfl(t.above, e.last);
-    if (lane == 0) *s_left = e;
-  }
-  __syncthreads();
-  return true;
-}
-
-template <bool kDrawn>
-__device__ __forceinline__ void last4(const Verify &a, const Left &e, int64_t row, int v, int end,
-                                      const double *s_f, const int64_t *s_tokens, bool some,
-                                      double (&w)[4]) {
-  left4(a.target + row * a.ld_target, kDrawn ? a.draft + row * a.ld_draft : nullptr, v, end,
-        kDrawn ? e.gone : 0, s_f, w);
-  if (!kDrawn && some)
-    for (int x = 0; x < e.n_tokens; ++x)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (s_tokens[x] == v + j) w[j] = 0.0;
-}
-
-// The last row's w, and its target probabilities, summed by runs.
+// The end of each walk: what was accepted, and the sums of the last row's w and of
+// its target probabilities by runs.  Latency, of loads that wait for each other: starts,
+// the tree, its tokens' probabilities, the row.  (A launch of its own for the draw
+// that follows takes 6 us; drawing in the last of a sequence's workgroups to finish
+// needs each of them to write back L2: 36 us for 16 sequences instead of 17.)
 template <bool kDrawn>
 __global__ __launch_bounds__(256) void last_kernel(Verify a) {
   extern __shared__ double s_dyn[];  // [max_children][64]
-  __shared__ double s_sum[4], s_f[kMaxNodes];
-  __shared__ int64_t s_tokens[kMaxNodes];
-  __shared__ Left s_left;
-  const int s = blockIdx.y;
-  Tree t;
-  if (!find_end<kDrawn>(a, s, t, reinterpret_cast<double(*)[64]>(s_dyn), s_f, s_tokens, &s_left))
-    return;
-  const Left e = s_left;
-  const int64_t row = t.start + e.last;
-  const int len = run_length(a.V);
-  for (int x = 0; x < a.per; ++x) {
-    const int run = blockIdx.x * a.per + x;
-    if (run >= kRuns) break;
-    const int64_t lo = (int64_t)run * len;
-    const int end = (int)min(lo + len, (int64_t)a.V);
-    bool some = false;
-    for (int i = 0; i < e.n_tokens; ++i) some |= s_tokens[i] >= lo && s_tokens[i] < end;
-    double sum = 0.0, whole = 0.0;
-    for (int64_t v = lo + 4 * (int)threadIdx.x; v < end; v += 1024) {
-      double w[4], p[4];
-      left4(a.target + row * a.ld_target, nullptr, (int)v, end, 0, nullptr, p);
-      last4<kDrawn>(a, e, row, (int)v, end, s_f, s_tokens, some, w);
-      sum += (w[0] + w[1]) + (w[2] + w[3]);
-      whole += (p[0] + p[1]) + (p[2] + p[3]);
-    }
-    sum = block_sum(sum, s_sum);
-    whole = block_sum(whole, s_sum);
-    if (threadIdx.x == 0) {
-      a.runs[(size_t)s * kRuns + run] = sum;
-      a.runs[(size_t)(a.seqs + s) * kRuns + run] = whole;
-    }
-  }
-}
-
-__device__ __forceinline__ double wave_scan(double v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const double u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-
-// The next token: the run that holds it, then the lane's elements, then the
-// element.  Then the outputs.
-template <bool kDrawn>
-__global__ __launch_bounds__(256) void pick_kernel(Verify a) {
-  extern __shared__ double s_dyn[];
-  __shared__ double s_sum[4], s_f[kMaxNodes], s_before, s_goal;
-  __shared__ int64_t s_tokens[kMaxNodes];
-  __shared__ Left s_left;
-  __shared__ int s_run, s_whole, s_at;
-  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ Ended s_end;
+  const int s = blockIdx.y, lane = threadIdx.x & 63;
+  const bool first = blockIdx.x == 0;  // writes what was accepted
   int *path = a.path + (size_t)s * a.max_nodes;
   int64_t *emitted = a.emitted + (size_t)s * a.max_nodes;
   Tree t;
-  if (s == 0 && threadIdx.x == 0 && a.refused && a.starts[a.seqs] > a.rows) *a.refused = 1;
-  if (!find_end<kDrawn>(a, s, t, reinterpret_cast<double(*)[64]>(s_dyn), s_f, s_tokens, &s_left)) {
-    if ((int)threadIdx.x < a.max_nodes) path[threadIdx.x] = -1, emitted[threadIdx.x] = -1;
-    if (threadIdx.x == 0) {
-      a.kept[s] = 0, a.next_token[s] = -1;
-      if (t.n != 0 && a.refused) *a.refused = 1;
+  if (!load_tree<kDrawn>(a, s, t)) {  // uniform, and in all workgroups alike
+    if (first && (int)threadIdx.x < a.max_nodes) path[threadIdx.x] = -1, emitted[threadIdx.x] = -1;
+    if (first && threadIdx.x == 0) {
+      a.kept[s] = 0, a.next_token[s] = -1, a.ended[s].row = -1;
+      if (a.refused && (t.n != 0 || (s == 0 && a.starts[a.seqs] > a.rows))) *a.refused = 1;
     }
     return;
   }
-  const Left e = s_left;
   if (threadIdx.x < 64) {
-    const double w = a.runs[(size_t)s * kRuns + lane];
-    const double p = a.runs[(size_t)(a.seqs + s) * kRuns + lane];
-    double upto = wave_scan(w);
-    double total = __shfl(upto, 63);
-    const bool whole = !(total > 0.0);
-    double mine = w;
-    if (whole) upto = wave_scan(p), total = __shfl(upto, 63), mine = p;
-    const double goal = fmax((double)a.sample[s], 0.0) * total;
-    const uint64_t over = __ballot(upto > goal), some = __ballot(mine > 0.0);
-    // (a sample of one or more: the last that there is)
-    const int run = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
-    const double before = __shfl(upto, max(run - 1, 0));
-    if (lane == 0) {
-      s_run = total > 0.0 && total < INFINITY ? run : -1;
-      s_whole = whole, s_goal = goal, s_before = run > 0 ? before : 0.0, s_at = -1;
+    int last, gone = 0, n_tokens = 0;
+    if constexpr (kDrawn) {
+      double(*s_inv)[64] = reinterpret_cast<double(*)[64]>(s_dyn);
+      Tried r;
+      try_drawn(a, s, t, a.max_children - 1, s_inv, r);
+      const uint64_t ends = __ballot(r.reached && r.next < 0);
+      last = ends ? __builtin_ctzll(ends) : 0;
+      gone = lane_of(r.gone, last);
+      if (lane < gone) s_end.inv[lane] = s_inv[lane][last];
+    } else {
+      const End w = walk_top(t);
+      last = w.last, n_tokens = __popcll(w.gone);
+      if ((w.gone >> lane) & 1) s_end.tokens[__popcll(w.gone & ((1ull << lane) - 1))] = t.token;
+    }
+    const uint64_t way = lane_of(t.above, last);
+    const int kept = __popcll(way);
+    if (lane == 0)
+      s_end.row = t.start + last, s_end.kept = kept, s_end.gone = gone, s_end.n_tokens = n_tokens;
+    if (first) {
+      const int place = __popcll(way & ((1ull << lane) - 1));
+      if ((way >> lane) & 1) {
+        path[place] = lane;
+        if (place > 0) emitted[place - 1] = t.token;
+      }
+      if (lane >= kept && lane < a.max_nodes) path[lane] = -1, emitted[lane] = -1;
+      const bool strange = __any(lane > 0 && lane < t.n && !t.in);
+      if (lane == 0) {
+        a.kept[s] = kept;
+        if (a.refused && (strange || (s == 0 && a.starts[a.seqs] > a.rows))) *a.refused = 1;
+      }
     }
   }
   __syncthreads();
-  const int run = s_run;
-  if (run >= 0) {  // uniform
-    const int64_t row = t.start + e.last;
-    const int len = run_length(a.V), lo = run * len;  // (run has elements)
-    const int end = min(lo + len, a.V);
-    const int each = ((end - lo + 255) / 256 + 3) / 4 * 4;
-    const int v0 = min(lo + each * (int)threadIdx.x, end), v1 = min(v0 + each, end);
-    Left way = e;
-    if (s_whole) way.gone = way.n_tokens = 0;
-    double sum = 0.0;
-    for (int v = v0; v < v1; v += 4) {
-      double w[4];
-      last4<kDrawn>(a, way, row, v, v1, s_f, s_tokens, true, w);
-      sum += (w[0] + w[1]) + (w[2] + w[3]);
+  const Row r{a.target + s_end.row * a.ld_target,
+              kDrawn ? a.draft + s_end.row * a.ld_draft : nullptr, s_end.gone, s_end.n_tokens,
+              s_end.inv, s_end.tokens};
+  sum_runs<true>(a, r, [&](int run, double sum, double whole) {
+    a.runs[(size_t)s * kRuns + run] = sum;
+    a.runs[(size_t)(a.seqs + s) * kRuns + run] = whole;
+  });
+  if (first) {  // for the next kernel
+    const int words = (int)(sizeof(Ended) / 8);
+    for (int i = threadIdx.x; i < words; i += 256)
+      reinterpret_cast<uint64_t *>(a.ended + s)[i] = reinterpret_cast<const uint64_t *>(&s_end)[i];
+  }
+}
+
+// The next token: the run that holds it, then the thread's elements, then the
+// element.  Two dependent loads and three scans.
+constexpr int kHeld = 4;  // units of four elements that stay in registers
+template <bool kDrawn>
+__global__ __launch_bounds__(256) void pick_kernel(Verify a) {
+  __shared__ Ended s_end;
+  __shared__ double s_sum[4], s_before, s_goal;
+  __shared__ int s_run, s_whole, s_first, s_last;
+  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Ended *ended = a.ended + s;
+  const int64_t row = ended->row;
+  if (threadIdx.x < 64) {
+    const double sum_w = a.runs[(size_t)s * kRuns + lane];
+    const double sum_p = a.runs[(size_t)(a.seqs + s) * kRuns + lane];
+    const double sample = (double)a.sample[s];
+    double upto = wave_scan(sum_w);
+    double total = lane_of(upto, 63), mine = sum_w;
+    const bool whole = !(total > 0.0);
+    if (whole) upto = wave_scan(sum_p), total = lane_of(upto, 63), mine = sum_p;
+    const double goal = fmax(sample, 0.0) * total;
+    const uint64_t over = __ballot(upto > goal), some = __ballot(mine > 0.0);
+    // (a sample of one or more: the last that there is)
+    const int run = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+    const double before = lane_of(upto, max(run - 1, 0));
+    if (lane == 0) {
+      s_run = total > 0.0 && total < INFINITY ? run : -1;
+      s_whole = whole, s_goal = goal, s_before = run > 0 ? before : 0.0;
+      s_first = 0x7fffffff, s_last = -1;
     }
-    const double upto = wave_scan(sum);
-    if (lane == 63) s_sum[wave] = upto;
-    __syncthreads();
-    double before = s_before + (upto - sum);
-    for (int x = 0; x < wave; ++x) before += s_sum[x];
-    // The first element that passes the goal; where rounding leaves none, the last
-    // above zero.
-    int first = 0x7fffffff, last = -1;
-    for (int v = v0; v < v1; v += 4) {
-      double w[4];
-      last4<kDrawn>(a, way, row, v, v1, s_f, s_tokens, true, w);
+  } else if (threadIdx.x < 128) {
+    s_end.tokens[lane] = ended->tokens[lane];  // (some were never written, nor are read)
+    s_end.inv[lane] = ended->inv[lane];
+    if (lane == 0)
+      s_end.kept = ended->kept, s_end.gone = ended->gone, s_end.n_tokens = ended->n_tokens;
+  }
+  if (row < 0) return;  // uniform
+  __syncthreads();
+  const int run = s_run;
+  int64_t *next = a.emitted + (size_t)s * a.max_nodes + s_end.kept - 1;
+  if (run < 0) {  // uniform
+    if (threadIdx.x == 0) {
+      *next = a.next_token[s] = -1;
+      if (a.refused) *a.refused = 1;
+    }
+    return;
+  }
+  const int len = run_length(a.V), lo = run * len;  // (run has elements)
+  const int end = min(lo + len, a.V);
+  const int each = ((end - lo + 255) / 256 + 3) / 4 * 4;
+  const int v0 = min(lo + each * (int)threadIdx.x, end), v1 = min(v0 + each, end);
+  const Row r{a.target + row * a.ld_target, kDrawn ? a.draft + row * a.ld_draft : nullptr,
+              s_whole ? 0 : s_end.gone, s_whole ? 0 : s_end.n_tokens, s_end.inv, s_end.tokens};
+  const bool some = r.any_token(lo, end);
+  v4f pv[kHeld], qv[kHeld];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        before += w[j];
-        if (w[j] > 0.0) {
-          if (before > s_goal) first = min(first, v + j);
-          last = v + j;
-        }
+  for (int i = 0; i < kHeld; ++i) r.load(min(v0 + 4 * i, v1), v1, pv[i], qv[i]);
+  auto each_unit = [&](auto use) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      double w[4];
+      r.left(v0 + 4 * i, pv[i], qv[i], some, w);
+      use(v0 + 4 * i, w);
+    }
+    for (int v = v0 + 4 * kHeld; v < v1; v += 4) {
+      v4f p, q;
+      double w[4];
+      r.load(v, v1, p, q);
+      r.left(v, p, q, some, w);
+      use(v, w);
+    }
+  };
+  double sum = 0.0;
+  each_unit([&](int, const double(&w)[4]) { sum += (w[0] + w[1]) + (w[2] + w[3]); });
+  const double upto = wave_scan(sum);
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+  double before = s_before + (upto - sum);
+  for (int x = 0; x < wave; ++x) before += s_sum[x];
+  // The first element that passes the goal; where rounding leaves none, the last
+  // above zero.
+  int first = 0x7fffffff, last = -1;
+  each_unit([&](int v, const double(&w)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      before += w[j];
+      if (w[j] > 0.0) {
+        if (before > s_goal) first = min(first, v + j);
+        last = v + j;
       }
     }
-    __shared__ int s_first, s_last;
-    if (threadIdx.x == 0) s_first = 0x7fffffff, s_last = -1;
-    __syncthreads();
-    if (first != 0x7fffffff) atomicMin(&s_first, first);
-    if (last >= 0) atomicMax(&s_last, last);
-    __syncthreads();
-    if (threadIdx.x == 0) s_at = s_first != 0x7fffffff ? s_first : s_last;
-    __syncthreads();
-  }
-  if (threadIdx.x >= 64) return;
-  const int kept = __popcll(e.path);
-  const bool on = (e.path >> lane) & 1;
-  const int place = __popcll(e.path & ((1ull << lane) - 1));
-  if (on) {
-    path[place] = lane;
-    if (place > 0) emitted[place - 1] = t.token;
-  }
-  if (lane >= kept && lane < a.max_nodes) path[lane] = -1, emitted[lane] = -1;
-  const bool strange = __any(lane > 0 && lane < t.n && !t.in);
-  if (lane == 0) {
-    emitted[kept - 1] = s_at;
-    a.kept[s] = kept, a.next_token[s] = s_at;
-    if ((s_at < 0 || strange) && a.refused) *a.refused = 1;
+  });
+  if (first != 0x7fffffff) atomicMin(&s_first, first);
+  if (last >= 0) atomicMax(&s_last, last);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int at = s_first != 0x7fffffff ? s_first : s_last;
+    *next = a.next_token[s] = at;
+    if (at < 0 && a.refused) *a.refused = 1;
   }
 }
 
 // ------------------------------------------------------- the cache's rows
 
-constexpr int kKeepPools = 128;
+constexpr int kKeepPools = 128, kKeepAtOnce = 8;
 struct Keep {
   const int *starts, *lengths, *table, *kept, *path;
   int *refused;
@@ -859,9 +928,11 @@ struct Keep {
   uint8_t *pool[kKeepPools];
 };
 
-// Workgroup: one sequence, `per` (pool, head) pairs, a wave each in turn.  Rows
-// move to earlier places and no further than the row before them, so a wave that
-// takes them in order, 64 / units at a time, never reads what it has written.
+// Workgroup: one sequence, `per` (pool, head) pairs, a wave kKeepAtOnce of them at a
+// time.  Rows move to earlier places and no further than the row before them, so a
+// wave that takes a pair's rows in order, 64 / units at a time, never reads what it
+// has written.  Latency of small moves: 64 sequences' paths in 36 layers (some 3 rows
+// each, 44 MB) 12 us, 15 with a pair at a time.
 __global__ __launch_bounds__(256) void keep_kernel(Keep a) {
   __shared__ uint32_t s_from[kMaxNodes], s_to[kMaxNodes];
   const int s = blockIdx.y, lane = threadIdx.x & 63;
@@ -893,12 +964,23 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep a) {
   __syncthreads();
   const int unit = lane % a.units, sub = lane / a.units, step = 64 / a.units;
   const int end = min((int)(blockIdx.x + 1) * a.per, a.n * a.Hkv);
-  for (int i = blockIdx.x * a.per + wave; i < end; i += 4) {
-    const uint32_t head = (uint32_t)(i % a.Hkv) << a.shift;
-    u32x4 *pool = reinterpret_cast<u32x4 *>(a.pool[i / a.Hkv]);
-    for (int r = sub; r < moved; r += step) {
-      const u32x4 v = pool[(size_t)(s_from[r] + head) * a.units + unit];
-      pool[(size_t)(s_to[r] + head) * a.units + unit] = v;
+  for (int i0 = blockIdx.x * a.per + wave; i0 < end; i0 += 4 * kKeepAtOnce) {
+    u32x4 *pool[kKeepAtOnce];  // of the pair, at its head
+#pragma unroll
+    for (int x = 0; x < kKeepAtOnce; ++x) {
+      const int i = min(i0 + 4 * x, end - 1);
+      pool[x] = reinterpret_cast<u32x4 *>(a.pool[i / a.Hkv]) +
+                (((size_t)(i % a.Hkv) << a.shift) * a.units + unit);
+    }
+    for (int r = sub; r - sub < moved; r += step) {  // uniform
+      const int row = min(r, moved - 1);
+      const size_t from = (size_t)s_from[row] * a.units, to = (size_t)s_to[row] * a.units;
+      u32x4 v[kKeepAtOnce];
+#pragma unroll
+      for (int x = 0; x < kKeepAtOnce; ++x) v[x] = pool[x][from];
+#pragma unroll
+      for (int x = 0; x < kKeepAtOnce; ++x)
+        if (r < moved && i0 + 4 * x < end) pool[x][to] = v[x];
     }
   }
 }
@@ -987,16 +1069,17 @@ extern "C" int ecf8_draft_verify(const ecf8_paged_batch *b, const ecf8_draft_tre
   Verify a{b->starts, t->parents, tokens, target, draft, accept, sample, ld_target, ld_draft,
            t->kept, t->path, b->refused, t->emitted, t->next_token,
            reinterpret_cast<double *>(base + w.runs), reinterpret_cast<double *>(base + w.mass),
-           w.nodes, b->seqs, (int)rows, (int)V, t->max_nodes, t->max_children, w.packed, 1};
-  const int64_t per = (int64_t)b->seqs * kRuns / 2048;
-  a.per = per < 1 ? 1 : per > 8 ? 8 : (int)per;
-  const dim3 grid((unsigned)((kRuns + a.per - 1) / a.per), (unsigned)b->seqs);
+           reinterpret_cast<Ended *>(base + w.ended), w.nodes, b->seqs, (int)rows, (int)V,
+           t->max_nodes, t->max_children, w.packed, 1, 256};
+  // a wave a run once that leaves four workgroups a CU
+  if (b->seqs * (kRuns / 4) >= 1024) a.per = 4, a.lanes = 64;
+  const dim3 grid((unsigned)(kRuns / a.per), (unsigned)b->seqs);
   const unsigned lds = draft ? (unsigned)(t->max_children * 64 * sizeof(double)) : 0;
   if (draft) {
     for (int level = 1; level < t->max_children; ++level)
       mass_kernel<<<grid, 256, lds, as_stream(stream)>>>(a, level);
     last_kernel<true><<<grid, 256, lds, as_stream(stream)>>>(a);
-    pick_kernel<true><<<(unsigned)b->seqs, 256, lds, as_stream(stream)>>>(a);
+    pick_kernel<true><<<(unsigned)b->seqs, 256, 0, as_stream(stream)>>>(a);
   } else {
     last_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(a);
     pick_kernel<false><<<(unsigned)b->seqs, 256, 0, as_stream(stream)>>>(a);
@@ -1020,8 +1103,10 @@ extern "C" int ecf8_draft_keep(const ecf8_paged_batch *b, const ecf8_draft_trees
   for (int i0 = 0; i0 < n_pools; i0 += kKeepPools) {
     a.n = n_pools - i0 < kKeepPools ? n_pools - i0 : kKeepPools;
     for (int i = 0; i < a.n; ++i) a.pool[i] = static_cast<uint8_t *>(pools[i0 + i]);
+    // a thousand workgroups, and whole turns of their waves
     const int64_t pairs = (int64_t)a.n * a.Hkv, each = pairs * b->seqs / 1024;
-    a.per = each < 4 ? 4 : (int)each;
+    constexpr int kTurn = 4 * kKeepAtOnce;
+    a.per = each < 4 ? 4 : each < kTurn ? (int)each : (int)(each / kTurn * kTurn);
     const dim3 grid((unsigned)((pairs + a.per - 1) / a.per), (unsigned)b->seqs);
     keep_kernel<<<grid, 256, 0, as_stream(stream)>>>(a);
   }

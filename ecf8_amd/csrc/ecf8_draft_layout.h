@@ -19,6 +19,7 @@ constexpr int kMaxNodes = 64;  // a row's mask is 64 bits
 constexpr int kUnitKeys = 128; // key ranges are cut at multiples
 // Runs of the vocabulary that a row's probabilities are summed by.
 constexpr int kRuns = 64;
+constexpr int kEndedBytes = 1056;  // of where a sequence's walk ended
 
 // Rows (token, head of the group) of a workgroup of the attention.
 inline int tile_rows(int max_nodes, int group) {
@@ -37,7 +38,7 @@ struct Counts {
 struct Work {
   int tile, target, parts, items;
   int64_t items_at, joins_at, stats, sums;  // of the attention
-  int64_t runs, mass, bytes;                // of the verification
+  int64_t runs, ended, mass, bytes;         // of the verification
   int64_t nodes;                            // rows that a step of trees can have
   bool packed;  // they are the step's rows (else max_nodes a sequence)
 };
@@ -65,6 +66,7 @@ inline Work work_layout(int64_t seqs, int64_t rows, int Hq, int Hkv, int max_nod
   w.sums = take(w.parts * (int64_t)Hkv * part_rows * kD * 4);
   // sums of what is left and of the target's own, by runs
   w.runs = take(2 * seqs * kRuns * 8);
+  w.ended = take(seqs * kEndedBytes);
   // of each row with children, what is left after one, two, ... of them
   w.mass = take(max_children > 1 ? (max_children - 1) * w.nodes * kRuns * 8 : 0);
   w.bytes = at;
