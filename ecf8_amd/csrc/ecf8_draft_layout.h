@@ -24,10 +24,10 @@ constexpr int kEndedBytes = 1056;  // of where a sequence's walk ended
 // Rows (token, head of the group) of a workgroup of the attention.
 inline int tile_rows(int max_nodes, int group) {
   const int r = max_nodes * group;
-  return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128;
+  return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256;
 }
-// Workgroups that a split aims at, over all KV heads: two a CU.
-constexpr int kSlots = 512;
+// Workgroups that a split aims at, over all KV heads: two a CU, one of 256 rows.
+inline int slots(int tile) { return tile <= 128 ? 512 : 256; }
 
 struct Counts {
   int items, joins;
@@ -48,7 +48,7 @@ inline Work work_layout(int64_t seqs, int64_t rows, int Hq, int Hkv, int max_nod
   Work w;
   const int G = Hq / Hkv;
   w.tile = tile_rows(max_nodes, G);
-  w.target = kSlots / Hkv > 1 ? kSlots / Hkv : 1;
+  w.target = slots(w.tile) / Hkv > 1 ? slots(w.tile) / Hkv : 1;
   w.parts = 2 * w.target;
   w.packed = rows <= seqs * max_nodes;
   w.nodes = w.packed ? rows : seqs * max_nodes;

@@ -1268,13 +1268,16 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 // neither hides the other: 2100 cycles a step of both instead of 1220, T = 2).
 // Keys and values go through registers, kDepth steps ahead, to a ring of LDS
 // stages.
-template <Source kSrc, int T, bool kFine, bool kOnce>
-__global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
+template <Source kSrc, int kWaves, int T, bool kFine, bool kOnce>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
   constexpr int kDepth = 2;
-  constexpr int kRows = 64 * T;
+  constexpr int kRows = 16 * T * kWaves, kThreads = 64 * kWaves;
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;               // 16-byte units of a row in memory
-  constexpr int kPass = 256 / kUnits, kLoads = 32 / kPass;
+  // rows a pass of the threads; twice a step's: keys and values have half of them each
+  constexpr int kPass = kThreads / kUnits;
+  constexpr bool kHalves = kPass > 32;
+  constexpr int kLoads = kHalves ? 1 : 32 / kPass;
   // after the barrier before step j the waves read steps j - 1 to j + 1 and write j + 2
   constexpr int kRing = 4;
   __shared__ u32x4 s_kv[kRing][32 * (kKeyRow + kValueRow)];
@@ -1293,7 +1296,9 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
 
   // load i of a step: row kPass i + sub of its keys and values.  kTail: past the
   // end the last row again.
-  const int unit = (int)threadIdx.x % kUnits, sub = (int)threadIdx.x / kUnits;
+  const int unit = (int)threadIdx.x % kUnits;
+  const int sub = (int)threadIdx.x / kUnits % (kHalves ? 32 : kPass);
+  const bool key_half = !kHalves || (int)threadIdx.x < kThreads / 2;
   const int *table = a.table + (size_t)p.seq * a.width;
   const int steps = (p.k1 - p.k0 + 31) / 32;
   auto key_of = [&](auto tail, int j, int i) {
@@ -1301,8 +1306,8 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
     return decltype(tail)::value ? min(key, p.k1 - 1) : key;
   };
   struct Staged {
-    u32x4 k[kLoads], v[kLoads];
-    int entry[kLoads];  // pages of the step kDepth later
+    u32x4 k[kLoads], v[kHalves ? 1 : kLoads];  // (kHalves: k alone, a key or a value)
+    int entry[kLoads];                         // pages of the step kDepth later
   };
   auto look = [&](auto tail, int j, Staged &r) {
 #pragma unroll
@@ -1323,7 +1328,8 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
         const u32x4 *x = static_cast<const u32x4 *>(pool) + at[i];
         return kOnce ? __builtin_nontemporal_load(x) : *x;
       };
-      r.k[i] = get(a.k), r.v[i] = get(a.v);
+      r.k[i] = get(key_half ? a.k : a.v);
+      if constexpr (!kHalves) r.v[i] = get(a.v);
     }
   };
   auto store = [&](auto tail, int j, const Staged &r) {
@@ -1341,11 +1347,15 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Attn a) {
       if constexpr (kFp8) {
         u32x4 w[2];
         widen16_pairs(r.k[i], w);
-        s_k[row * kKeyRow + 2 * unit] = w[0];
-        s_k[row * kKeyRow + 2 * unit + 1] = w[1];
-        widen16_pairs(r.v[i], w);
-        s_v[row * kValueRow + 2 * unit] = finite(w[0]);
-        s_v[row * kValueRow + 2 * unit + 1] = finite(w[1]);
+        if (key_half) {
+          s_k[row * kKeyRow + 2 * unit] = w[0];
+          s_k[row * kKeyRow + 2 * unit + 1] = w[1];
+        }
+        if constexpr (!kHalves) widen16_pairs(r.v[i], w);
+        if (!kHalves || !key_half) {
+          s_v[row * kValueRow + 2 * unit] = finite(w[0]);
+          s_v[row * kValueRow + 2 * unit + 1] = finite(w[1]);
+        }
       } else {
         s_k[row * kKeyRow + unit] = r.k[i];
         s_v[row * kValueRow + unit] = finite(r.v[i]);
@@ -1745,10 +1755,10 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
     if (fp8) few_kernel<kPagesFp8, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);      \
     else few_kernel<kPages, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);             \
   } while (0)
-#define ECF8_TREE(T, F, O)                                                             \
-  do {                                                                                    \
-    if (fp8) tree_kernel<kPagesFp8, T, F, O><<<grid, 256, 0, as_stream(stream)>>>(a);  \
-    else tree_kernel<kPages, T, F, O><<<grid, 256, 0, as_stream(stream)>>>(a);         \
+#define ECF8_TREE(W, T, F, O)                                                                   \
+  do {                                                                                          \
+    if (fp8) tree_kernel<kPagesFp8, W, T, F, O><<<grid, 64 * W, 0, as_stream(stream)>>>(a);     \
+    else tree_kernel<kPages, W, T, F, O><<<grid, 64 * W, 0, as_stream(stream)>>>(a);            \
   } while (0)
   switch (w.tile) {
     case 16:
@@ -1758,11 +1768,14 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
       ECF8_TREE_FEW(2);
       break;
     case 64:
-      ECF8_TREE(1, true, true);
+      ECF8_TREE(4, 1, true, true);
       break;
-    default:
-      if (trees->max_nodes * a.group <= 128) ECF8_TREE(2, false, true);
-      else ECF8_TREE(2, false, false);  // tiles of a sequence share its pages in L2
+    case 128:
+      ECF8_TREE(4, 2, false, true);
+      break;
+    default:  // (tiles of a sequence share its pages in L2)
+      if (trees->max_nodes * a.group <= 256) ECF8_TREE(8, 2, false, true);
+      else ECF8_TREE(8, 2, false, false);
   }
 #undef ECF8_TREE_FEW
 #undef ECF8_TREE
