@@ -233,6 +233,31 @@ def test_attention_of_split_keys(cuda_device, Hq, Hkv, nodes, cached, fp8):
         _check(out[at].view(nodes, Hq, D), want, A, nodes * (Hq // Hkv) <= 64)
 
 
+@pytest.mark.parametrize("Hq,Hkv,nodes", [(4, 1, 3), (8, 1, 8), (16, 1, 9)])
+def test_attention_of_thousands_of_sequences(cuda_device, Hq, Hkv, nodes):
+    """More tiles than the plan has threads, in a batch with room for more rows than
+    its trees can have: equal values of a sequence, so each output is its value."""
+    from ecf8_amd.draft_kernels import draft_attention
+
+    dev, S, rng = cuda_device, 2500, random.Random(nodes)
+    new = [rng.choice([0, 1, nodes]) for _ in range(S)]
+    cached = [rng.choice([0, 3, 40]) for _ in range(S)]
+    cached[7], new[7] = 9000, nodes
+    trees = [M.random_tree(rng, n, 3) for n in new]
+    b, t, _ = _step(dev, cached, trees, 16, Hq, Hkv, max_nodes=nodes, rows=S * nodes + 1000)
+    owner = torch.zeros(b.pages, dtype=torch.float32, device=dev)
+    for s in range(S):
+        owner[b.table[s, : int(b.owned[s])].long()] = s % 256 - 100
+    pool = owner[:, None, None, None].expand(-1, Hkv, 16, D).bfloat16().contiguous()
+    q = torch.randn(sum(new), Hq, D, generator=torch.Generator(device=dev).manual_seed(1),
+                    device=dev).bfloat16()
+    out = torch.full((sum(new), Hq * D), 7.0, dtype=torch.bfloat16, device=dev)
+    draft_attention(q, torch.zeros_like(pool), pool, t, out)
+    assert not _refused(b)
+    want = _ints([s % 256 - 100 for s in range(S) for _ in range(new[s])], dev).float()
+    assert bool((out.float() == want[:, None]).all())
+
+
 @pytest.mark.parametrize("Hq,Hkv", [(4, 4), (8, 2), (16, 2), (32, 2), (32, 1)])
 @pytest.mark.parametrize("cached", [0, 5, 31, 32, 300, 3000])
 def test_masks_of_the_callers_own(cuda_device, cached, Hq, Hkv):
@@ -492,6 +517,32 @@ def _drafted(trees, draft, gen, drawn):
             given[p] += 1
         a += len(tree)
     return tokens
+
+
+@pytest.mark.parametrize("rows", [None, 1000])
+@pytest.mark.parametrize("V", [1, 2, 255, 257])
+def test_verify_of_small_vocabularies_in_large_batches(cuda_device, V, rows):
+    """A batch with room for more rows than its trees can have; one token."""
+    from ecf8_amd.draft_kernels import draft_verify
+
+    dev, S, n, rng = cuda_device, 7, 9, random.Random(V)
+    gen = torch.Generator(device=dev).manual_seed(V)
+    trees = [M.random_tree(rng, rng.choice([n, 4, 0]), 3) for _ in range(S)]
+    b, t, _ = _step(dev, [5] * S, trees, 16, max_nodes=n, kids=3, rows=rows)
+    N = sum(len(x) for x in trees)
+    target, draft = _distributions(N, V, gen, 1.0, 0.7)
+    tokens = _drafted(trees, draft, gen, True)
+    accept, sample = (torch.rand(k, generator=gen, device=dev) for k in (N, S))
+    draft_verify(t, _ints(tokens, dev, torch.int64), target, accept, sample, draft=draft)
+    assert not _refused(b)
+    a = 0
+    for s, tree in enumerate(trees):
+        k = len(tree)
+        if k:
+            assert _verified(t, s) == M.verify(
+                tree, tokens[a: a + k], target[a: a + k].double().cpu(), accept[a: a + k].tolist(),
+                float(sample[s]), draft[a: a + k].double().cpu())
+        a += k
 
 
 def _verified(t, s):
