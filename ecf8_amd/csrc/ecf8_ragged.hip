@@ -167,8 +167,10 @@ struct Operands {
 // parts of bf16, where the matrix unit has nothing better to do; the error
 // against 64 bits is then the output's rounding, and else 1.4 times that.
 // kAhead: operands are read from LDS this many ahead of their products (and not all
-// at once, which would take registers that the other operands live in).
-template <int T, bool kFine = false, int kAhead = 1>
+// at once, which would take registers that the other operands live in).  kFirst: the
+// wave goes before the SIMD's other one while it mixes products and softmax, and
+// after it in the scores, which are products alone (trees: 2 to 5% of the time).
+template <int T, bool kFine = false, int kAhead = 1, bool kFirst = false>
 struct Rows {
   v4f o[T][8];
   // of the lane's query (alike in its four lanes): the whole number that its
@@ -323,6 +325,7 @@ struct Rows {
   __device__ __forceinline__ void stream(lds_u8 *v, lds_u8 *k, u32x4 (&was)[T],
                                          const v8bf (&q)[T][4], v4f (&s)[T][2], float c,
                                          Between between) {
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
     u32x4 f[kAhead + 1], p[T], rest[kFine ? T : 1];
     if constexpr (kFine) {
 #pragma unroll
@@ -366,6 +369,7 @@ struct Rows {
     if (__any((bits & 0x40004000u) != 0)) raise(s, c, p, false);
 #pragma unroll
     for (int t = 0; t < T; ++t) was[t] = p[t];
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i + kAhead < 8) f[(8 + i + kAhead) % (kAhead + 1)] = operand(v, k, 8 + i + kAhead);
@@ -1270,7 +1274,8 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 // stages.
 template <Source kSrc, int kWaves, int T, bool kFine, bool kOnce>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
-  constexpr int kDepth = 2;
+  // (three steps for e4m3, half the bytes: 64-node trees after 32768 192 -> 187 us)
+  constexpr int kDepth = kWaves == 8 && kSrc == kPagesFp8 ? 3 : 2;
   constexpr int kRows = 16 * T * kWaves, kThreads = 64 * kWaves;
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;               // 16-byte units of a row in memory
@@ -1425,7 +1430,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
       }
     return;
   }
-  Rows<T, kFine, 2> w;
+  Rows<T, kFine, 2, true> w;
   w.init();
   v4f s[T][2];
   u32x4 pr[T];
