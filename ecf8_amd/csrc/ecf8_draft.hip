@@ -35,13 +35,16 @@ struct Plan {
   Counts *counts;
   Item *items;
   Join *joins;
-  int seqs, rows, all_rows, group, max_nodes, max_children, tile, target, begin;
+  int seqs, rows, all_rows, group, max_nodes, max_children, tile, target;
   uint64_t stamp;
 };
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPer = kMaxSeqs / kPlanThreads;
 constexpr int kLeast = 1;  // units on both sides of a cut
+// What a workgroup's first loads and last sums take, in units.  64 trees after 512
+// keys: of 8 tokens 26.6 us, 29.8 with one; of 32 39 and 47; few long ones alike.
+constexpr int kBegin = 5;
 
 // The exclusive prefix sums of N values over the workgroup, and their totals.
 // Calls in a row alternate between two halves of `waves`.
@@ -115,7 +118,7 @@ __device__ __forceinline__ int bucket_of(int length, int share) {
 }
 
 // The attention's schedule, by one workgroup.  Every (sequence, tile of rows)
-// has ceil(length / kUnitKeys) units, and begin for its first loads and last
+// has ceil(length / kUnitKeys) units, and kBegin for its first loads and last
 // sums; laid end to end they are cut at the multiples of a workgroup's share, and
 // the pieces listed from the longest on.
 __device__ __forceinline__ void plan_schedule(const Plan &a) {
@@ -135,7 +138,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
     if (n < 1 || n > a.max_nodes || start < 0 || start > a.rows - n || len < n) continue;
     tiles[i] = (n * a.group + a.tile - 1) / a.tile;
     sum += tiles[i];
-    units += tiles[i] * ((len + kUnitKeys - 1) / kUnitKeys + a.begin);
+    units += tiles[i] * ((len + kUnitKeys - 1) / kUnitKeys + kBegin);
   }
   // (the sum of all can pass 32 bits, a thread's cannot)
   const int one[1] = {sum}, halves[2] = {units & 0xffff, units >> 16};
@@ -176,10 +179,10 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
       t.len = a.lengths[lo], t.it.cached = t.len - t.it.n;
       t.units = (t.len + kUnitKeys - 1) / kUnitKeys;
     }
-    const int all_units[1] = {t.units ? t.units + a.begin : 0};
+    const int all_units[1] = {t.units ? t.units + kBegin : 0};
     int from[1], total[1];
     block_scan(all_units, s_waves[0], from, total);
-    t.f = from0 + from[0] + a.begin;
+    t.f = from0 + from[0] + kBegin;
     t.c0 = (t.f + kLeast + share - 1) / share;
     const int c1 = (t.f + t.units - kLeast) / share;
     t.k = t.units ? max(0, c1 - t.c0 + 1) + 1 : 0;
@@ -224,7 +227,8 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
   if (tid == 0) *a.counts = Counts{n_items, n_joins, a.stamp};
 }
 
-// The first workgroup schedules, the others take 16 sequences' trees each.
+// The first workgroup schedules, the others take 16 sequences' trees each.  Latency of
+// loads, scans and barriers in a row: 6.5 us of one tree, 7.5 of 512.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   if (blockIdx.x == 0) {
     plan_schedule(a);
@@ -707,7 +711,8 @@ __device__ __forceinline__ void sum_runs(const Verify &a, const Row &r, Done don
     if constexpr (kWhole) whole = wave_sum(whole);
     if (a.lanes > 64) {  // uniform
       __syncthreads();
-      if ((threadIdx.x & 63) == 0) s_sum[0][threadIdx.x >> 6] = sum, s_sum[1][threadIdx.x >> 6] = whole;
+      if ((threadIdx.x & 63) == 0)
+        s_sum[0][threadIdx.x >> 6] = sum, s_sum[1][threadIdx.x >> 6] = whole;
       __syncthreads();
       sum = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]);
       whole = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
@@ -954,8 +959,8 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep a) {
   const int first = __builtin_ctzll(moves), moved = kept - first;  // (and all after it)
   if (threadIdx.x < 64 && lane >= first && lane < kept) {
     auto slot = [&](int pos) {
-      const uint32_t page =
-          min((uint32_t)a.table[(size_t)s * a.width + min(pos >> a.shift, a.width - 1)], a.pages - 1);
+      const int at = min(pos >> a.shift, a.width - 1);
+      const uint32_t page = min((uint32_t)a.table[(size_t)s * a.width + at], a.pages - 1);
       return ((page * a.Hkv) << a.shift) + (uint32_t)(pos & ((1 << a.shift) - 1));
     };
     s_from[lane - first] = slot(cached + row);
@@ -1014,8 +1019,9 @@ extern "C" int ecf8_draft_plan(const ecf8_paged_batch *b, const ecf8_draft_trees
   auto *base = static_cast<uint8_t *>(t->work);
   const Plan a{b->starts, b->lengths, parents, t->masks, t->parents, b->positions, b->refused,
                reinterpret_cast<Counts *>(base), reinterpret_cast<Item *>(base + w.items_at),
-               reinterpret_cast<Join *>(base + w.joins_at), b->seqs, (int)rows, b->rows, b->Hq / b->Hkv,
-               t->max_nodes, t->max_children, w.tile, w.target, w.tile <= 32 ? 1 : 5, schedule_stamp(b, t)};
+               reinterpret_cast<Join *>(base + w.joins_at), b->seqs, (int)rows, b->rows,
+               b->Hq / b->Hkv, t->max_nodes, t->max_children, w.tile, w.target,
+               schedule_stamp(b, t)};
   const unsigned grid = 1 + (unsigned)((b->seqs + kPlanWaves - 1) / kPlanWaves);
   plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
   return launched();
@@ -1071,7 +1077,8 @@ extern "C" int ecf8_draft_verify(const ecf8_paged_batch *b, const ecf8_draft_tre
            reinterpret_cast<double *>(base + w.runs), reinterpret_cast<double *>(base + w.mass),
            reinterpret_cast<Ended *>(base + w.ended), w.nodes, b->seqs, (int)rows, (int)V,
            t->max_nodes, t->max_children, w.packed, 1, 256};
-  // a wave a run once that leaves four workgroups a CU
+  // A wave a run once that leaves four workgroups a CU.  64 chains of 5 drawn from 32000:
+  // 15 us, 22 with four waves; 8 trees of 32 from 151936: 32 with four, 39 with one.
   if (b->seqs * (kRuns / 4) >= 1024) a.per = 4, a.lanes = 64;
   const dim3 grid((unsigned)(kRuns / a.per), (unsigned)b->seqs);
   const unsigned lds = draft ? (unsigned)(t->max_children * 64 * sizeof(double)) : 0;

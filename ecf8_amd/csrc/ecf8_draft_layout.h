@@ -21,12 +21,18 @@ constexpr int kUnitKeys = 128; // key ranges are cut at multiples
 constexpr int kRuns = 64;
 constexpr int kEndedBytes = 1056;  // of where a sequence's walk ended
 
-// Rows (token, head of the group) of a workgroup of the attention.
+// Rows (token, head of the group) of a workgroup of the attention: what a sequence
+// has, in as few workgroups as registers allow, since each reads the sequence's pages.
+// One tree of 8 in groups of four after 4096: 12.6 us in 32 rows, 13.2 in 64; 16 trees
+// of 32 after 8192 e4m3 keys 63 in 128, 72 in 256; of 64 after as many bf16 ones 95 in
+// 256, 109 in two of 128.
 inline int tile_rows(int max_nodes, int group) {
   const int r = max_nodes * group;
   return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256;
 }
-// Workgroups that a split aims at, over all KV heads: two a CU, one of 256 rows.
+// Workgroups that a split aims at, over all KV heads: two a CU, one of 256 rows.  64
+// chains of 5 after up to 8192: 177 us, 205 with 256; 16 trees of 64 after 8192: 95,
+// 109 with 512.
 inline int slots(int tile) { return tile <= 128 ? 512 : 256; }
 
 struct Counts {

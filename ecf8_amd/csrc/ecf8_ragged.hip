@@ -169,7 +169,8 @@ struct Operands {
 // kAhead: operands are read from LDS this many ahead of their products (and not all
 // at once, which would take registers that the other operands live in).  kFirst: the
 // wave goes before the SIMD's other one while it mixes products and softmax, and
-// after it in the scores, which are products alone (trees: 2 to 5% of the time).
+// after it in the scores, which are products alone (16 trees of 64 after 8192: 95 us,
+// 100 without).
 template <int T, bool kFine = false, int kAhead = 1, bool kFirst = false>
 struct Rows {
   v4f o[T][8];
@@ -701,7 +702,9 @@ __device__ __forceinline__ void lds_barrier() {
 // if page loads go through the caches, which a page, read once, gains nothing from;
 // 173 and 78 with T = 2 where the step's rows allow 1.
 //
-// kTree: the step's trees (rows read the cached positions and their masks').
+// kTree: the step's trees (rows read the cached positions and their masks'), up to 32
+// rows.  64 chains of 5 in groups of four after up to 8192 keys, 1.1 GB: 178 us, 6.1
+// TB/s.  T = 1 up to 16 rows: one tree of 4 after 4096 11 us, 12 with T = 2.
 template <Source kSrc, int T, bool kTree = false>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
@@ -1265,17 +1268,27 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 
 // ------------------------------------------------------------ drafted trees
 
-// Workgroup of four waves, two a CU: 64 T rows (token, head of the group) of one KV
-// head, 16 T a wave, against positions [k0, k1), 32 a step.  As in tile_kernel a
-// wave's softmax of a step runs beside the second product of the step before
-// (two waves of a SIMD that each do one after the other fall into step, and
-// neither hides the other: 2100 cycles a step of both instead of 1220, T = 2).
-// Keys and values go through registers, kDepth steps ahead, to a ring of LDS
-// stages.
+// Workgroup: 16 T rows (token, head of the group) a wave of one KV head, against
+// positions [k0, k1), 32 a step: 64 and 128 rows in four waves, two workgroups a CU,
+// or 256 in eight, one a CU.  As in tile_kernel a wave's softmax of a step runs
+// beside the second product of the step before.  Keys and values go through
+// registers, two steps ahead, to a ring of LDS stages.
+//
+// Bound by what of the softmax does not hide behind the products: both together take
+// 0.8 to 1.0 of their sum, whatever their order, and a step's 32 keys cost 16 T rows
+// 24 T products and some 100 T vector instructions.  Trees of 64 (256 rows), 8 after
+// 32768 e4m3 keys: 175 us with the join, 870 TFLOP/s of the 1240 that a large library
+// product reaches here; 64 rows wait for memory too: 24 trees of up to 26 after up to
+// 6000 bf16 keys, 55 us, 3.9 TB/s.
+// kOnce, pages past the caches, where a sequence's pages are read by one workgroup:
+// those take 55 us, 63 through the caches; of two tiles (16 trees of 64 with 8
+// heads a group, after 8192) 92 us, and 95 past the caches.
+// Not faster: 128 rows in eight waves, 192 in four (registers spill), half of the
+// waves for the staging alone (bf16 5% faster where contexts are long, e4m3 and short
+// ones 10% slower), loads three steps ahead.
 template <Source kSrc, int kWaves, int T, bool kFine, bool kOnce>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
-  // (three steps for e4m3, half the bytes: 64-node trees after 32768 192 -> 187 us)
-  constexpr int kDepth = kWaves == 8 && kSrc == kPagesFp8 ? 3 : 2;
+  constexpr int kDepth = 2;
   constexpr int kRows = 16 * T * kWaves, kThreads = 64 * kWaves;
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;               // 16-byte units of a row in memory
@@ -1519,7 +1532,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
 
 // Joins the parts of split rows: workgroup of `per` rows of a tile and KV head, four
 // dims a lane, eight parts' loads at a time.  Half a wave a row, or, for many parts
-// of few rows, a row at a time, its parts dealt to the eight half waves.
+// of few rows, a row at a time, its parts dealt to the eight half waves.  Latency of
+// three loads in a row: 3 us of one tree, 6 to 11 of many.
 __global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o, int part_rows, int per) {
   __shared__ float s_top[8], s_l[8];
   __shared__ v4f s_sum[8][32];
@@ -1748,7 +1762,8 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
   Joins j{};
   j.n = &counts->joins, j.list = reinterpret_cast<const Join *>(base + w.joins_at);
   j.stats = a.stats, j.sums = a.sums;
-  // rows a workgroup: eight, fewer while there are not a thousand workgroups
+  // rows a workgroup: eight, fewer while there are not a thousand workgroups (one tree
+  // of 8 after 4096: 12.6 us, 14.3 with eight; 16 of 32 after 8192: 75, 91 with one)
   const int most_rows = trees->max_nodes * a.group < w.tile ? trees->max_nodes * a.group : w.tile;
   const int64_t splits = (tiles < cuts ? tiles : cuts) * a.Hkv;
   int per = 8;
@@ -1778,7 +1793,7 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
     case 128:
       ECF8_TREE(4, 2, false, true);
       break;
-    default:  // (tiles of a sequence share its pages in L2)
+    default:  // (see kOnce)
       if (trees->max_nodes * a.group <= 256) ECF8_TREE(8, 2, false, true);
       else ECF8_TREE(8, 2, false, false);
   }

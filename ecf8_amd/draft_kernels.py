@@ -16,7 +16,8 @@ A step in which every sequence runs its last token and a tree of drafted ones is
 and emits ``trees.emitted[s, :kept[s]]`` of each sequence, whose last token is row
 0 of its next tree.  All calls launch on torch's current stream and read lengths,
 trees and results on the device, so a step can be captured as a HIP graph.  Trees
-hold one step at a time, like their batch."""
+hold one step at a time, like their batch, and one work buffer: calls with the same
+trees have to be ordered, on one stream or by events."""
 
 from __future__ import annotations
 
@@ -195,7 +196,8 @@ class KeepPlan:
 def draft_keep(plan: KeepPlan):
     """Move the keys and values of the accepted rows together: in all pools the row
     at position cached[s] + path[s, i] goes to cached[s] + i, i < kept[s].  The next
-    step has ``kept`` more tokens in the cache."""
+    step has ``kept`` more tokens in the cache.  Once a step and list of pools: a
+    second call would move what is in its place."""
     trees, batch = plan.trees, plan.trees.batch
     _launch("ecf8_draft_keep", batch.device, batch._ref, trees._ref, plan._ref, len(plan.pools),
             plan.fp8)

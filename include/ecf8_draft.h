@@ -8,7 +8,8 @@
  * transformers' generate, one token a step (scripts/inference_llm.py:108-142).
  *
  * Conventions as in ecf8.h: device pointers, stream as void*, ECF8_* status,
- * asynchronous, no allocation.  Deterministic.
+ * asynchronous, no allocation.  Deterministic.  Calls with the same trees share
+ * their work buffer and have to be ordered, on one stream or by events.
  *
  * In a step that ecf8_paged_plan planned, the new tokens of a sequence are a
  * tree: row 0 is its last accepted token (not in the cache yet), every other
@@ -77,8 +78,8 @@ int ecf8_draft_plan(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees
  * positions [0, cached[s]) and position cached[s] + j for every set bit j of its
  * mask (masks may be rewritten after the plan).  A row that reads nothing is
  * zeros.  Probabilities are rounded to bf16 in two parts, to 2^-15, where
- * max_nodes * Hq / Hkv is up to 64, else once.  Trees that were not planned for this step of the
- * batch set `refused`; nothing is written for them.
+ * max_nodes * Hq / Hkv is up to 64, else once.  Trees that were not planned for
+ * this step of the batch set `refused`; nothing is written for them.
  */
 int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t rows,
                          const ecf8_paged_batch *batch, const ecf8_draft_trees *trees,
@@ -128,9 +129,10 @@ int ecf8_draft_verify(const ecf8_paged_batch *batch, const ecf8_draft_trees *tre
  * Moves what was accepted together: in each of n_pools pools (an array of device
  * pointers in host memory, read by this call; [pages, Hkv, page_size, 128], bf16
  * or, fp8 != 0, e4m3fn), the row at position cached[s] + path[s][i] goes to
- * cached[s] + i for i < kept[s], as if all were read before any is written.  cached: the batch's lengths less
- * the step's rows.  A path that is not ascending from 0 within the sequence's rows
- * sets `refused` and is cut there.
+ * cached[s] + i for i < kept[s], as if all were read before any is written.
+ * cached: the batch's lengths less the step's rows.  A path that is not ascending
+ * from 0 within the sequence's rows sets `refused` and is cut there.  Once a step:
+ * a second call would move what is in its place.
  */
 int ecf8_draft_keep(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees,
                     void *const *pools, int n_pools, int fp8, void *stream);
