@@ -7,6 +7,8 @@
   checks;
 * ``paged_kernels``: sequences of different lengths over a paged KV cache
   (``include/ecf8_paged.h``);
+* ``draft_kernels``: trees of drafted tokens over that cache, and their
+  verification (``include/ecf8_draft.h``);
 * ``llm``, ``moe``, ``dit``, ``prefetch``: the Qwen3-8B-, Qwen3-30B-A3B- and
   FLUX-shaped engines that consume the decoded weights.
 

@@ -1276,10 +1276,10 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 //
 // Bound by what of the softmax does not hide behind the products: both together take
 // 0.8 to 1.0 of their sum, whatever their order, and a step's 32 keys cost 16 T rows
-// 24 T products and some 100 T vector instructions.  Trees of 64 (256 rows), 8 after
-// 32768 e4m3 keys: 175 us with the join, 870 TFLOP/s of the 1240 that a large library
-// product reaches here; 64 rows wait for memory too: 24 trees of up to 26 after up to
-// 6000 bf16 keys, 55 us, 3.9 TB/s.
+// 17 T products (kFine 25 T) and some 45 T vector instructions.  Eight trees of 64 with
+// 8 heads a group (two tiles of 256) after 32768 e4m3 keys: 175 us with the join, 870
+// TFLOP/s of the 1240 that a large library product reaches beside it.  Smaller trees
+// wait for memory too: 24 of up to 26 after up to 6000 bf16 keys 55 us, 3.9 TB/s.
 // kOnce, pages past the caches, where a sequence's pages are read by one workgroup:
 // those take 55 us, 63 through the caches; of two tiles (16 trees of 64 with 8
 // heads a group, after 8192) 92 us, and 95 past the caches.
