@@ -30,10 +30,19 @@ inline int tile_rows(int max_nodes, int group) {
   const int r = max_nodes * group;
   return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256;
 }
-// Workgroups that a split aims at, over all KV heads: two a CU, one of 256 rows.  64
+// Does a workgroup of 64 or 128 rows have a second group of waves, for half of its keys?
+// Where every sequence and head can have a CU of its own: half as many pieces to join.
+// Eight trees of 26 after 8192: 35 us, 40 without; 32 of 32 after 512 29 and 34; 64
+// (two rounds of CUs) of 32 after 512 49 and 39; short e4m3 ones up to 2 us more.
+inline bool in_halves(int tile, int64_t seqs, int Hkv) {
+  return (tile == 64 || tile == 128) && seqs * Hkv <= 256;
+}
+// Workgroups that a split aims at, over all KV heads: two a CU, one of eight waves.  64
 // chains of 5 after up to 8192: 177 us, 205 with 256; 16 trees of 64 after 8192: 95,
 // 109 with 512.
-inline int slots(int tile) { return tile <= 128 ? 512 : 256; }
+inline int slots(int tile, int64_t seqs, int Hkv) {
+  return tile > 128 || in_halves(tile, seqs, Hkv) ? 256 : 512;
+}
 
 struct Counts {
   int items, joins;
@@ -54,7 +63,7 @@ inline Work work_layout(int64_t seqs, int64_t rows, int Hq, int Hkv, int max_nod
   Work w;
   const int G = Hq / Hkv;
   w.tile = tile_rows(max_nodes, G);
-  w.target = slots(w.tile) / Hkv > 1 ? slots(w.tile) / Hkv : 1;
+  w.target = slots(w.tile, seqs, Hkv) / Hkv > 1 ? slots(w.tile, seqs, Hkv) / Hkv : 1;
   w.parts = 2 * w.target;
   w.packed = rows <= seqs * max_nodes;
   w.nodes = w.packed ? rows : seqs * max_nodes;

@@ -1272,24 +1272,26 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 // positions [k0, k1), 32 a step: 64 and 128 rows in four waves, two workgroups a CU,
 // or 256 in eight, one a CU.  As in tile_kernel a wave's softmax of a step runs
 // beside the second product of the step before.  Keys and values go through
-// registers, two steps ahead, to a ring of LDS stages.
+// registers, two steps ahead, to a ring of LDS stages.  kGroups = 2: eight waves, two
+// groups with a ring each, which take half of the keys and join over LDS.
 //
 // Bound by what of the softmax does not hide behind the products: both together take
 // 0.8 to 1.0 of their sum, whatever their order, and a step's 32 keys cost 16 T rows
 // 17 T products (kFine 25 T) and some 45 T vector instructions.  Eight trees of 64 with
 // 8 heads a group (two tiles of 256) after 32768 e4m3 keys: 175 us with the join, 870
 // TFLOP/s of the 1240 that a large library product reaches beside it.  Smaller trees
-// wait for memory too: 24 of up to 26 after up to 6000 bf16 keys 55 us, 3.9 TB/s.
+// wait for memory too: 24 of up to 26 after up to 6000 bf16 keys 52 to 56 us by card,
+// 4 TB/s.
 // kOnce, pages past the caches, where a sequence's pages are read by one workgroup:
-// those take 55 us, 63 through the caches; of two tiles (16 trees of 64 with 8
+// those took 55 us, 63 through the caches; of two tiles (16 trees of 64 with 8
 // heads a group, after 8192) 92 us, and 95 past the caches.
 // Not faster: 128 rows in eight waves, 192 in four (registers spill), half of the
 // waves for the staging alone (bf16 5% faster where contexts are long, e4m3 and short
 // ones 10% slower), loads three steps ahead.
-template <Source kSrc, int kWaves, int T, bool kFine, bool kOnce>
-__global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
+template <Source kSrc, int kGroups, int kWaves, int T, bool kFine, bool kOnce>
+__global__ __launch_bounds__(64 * kGroups * kWaves, 2) void tree_kernel(Attn a) {
   constexpr int kDepth = 2;
-  constexpr int kRows = 16 * T * kWaves, kThreads = 64 * kWaves;
+  constexpr int kRows = 16 * T * kWaves, kThreads = 64 * kWaves;  // of a group
   constexpr bool kFp8 = kSrc == kPagesFp8;
   constexpr int kUnits = kFp8 ? 8 : 16;               // 16-byte units of a row in memory
   // rows a pass of the threads; twice a step's: keys and values have half of them each
@@ -1298,25 +1300,43 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
   constexpr int kLoads = kHalves ? 1 : 32 / kPass;
   // after the barrier before step j the waves read steps j - 1 to j + 1 and write j + 2
   constexpr int kRing = 4;
-  __shared__ u32x4 s_kv[kRing][32 * (kKeyRow + kValueRow)];
-  __shared__ int s_odd;
+  // steps that two groups share: one tree of 32 after 4096 (pieces of 13 steps) 19.6 us,
+  // 21 from eight on; 32 of 8, 8 heads a group, after up to 512 19.2 and 18.0
+  constexpr int kBoth = 16;
+  __shared__ u32x4 s_rings[kGroups][kRing][32 * (kKeyRow + kValueRow)];
+  __shared__ int s_odds[kGroups];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = kGroups > 1 ? (int)threadIdx.x % kThreads : (int)threadIdx.x;
+  const int group = kGroups > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = (int)blockIdx.x % a.Hkv;
   const Operands ops(lane);
+  auto &s_kv = s_rings[group];
+  int &s_odd = s_odds[group];
 
   TreePlace p;
   if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
   const int all_rows = min(p.n * a.group - p.row0, kRows);
-  const int first_row = 16 * T * wave, n_rows = min(all_rows - first_row, 16 * T);
+  const int first_row = 16 * T * wave;
+  const int n_rows = min(all_rows - first_row, 16 * T);
+  int most = (p.k1 - p.k0 + 31) / 32;  // steps of a group
+  const bool both = kGroups > 1 && most >= kBoth;
+  if (both) {
+    most = (most + 1) / 2;
+    const int middle = p.k0 + 32 * most;
+    if (group) p.k0 = middle;
+    else p.k1 = middle;
+  } else if (group) {
+    return;  // (barriers wait for the waves that are left)
+  }
   float c = a.scale, vscale = 1.f;
   if constexpr (kFp8) c *= a.ks[kvh], vscale = a.vs[kvh];
 
   // load i of a step: row kPass i + sub of its keys and values.  kTail: past the
   // end the last row again.
-  const int unit = (int)threadIdx.x % kUnits;
-  const int sub = (int)threadIdx.x / kUnits % (kHalves ? 32 : kPass);
-  const bool key_half = !kHalves || (int)threadIdx.x < kThreads / 2;
+  const int unit = tid % kUnits;
+  const int sub = tid / kUnits % (kHalves ? 32 : kPass);
+  const bool key_half = !kHalves || tid < kThreads / 2;
   const int *table = a.table + (size_t)p.seq * a.width;
   const int steps = (p.k1 - p.k0 + 31) / 32;
   auto key_of = [&](auto tail, int j, int i) {
@@ -1398,7 +1418,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
   v8bf q[T][4];
   const int row0 = p.row0 + min(first_row, all_rows - 1), row_end = p.row0 + all_rows;
   load_queries<T>(a, kvh, p.start, row0, row_end, lane, q);
-  if (threadIdx.x == 0) s_odd = 0;
+  if (tid == 0) s_odd = 0;
   size_t at[kLoads];
 #pragma unroll
   for (int x = 0; x < 2; ++x) place(kTail, x, lead[x], at), load(at, lead[x]);
@@ -1428,7 +1448,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
     }
   };
   // all waves pass as many barriers: one for step 0, kDepth a turn
-  const int turns = (steps - 1 + kDepth - 1) / kDepth;
+  const int turns = (most - 1 + kDepth - 1) / kDepth;
   if (n_rows <= 0) {  // uniform: a wave without rows stages its share
     barrier();
 #pragma unroll
@@ -1441,6 +1461,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) between(kTail, turn * kDepth + x, i, r[x % kDepth]);
       }
+    if (both && !p.stale) barrier(), barrier();  // (the groups' join)
     return;
   }
   Rows<T, kFine, 2, true> w;
@@ -1504,6 +1525,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
           [&](int t, int key) { return (tree_word(bits[t], key, p.cached, p.k1) & 1) != 0; });
   }
 #pragma unroll
+  for (int t = 0; t < T; ++t)
+    if (w.l[t][0] == 0.f) w.m[t] = kLowest;
+  if (both) {  // the second group's sums over LDS (its ring) to the first
+    v4f *sums = reinterpret_cast<v4f *>(s_rings[kGroups - 1]) + wave * (T * 8 * 64) + lane;
+    float2 *stats = reinterpret_cast<float2 *>(reinterpret_cast<v4f *>(s_rings[kGroups - 1]) +
+                                               kWaves * T * 8 * 64) + wave * (T * 64) + lane;
+    barrier();
+    if (group) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        stats[64 * t] = make_float2(w.m[t], w.l[t][0]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) sums[64 * (8 * t + d)] = w.o[t][d];
+      }
+    }
+    barrier();
+    if (group) return;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float2 st = stats[64 * t];
+      const float top = fmaxf(w.m[t], st.x);
+      const float f0 = __builtin_amdgcn_exp2f(w.m[t] - top);
+      const float f1 = __builtin_amdgcn_exp2f(st.x - top);
+      w.m[t] = top;
+      w.l[t][0] = fmaf(f1, st.y, w.l[t][0] * f0);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const v4f v = sums[64 * (8 * t + d)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.o[t][d][i] = fmaf(f1, v[i], w.o[t][d][i] * f0);
+      }
+    }
+  }
+#pragma unroll
   for (int t = 0; t < T; ++t) {
     const float l = w.l[t][0];
     const int row = first_row + 16 * t + (lane & 15), g = lane >> 4;
@@ -1513,7 +1568,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(Attn a) {
       v4f *sums = reinterpret_cast<v4f *>(a.sums) + at * 32 + g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) sums[4 * d] = w.o[t][d];
-      if (g == 0) a.stats[at] = make_float2(l == 0.f ? kLowest : w.m[t], l);
+      if (g == 0) a.stats[at] = make_float2(w.m[t], l);
     } else {
       const int at = p.row0 + row, tk = p.start + at / a.group;
       const float inv = l == 0.f ? 0.f : vscale / l;  // (a mask can be empty)
@@ -1775,11 +1830,13 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
     if (fp8) few_kernel<kPagesFp8, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);      \
     else few_kernel<kPages, T, true><<<grid, 256, 0, as_stream(stream)>>>(a);             \
   } while (0)
-#define ECF8_TREE(W, T, F, O)                                                                   \
+#define ECF8_TREE(G, W, T, F, O)                                                                \
   do {                                                                                          \
-    if (fp8) tree_kernel<kPagesFp8, W, T, F, O><<<grid, 64 * W, 0, as_stream(stream)>>>(a);     \
-    else tree_kernel<kPages, W, T, F, O><<<grid, 64 * W, 0, as_stream(stream)>>>(a);            \
+    constexpr unsigned threads = 64 * G * W;                                                    \
+    if (fp8) tree_kernel<kPagesFp8, G, W, T, F, O><<<grid, threads, 0, as_stream(stream)>>>(a); \
+    else tree_kernel<kPages, G, W, T, F, O><<<grid, threads, 0, as_stream(stream)>>>(a);        \
   } while (0)
+  const bool halves = ecf8::draft::in_halves(w.tile, b->seqs, b->Hkv);
   switch (w.tile) {
     case 16:
       ECF8_TREE_FEW(1);
@@ -1787,15 +1844,17 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
     case 32:
       ECF8_TREE_FEW(2);
       break;
-    case 64:
-      ECF8_TREE(4, 1, true, true);
+    case 64:  // (two parts cost nothing in bf16, a tenth in e4m3)
+      if (halves) ECF8_TREE(2, 4, 1, true, true);
+      else ECF8_TREE(1, 4, 1, true, true);
       break;
-    case 128:
-      ECF8_TREE(4, 2, false, true);
+    case 128:  // (one: in two 10 to 17% more)
+      if (halves) ECF8_TREE(2, 4, 2, false, true);
+      else ECF8_TREE(1, 4, 2, false, true);
       break;
     default:  // (see kOnce)
-      if (trees->max_nodes * a.group <= 256) ECF8_TREE(8, 2, false, true);
-      else ECF8_TREE(8, 2, false, false);
+      if (trees->max_nodes * a.group <= 256) ECF8_TREE(1, 8, 2, false, true);
+      else ECF8_TREE(1, 8, 2, false, false);
   }
 #undef ECF8_TREE_FEW
 #undef ECF8_TREE

@@ -361,6 +361,92 @@ def test_scores_of_any_size(cuda_device):
         assert bool((out[6:].double() == v[c + 6]).all())
 
 
+# One workgroup a sequence and head where all of them can have a CU of their own, its
+# keys in two halves; two a CU, of half the waves, in larger batches (idle sequences
+# here).  32 KV heads: pieces of many steps.
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("idle", [0, 9])
+@pytest.mark.parametrize("nodes", [10, 16, 29, 32])
+def test_attention_of_long_pieces(cuda_device, nodes, idle, fp8):
+    """Lengths at the border of one and two halves, and far from it; callers' masks."""
+    from ecf8_amd.draft_kernels import draft_attention
+
+    dev, rng, Hq, Hkv = cuda_device, random.Random(nodes + idle), 128, 32
+    gen = torch.Generator(device=dev).manual_seed(nodes)
+    lengths = [480, 4100, 481, 513, 1030, 512] + [0] * idle
+    cached = [max(0, L - nodes) for L in lengths]
+    trees = [M.random_tree(rng, nodes if L else 0, 3) for L in lengths]
+    b, t, _ = _step(dev, cached, trees, 16, Hq, Hkv, max_nodes=nodes)
+    pools, scales, dense = _filled(b, lengths, fp8, gen)
+    bits = [[rng.choice([m, 0, rng.getrandbits(64)]) for m in M.masks(tree)] for tree in trees]
+    t.masks.copy_(_ints([M.signed(m) for x in bits for m in x], dev, torch.int64))
+    q = _rand(6 * nodes, Hq, D, gen=gen, scale=1.5)
+    out = torch.empty(6 * nodes, Hq * D, dtype=torch.bfloat16, device=dev)
+    draft_attention(q, *pools, t, out, *scales)
+    assert not _refused(b)
+    for i, (c, (k, v)) in enumerate(zip(cached[:6], dense)):
+        at = slice(i * nodes, (i + 1) * nodes)
+        want, A = M.attention(q[at].double(), k, v, _seen(bits[i], c, nodes, dev))
+        _check(out[at].view(nodes, Hq, D), want, A, nodes * (Hq // Hkv) <= 64)
+
+
+@pytest.mark.parametrize("idle", [0, 9])
+@pytest.mark.parametrize("nodes", [12, 30])
+def test_infinities_in_long_pieces(cuda_device, nodes, idle):
+    """Infinities and NaN of both halves and of the tree; scores of -inf in either half,
+    and thousands apart."""
+    from ecf8_amd.draft_kernels import draft_attention
+
+    dev, rng, Hq, Hkv, S, c = cuda_device, random.Random(nodes), 128, 32, 4, 2500
+    gen = torch.Generator(device=dev).manual_seed(nodes)
+    cached, L = [c] * S + [0] * idle, c + nodes
+    tree = M.random_tree(rng, nodes, 3)
+    b, t, _ = _step(dev, cached, [tree] * S + [[]] * idle, 16, Hq, Hkv, max_nodes=nodes)
+    pools, _, dense = _filled(b, [L] * S + [0] * idle, False, gen)
+    q = _rand(S * nodes, Hq, D, gen=gen)
+    out = torch.empty(S * nodes, Hq, D, dtype=torch.bfloat16, device=dev)
+    draft_attention(q, *pools, t, out)
+    clean = out.clone()
+    seen = _seen(M.masks(tree), c, nodes, dev)
+    marks = [(3, 5, math.inf), (1100, 9, -math.inf), (2400, 11, math.nan), (1300, 13, math.inf),
+             (7, 13, -math.inf), (c + 2, 20, math.inf), (c + nodes - 1, 21, math.nan)]
+    want = clean.clone()
+    saved = pools[1].clone()
+    for pos, d, x in marks:
+        pools[1][b.table[:S, pos // 16].long(), :, pos % 16, d] = x
+        reads = seen[:, pos].repeat(S)
+        old = want[reads, :, d]
+        want[reads, :, d] = torch.where(old.isfinite(), torch.zeros_like(old), old) + x
+    draft_attention(q, *pools, t, out)
+    assert not _refused(b)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[~want.isnan()], want[~want.isnan()])
+    pools[1].copy_(saved)
+    pos = torch.arange(L, device=dev)
+    q.fill_(1.0)
+    for only in (40, 2450):  # in the first and in the last half
+        for s in range(S):
+            where = b.table[s, pos // 16].long(), slice(None), pos % 16
+            k = torch.where(pos[:, None, None] == only, 1.0, -math.inf).bfloat16()
+            pools[0][where] = k.expand(L, Hkv, D)
+        draft_attention(q, *pools, t, out)
+        torch.cuda.synchronize()
+        for s in range(S):
+            v = dense[s][1][only].repeat_interleave(Hq // Hkv, 0)
+            assert bool((out[s * nodes: (s + 1) * nodes].double() == v).all()), (only, s)
+    for slope in (1, -1):
+        key = torch.linspace(-20_000 * slope, 100 * slope, L, device=dev)
+        k = torch.zeros(L, Hkv, D, device=dev)
+        k[:, :, 0] = key[:, None]
+        for s in range(S):
+            pools[0][b.table[s, pos // 16].long(), :, pos % 16] = k.bfloat16()
+        draft_attention(q, *pools, t, out)
+        for s in range(S):
+            at = slice(s * nodes, (s + 1) * nodes)
+            x, A = M.attention(q[at].double(), k.bfloat16().double(), dense[s][1], seen)
+            _check(out[at], x, A, nodes * (Hq // Hkv) <= 64)
+
+
 def test_a_plan_of_another_step_is_refused(cuda_device):
     """Trees never planned, planned for the step before, or for other sizes."""
     from ecf8_amd.draft_kernels import DraftTrees, draft_attention, draft_plan
