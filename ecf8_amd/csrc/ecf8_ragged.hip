@@ -1848,11 +1848,14 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
       if (halves) ECF8_TREE(2, 4, 1, true, true);
       else ECF8_TREE(1, 4, 1, true, true);
       break;
-    case 128:  // (one: in two 10 to 17% more)
-      if (halves) ECF8_TREE(2, 4, 2, false, true);
-      else ECF8_TREE(1, 4, 2, false, true);
+    case 128:  // (16 trees of 26 after 8192: 78 us, 65 in one)
+      if (halves) ECF8_TREE(2, 4, 2, true, true);
+      else ECF8_TREE(1, 4, 2, true, true);
       break;
-    default:  // (see kOnce)
+    // (see kOnce.  Rounded to bf16 once, as in tile_kernel, since the products bound these:
+    // eight trees of 64 with 8 heads a group after 32768 e4m3 keys 179 us, 228 in two
+    // parts; 16 of 64 after 8192 bf16 ones 95 and 121)
+    default:
       if (trees->max_nodes * a.group <= 256) ECF8_TREE(1, 8, 2, false, true);
       else ECF8_TREE(1, 8, 2, false, false);
   }

@@ -92,7 +92,7 @@ def draft_attention(q, k_pool, v_pool, trees: DraftTrees, out, k_scale=None, v_s
     positions and those of the rows in its mask (``trees.masks``, which a caller
     may rewrite after the plan).  A row that reads nothing is zeros; rows past the
     last sequence of ``out`` are left as they were.  Probabilities are kept to
-    2^-15 where max_nodes * Hq / Hkv is up to 64, and rounded to bf16 once above.
+    2^-15 where max_nodes * Hq / Hkv is up to 128, and rounded to bf16 once above.
     Returns ``out``."""
     batch = trees.batch
     dev, rows = batch.device, q.shape[0]

@@ -78,7 +78,7 @@ int ecf8_draft_plan(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees
  * positions [0, cached[s]) and position cached[s] + j for every set bit j of its
  * mask (masks may be rewritten after the plan).  A row that reads nothing is
  * zeros.  Probabilities are rounded to bf16 in two parts, to 2^-15, where
- * max_nodes * Hq / Hkv is up to 64, else once.  Trees that were not planned for
+ * max_nodes * Hq / Hkv is up to 128, else once.  Trees that were not planned for
  * this step of the batch set `refused`; nothing is written for them.
  */
 int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t rows,
