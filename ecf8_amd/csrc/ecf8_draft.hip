@@ -37,6 +37,7 @@ struct Plan {
   Join *joins;
   int seqs, rows, all_rows, group, max_nodes, max_children, tile, target;
   uint64_t stamp;
+  const uint64_t *step;  // the batch's
 };
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
@@ -126,6 +127,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
   __shared__ int s_waves[2][2][kPlanWaves];
   __shared__ int s_bucket[kBuckets];
   const int tid = threadIdx.x, S = a.seqs;
+  const uint64_t planned = *a.step;
   const int step = (S + kPlanThreads - 1) / kPlanThreads;
   if (tid < kBuckets) s_bucket[tid] = 0;
   int tiles[kPer], sum = 0, units = 0;
@@ -211,8 +213,8 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
         }
       }
       if (write && mine.k > 1)
-        a.joins[mine.join] = Join{mine.it.row0, mine.part, mine.k, mine.it.start, mine.it.n,
-                                  {mine.it.seq, mine.it.cached, 0}};
+        a.joins[mine.join] =
+            Join{mine.it.row0, mine.part, mine.k, mine.it.start, mine.it.n, {0, 0, 0}};
     }
     __syncthreads();
     if (!write) {
@@ -224,7 +226,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
       __syncthreads();
     }
   }
-  if (tid == 0) *a.counts = Counts{n_items, n_joins, a.stamp};
+  if (tid == 0) *a.counts = Counts{n_items, n_joins, a.stamp, planned};
 }
 
 // The first workgroup schedules, the others take 16 sequences' trees each.  Latency of
@@ -1021,7 +1023,7 @@ extern "C" int ecf8_draft_plan(const ecf8_paged_batch *b, const ecf8_draft_trees
                reinterpret_cast<Counts *>(base), reinterpret_cast<Item *>(base + w.items_at),
                reinterpret_cast<Join *>(base + w.joins_at), b->seqs, (int)rows, b->rows,
                b->Hq / b->Hkv, t->max_nodes, t->max_children, w.tile, w.target,
-               schedule_stamp(b, t)};
+               schedule_stamp(b, t), step_of(b)};
   const unsigned grid = 1 + (unsigned)((b->seqs + kPlanWaves - 1) / kPlanWaves);
   plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
   return launched();

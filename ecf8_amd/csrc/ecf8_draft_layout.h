@@ -44,9 +44,11 @@ inline int slots(int tile, int64_t seqs, int Hkv) {
   return tile > 128 || in_halves(tile, seqs, Hkv) ? 256 : 512;
 }
 
+// At the start of the work buffer.  stamp: as in the batch's; step: the batch's that
+// the trees were planned for.
 struct Counts {
   int items, joins;
-  uint64_t stamp;
+  uint64_t stamp, step;
 };
 
 // Byte offsets of the work buffer's parts.
@@ -100,6 +102,11 @@ inline bool sizes_ok(int64_t seqs, int64_t rows, int Hq, int Hkv, int max_nodes,
                      int max_children) {
   return paged::sizes_ok(seqs, rows, Hq, Hkv) && max_nodes >= 1 && max_nodes <= kMaxNodes &&
          max_children >= 1 && max_children <= kMaxNodes;
+}
+
+// How many steps of a batch were planned.
+inline const uint64_t *step_of(const ecf8_paged_batch *b) {
+  return &static_cast<const paged::Counts *>(b->work)->step;
 }
 
 // A batch's and its trees' sizes and pointers.

@@ -146,6 +146,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   if (tid < 2 * kBuckets) s_bucket[tid / kBuckets][tid % kBuckets] = 0;
   __syncthreads();
   const int n_free = a.n_free[0];
+  uint64_t planned = 0;  // (here: its load waits for nothing)
+  if (tid == 0) planned = a.counts->step + 1;
   int c[kPer], n[kPer], own[kPer], take[kPer], back[kPer];
   bool bad = n_free < 0 || n_free > a.pages;
 #pragma unroll
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
     }
     __syncthreads();
     if (tid == 0) {
-      *a.counts = Counts{0, 0, 0, 0, a.stamp};
+      *a.counts = Counts{0, 0, 0, 0, a.stamp, planned};
       if (a.refused) *a.refused = 1;
     }
     if (a.fill_rows)
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
       if (!write) t_items = start_buckets(s_bucket[1], s_waves[0]);
     }
   }
-  if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins, a.stamp};
+  if (tid == 0) *a.counts = Counts{n_items, t_items, n_joins, t_joins, a.stamp, planned};
   if (a.fill_rows) {
     __threadfence_block();
     __syncthreads();

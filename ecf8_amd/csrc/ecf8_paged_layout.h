@@ -44,9 +44,11 @@ struct Join {
 // At the start of the work buffer.  stamp: of the sizes that the plan wrote the
 // lists for (schedule_stamp), zero before the first plan.  The attention reads no
 // item under another: a list of anything else would send it out of its buffers.
+// step: how many steps were planned, so that what is planned beside a step
+// (ecf8_draft_layout.h) can tell whether it is this one.
 struct Counts {
   int few, tiles, few_joins, tile_joins;
-  uint64_t stamp;
+  uint64_t stamp, step;
 };
 
 // Byte offsets of the work buffer's parts.

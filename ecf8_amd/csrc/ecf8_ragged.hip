@@ -127,7 +127,7 @@ struct Attn {
   int max_new;                             // new tokens of a sequence
   float scale;                             // of the scores, times log2(e)
   const uint64_t *masks;                   // trees: of the packed rows
-  const int *lengths;
+  const uint64_t *planned, *step;          // their step, and the batch's
 };
 
 enum Source { kPages, kPagesFp8, kPacked };
@@ -609,36 +609,22 @@ __device__ __forceinline__ bool get_item(const Attn &a, int tile_rows, int item,
   }
 }
 
-// The item of slot `item` of a step's trees; false past the last.  A plan of these
-// sizes may be of another step (stale): its items lead to no place out of range,
-// so what was loaded for the check is looked at only where outputs are written.
-struct TreePlace : Place {
-  bool stale, report;
-};
-__device__ __forceinline__ bool get_tree_item(const Attn &a, int item, TreePlace &p) {
+// The item of slot `item` of a step's trees; false past the last, and of trees that
+// were planned for another step or sizes.
+__device__ __forceinline__ bool get_tree_item(const Attn &a, int item, Place &p) {
   const Item it = a.items[item];  // item < a.grid: in the list, filled or not
-  const uint64_t stamp = *a.stamp;
+  const uint64_t stamp = *a.stamp, planned = *a.planned, step = *a.step;
   const int n_items = *a.n_items, step_rows = a.starts[a.seqs];
   // (all before the first wait)
-  asm volatile("" ::"s"(it.seq), "s"(it.start), "s"(n_items), "s"((int)stamp), "s"(step_rows));
-  p.report = blockIdx.x == gridDim.x - 1 && (step_rows > a.rows || stamp != a.want_stamp);
-  if (stamp != a.want_stamp || item >= n_items) {
-    if (p.report && threadIdx.x == 0 && a.refused) *a.refused = 1;
-    return false;
-  }
+  asm volatile("" ::"s"(it.seq), "s"(it.start), "s"(n_items), "s"(stamp), "s"(planned), "s"(step),
+               "s"(step_rows));
+  const bool ours = stamp == a.want_stamp && planned == step;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && a.refused && (!ours || step_rows > a.rows))
+    *a.refused = 1;
+  if (!ours || item >= n_items) return false;
   p.seq = it.seq, p.row0 = it.row0, p.k0 = it.k0, p.k1 = it.k1, p.part = it.part;
   p.start = it.start, p.n = it.n, p.cached = it.cached;
-  // (scalar loads: the wait for vector ones would be here)
-  typedef const __attribute__((address_space(4))) int constant_int;
-  auto *starts = (constant_int *)a.starts, *lengths = (constant_int *)a.lengths;
-  const int start = starts[it.seq], next = starts[it.seq + 1], length = lengths[it.seq];
-  p.stale = ((start ^ it.start) | (next ^ (it.start + it.n)) |
-             (length ^ (it.cached + it.n))) != 0;
   return true;
-}
-__device__ __forceinline__ bool may_write(const Attn &a, const TreePlace &p) {
-  if ((p.report || p.stale) && threadIdx.x == 0 && a.refused) *a.refused = 1;
-  return !p.stale;
 }
 
 // The masks of the lane's queries, as load_queries has them.
@@ -719,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   const int unit = lane % kUnits;
   const Operands ops(lane);
 
-  std::conditional_t<kTree, TreePlace, Place> p;
+  Place p;
   if constexpr (kTree) {
     if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
   } else {
@@ -847,9 +833,6 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
         }
   }
 
-  if constexpr (kTree) {
-    if (!may_write(a, p)) return;
-  }
   // join the waves
   float l[T];
 #pragma unroll
@@ -1314,7 +1297,7 @@ __global__ __launch_bounds__(64 * kGroups * kWaves, 2) void tree_kernel(Attn a) 
   auto &s_kv = s_rings[group];
   int &s_odd = s_odds[group];
 
-  TreePlace p;
+  Place p;
   if (!get_tree_item(a, (int)blockIdx.x / a.Hkv, p)) return;
   const int all_rows = min(p.n * a.group - p.row0, kRows);
   const int first_row = 16 * T * wave;
@@ -1461,7 +1444,7 @@ __global__ __launch_bounds__(64 * kGroups * kWaves, 2) void tree_kernel(Attn a) 
 #pragma unroll
         for (int i = 0; i < 8; ++i) between(kTail, turn * kDepth + x, i, r[x % kDepth]);
       }
-    if (both && !p.stale) barrier(), barrier();  // (the groups' join)
+    if (both) barrier(), barrier();  // (the groups' join)
     return;
   }
   Rows<T, kFine, 2, true> w;
@@ -1513,7 +1496,6 @@ __global__ __launch_bounds__(64 * kGroups * kWaves, 2) void tree_kernel(Attn a) 
       }
     }
   }
-  if (!may_write(a, p)) return;
   w.second(ops, values(steps - 1), pr);
   if (s_odd) {  // (written before the last barrier)
     uint64_t bits[T];
@@ -1596,16 +1578,12 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o, int par
   const int kvh = (int)blockIdx.x % a.Hkv, group = (int)blockIdx.x / a.Hkv;
   const int y = group % o.rows_groups, j = group / o.rows_groups;
   const Join jn = o.list[j];  // j: in the list, filled or not
-  const uint64_t stamp = *a.stamp;
+  const uint64_t stamp = *a.stamp, planned = *a.planned, step_now = *a.step;
   const int n_joins = *o.n;
-  asm volatile("" ::"s"(jn.row0), "s"(jn.start), "s"((int)stamp), "s"(n_joins));
-  if (stamp != a.want_stamp || j >= n_joins) return;
-  // (pad: the sequence and its cached tokens; as in get_tree_item)
-  typedef const __attribute__((address_space(4))) int constant_int;
-  auto *starts = (constant_int *)a.starts, *lengths = (constant_int *)a.lengths;
-  const int seq = jn.pad[0];
-  const bool stale = ((starts[seq] ^ jn.start) | (starts[seq + 1] ^ (jn.start + jn.tokens)) |
-                      (lengths[seq] ^ (jn.pad[1] + jn.tokens))) != 0;
+  asm volatile("" ::"s"(jn.row0), "s"(jn.start), "s"(stamp), "s"(planned), "s"(step_now),
+               "s"(n_joins));
+  // (as in get_tree_item)
+  if (stamp != a.want_stamp || planned != step_now || j >= n_joins) return;
   const int end = min(min(jn.tokens * a.group - jn.row0, part_rows), (y + 1) * per);
   const float vscale = a.vs ? a.vs[kvh] : 1.f;
   const size_t step = (size_t)a.Hkv * part_rows;
@@ -1644,7 +1622,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Attn a, Joins o, int par
   auto put = [&](int row) {
     const int g = jn.row0 + row, tk = jn.start + g / a.group;
     const float inv = l == 0.f ? 0.f : vscale / l;  // (a mask can be empty)
-    if (tk < a.rows && !stale)
+    if (tk < a.rows)
       *reinterpret_cast<u32x2 *>(a.out + (int64_t)tk * a.out_stride +
                                  (kvh * a.group + g % a.group) * kD + 4 * lane) =
           u32x2{pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv)};
@@ -1796,7 +1774,7 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
   a.q_stride = q_stride, a.out_stride = out_stride;
   a.ks = fp8 ? k_scale : nullptr, a.vs = fp8 ? v_scale : nullptr;
   a.starts = b->starts, a.table = b->table, a.refused = b->refused;
-  a.masks = trees->masks, a.lengths = b->lengths;
+  a.masks = trees->masks, a.planned = &counts->step, a.step = ecf8::draft::step_of(b);
   a.stamp = &counts->stamp, a.want_stamp = ecf8::draft::schedule_stamp(b, trees);
   a.Hkv = b->Hkv, a.group = b->Hq / b->Hkv, a.rows = (int)rows, a.seqs = b->seqs;
   a.width = b->width;

@@ -78,7 +78,8 @@ def draft_plan(trees: DraftTrees, parents):
     [rows], of each packed row the row of its sequence that it follows, -1 for
     row 0.  Fills ``masks`` and ``parents``, sets the batch's positions to cached +
     depth, and plans ``draft_attention``.  A tree that is none, has more than
-    ``max_nodes`` rows or ``max_children`` children sets the batch's ``refused``."""
+    ``max_nodes`` rows or ``max_children`` children sets the batch's ``refused``.
+    Once for every ``paged_plan``, also where that plans a step a second time."""
     batch = trees.batch
     _want(parents, torch.int32, "parents", batch.device)
     if parents.numel() > batch.max_rows or parents.numel() < 1:
@@ -91,7 +92,8 @@ def draft_attention(q, k_pool, v_pool, trees: DraftTrees, out, k_scale=None, v_s
     """paged_attention of a step's trees: row t of sequence s reads the cached
     positions and those of the rows in its mask (``trees.masks``, which a caller
     may rewrite after the plan).  A row that reads nothing is zeros; rows past the
-    last sequence of ``out`` are left as they were.  Probabilities are kept to
+    last sequence of ``out`` are left as they were, and all of them, with the batch's
+    ``refused`` set, where the trees were not planned for the batch's step.  Probabilities are kept to
     2^-15 where max_nodes * Hq / Hkv is up to 128, and rounded to bf16 once above.
     Returns ``out``."""
     batch = trees.batch

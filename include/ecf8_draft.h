@@ -68,7 +68,8 @@ int64_t ecf8_draft_work_bytes(int64_t seqs, int64_t rows, int Hq, int Hkv, int m
  * then on their own: row 0's position, no parents, masks of their own bit.  So
  * does one of more than max_nodes rows, or with rows past the `rows` that parents
  * holds, of which nothing is attended.  Entries past the step's last row are left
- * as they were.
+ * as they were.  Once for every step that ecf8_paged_plan plans, also for one that
+ * it plans a second time: it sets the positions to a chain's.
  */
 int ecf8_draft_plan(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees,
                     const int *parents, int64_t rows, void *stream);

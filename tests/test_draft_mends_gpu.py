@@ -36,3 +36,45 @@ def test_probabilities_of_up_to_128_rows_enter_in_two_parts(cuda_device, Hq, Hkv
         want, A = M.attention(q[at].double(), *dense[i],
                               _seen(M.masks(trees[i]), cached[i], nodes, dev))
         _check(out[at].view(nodes, Hq, D), want, A, True)
+
+
+# rows of a sequence and KV head: the kernels of 16, 32, 64, 128 and 256
+@pytest.mark.parametrize("Hq", [4, 8, 16, 32, 64])
+@pytest.mark.parametrize("cached", [20, 3000])
+def test_attention_over_a_plan_of_another_step_writes_nothing(cuda_device, cached, Hq):
+    """Where none of the sequences that the plan knew has changed: all were idle, or the
+    last one was; where one was too long for a tree; and where the step is planned again."""
+    from ecf8_amd.draft_kernels import DraftTrees, draft_attention, draft_plan
+    from ecf8_amd.paged_kernels import PagedBatch, paged_plan
+
+    dev, n = cuda_device, 4
+    b = PagedBatch(3, 3 * n, 1000, 16, 4000, Hq, 1, dev)
+    t = DraftTrees(b, n, 2)
+    pools = [torch.full((b.pages, 1, 16, D), 2.0, dtype=torch.bfloat16, device=dev)
+             for _ in range(2)]
+    parents = torch.tensor([-1, 0, 0, 1] * 3, dtype=torch.int32).to(dev)
+    q = torch.zeros(3 * n, Hq, D, dtype=torch.bfloat16, device=dev)
+    out = torch.empty(3 * n, Hq * D, dtype=torch.bfloat16, device=dev)
+
+    def plan(*new):
+        lengths = [[cached if k else 0 for k in new], new]
+        paged_plan(b, *(torch.tensor(x, dtype=torch.int32).to(dev) for x in lengths))
+
+    def attend():
+        out.fill_(3.0)
+        draft_attention(q, *pools, t, out)
+        return _refused(b)
+
+    for before, now in (((0, 0, 0), (n, n, n)), ((0, 0, 0), (0, 0, 1)), ((n, n, 0), (n, n, n)),
+                        ((n, 0, 0), (n, 0, 1)), ((n, 0, n), (n, 0, n)), ((n, 2 * n, 0), (n, n, n))):
+        plan(*before)
+        draft_plan(t, parents)
+        assert _refused(b) == (max(before) > n)
+        attend()
+        plan(*now)
+        assert attend() == 1, (before, now)
+        assert bool((out == 3.0).all()), (before, now)
+        draft_plan(t, parents)
+        assert attend() == 0
+        rows = sum(now)
+        assert bool((out[:rows] == 2.0).all()) and bool((out[rows:] == 3.0).all())
