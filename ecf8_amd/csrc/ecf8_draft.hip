@@ -455,6 +455,16 @@ __global__ __launch_bounds__(256) void probability_kernel(Probs a) {
 
 // --------------------------------------------------------- verification
 
+// What says whether trees were planned for the batch's step.
+struct Planned {
+  const Counts *counts;
+  const uint64_t *step;
+  uint64_t stamp;
+  __device__ __forceinline__ bool now() const {
+    return (int)(counts->stamp == stamp) & (int)(counts->step == *step);
+  }
+};
+
 // Where a sequence's walk ended, for the kernel that draws its next token.
 struct Ended {
   int64_t row;                // packed row whose w is drawn from, -1: none
@@ -476,6 +486,7 @@ struct Verify {
   int64_t nodes;
   int seqs, rows, V, max_nodes, max_children, packed;
   int per, lanes;  // runs a workgroup, threads a run
+  Planned planned;
 };
 
 // Lane i's value, for an i that is the same in all lanes (a read of a scalar
@@ -527,10 +538,12 @@ template <bool kDrawn>
 __device__ __forceinline__ bool load_tree(const Verify &a, int s, Tree &t) {
   const int lane = threadIdx.x & 63;
   t.start = a.starts[s], t.n = a.starts[s + 1] - t.start;
-  if (t.n < 1 || t.n > a.max_nodes || t.start < 0 || t.start > a.rows - t.n) return false;
+  const bool planned = a.planned.now();
+  if (!planned || t.n < 1 || t.n > a.max_nodes || t.start < 0 || t.start > a.rows - t.n)
+    return false;
   const int row = t.start + min(lane, t.n - 1);
   t.up = lane < t.n ? a.parents[row] : -1;
-  if (t.up >= lane) t.up = -1;  // (of a plan that was never made)
+  if (t.up >= lane) t.up = -1;  // (of parents that were written over)
   t.token = a.tokens[row];
   t.in = t.token >= 0 && t.token < a.V;
   t.u = (double)a.accept[row];
@@ -1078,7 +1091,8 @@ extern "C" int ecf8_draft_verify(const ecf8_paged_batch *b, const ecf8_draft_tre
            t->kept, t->path, b->refused, t->emitted, t->next_token,
            reinterpret_cast<double *>(base + w.runs), reinterpret_cast<double *>(base + w.mass),
            reinterpret_cast<Ended *>(base + w.ended), w.nodes, b->seqs, (int)rows, (int)V,
-           t->max_nodes, t->max_children, w.packed, 1, 256};
+           t->max_nodes, t->max_children, w.packed, 1, 256,
+           {reinterpret_cast<const Counts *>(base), step_of(b), schedule_stamp(b, t)}};
   // A wave a run once that leaves four workgroups a CU.  64 chains of 5 drawn from 32000:
   // 15 us, 22 with four waves; 8 trees of 32 from 151936: 32 with four, 39 with one.
   if (b->seqs * (kRuns / 4) >= 1024) a.per = 4, a.lanes = 64;

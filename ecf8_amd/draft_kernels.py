@@ -149,7 +149,8 @@ def draft_verify(trees: DraftTrees, tokens, target, accept, sample, draft=None):
     in any way that does not look at the random numbers (a drafter's most probable
     ones); with ``draft`` fp32 [N, V] they were drawn, independently, from that
     row's probabilities.  Either way the emitted tokens are distributed as the
-    target's own.  Fills ``kept``, ``path``, ``emitted`` and ``next_token``."""
+    target's own.  Fills ``kept``, ``path``, ``emitted`` and ``next_token``; trees that
+    were not planned for the batch's step are refused, all sequences idle."""
     batch = trees.batch
     dev = batch.device
     _unfollowed("target accept sample draft", target, accept, sample, draft)

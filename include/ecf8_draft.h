@@ -118,8 +118,9 @@ int ecf8_token_probabilities(const void *logits, int64_t ld, int64_t rows, int64
  * target probabilities.  All in 64 bits.  The tokens so emitted are distributed
  * as the target's own.  Fills kept, path, emitted and next_token.
  * rows: those of target, draft and tokens; a step of more rows sets `refused`,
- * and so do tokens outside [0, V), which are never accepted, and probabilities
- * whose sum is not above zero and finite (next token -1).
+ * and so do tokens outside [0, V), which are never accepted, probabilities
+ * whose sum is not above zero and finite (next token -1), and trees that were not
+ * planned for this step, of which every sequence is left idle.
  */
 int ecf8_draft_verify(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees,
                       const int64_t *tokens, int64_t rows, const float *target, int64_t ld_target,

@@ -78,3 +78,37 @@ def test_attention_over_a_plan_of_another_step_writes_nothing(cuda_device, cache
         assert attend() == 0
         rows = sum(now)
         assert bool((out[:rows] == 2.0).all()) and bool((out[rows:] == 3.0).all())
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_verification_over_a_plan_of_another_step_is_refused(cuda_device, drawn):
+    """Never planned, planned before the step changed, and planned again: no sequence has a
+    result of another step's parents."""
+    from ecf8_amd.draft_kernels import DraftTrees, draft_plan, draft_verify
+    from ecf8_amd.paged_kernels import paged_plan
+
+    dev, V = cuda_device, 40
+    b, t, _ = _step(dev, [5, 9, 0], [[-1, 0, 1], [-1, 0], []], max_nodes=4, kids=2, rows=12)
+    p = torch.full((6, V), 1.0 / V, device=dev)
+    tokens = torch.arange(6, device=dev)
+    accept, sample = torch.zeros(6, device=dev), torch.zeros(3, device=dev)
+
+    def verify(t):
+        for x in (t.kept, t.path, t.emitted, t.next_token):
+            x.fill_(77)
+        draft_verify(t, tokens, p, accept, sample, draft=p if drawn else None)
+        return _refused(b)
+
+    def idle(t):
+        return (bool((t.kept == 0).all()) and
+                all(bool((x == -1).all()) for x in (t.path, t.emitted, t.next_token)))
+
+    assert verify(t) == 0 and t.kept.tolist() == [3, 2, 0]
+    assert verify(DraftTrees(b, 4, 2)) == 1
+    fresh = DraftTrees(b, 4, 2)
+    assert verify(fresh) == 1 and idle(fresh)
+    for cached, new in (([8, 11, 0], [3, 2, 0]), ([5, 9, 0], [3, 2, 1]), ([5, 9, 0], [3, 2, 1])):
+        paged_plan(b, *(torch.tensor(x, dtype=torch.int32).to(dev) for x in (cached, new)))
+        assert verify(t) == 1 and idle(t)
+        draft_plan(t, torch.tensor([-1, 0, 0, -1, 0, -1], dtype=torch.int32).to(dev))
+        assert verify(t) == 0 and t.kept.tolist() == [2, 2, new[2]]
