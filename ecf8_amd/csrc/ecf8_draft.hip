@@ -463,6 +463,8 @@ struct Planned {
   __device__ __forceinline__ bool now() const {
     return (int)(counts->stamp == stamp) & (int)(counts->step == *step);
   }
+  // (neither, of trees that never were planned)
+  __device__ __forceinline__ bool other() const { return !now() && counts->stamp != 0; }
 };
 
 // Where a sequence's walk ended, for the kernel that draws its next token.
@@ -943,6 +945,7 @@ constexpr int kKeepPools = 128, kKeepAtOnce = 8;
 struct Keep {
   const int *starts, *lengths, *table, *kept, *path;
   int *refused;
+  Planned planned;
   int width, shift, Hkv, max_nodes, units, n, per;  // units: of 16 bytes a row
   uint32_t pages;
   uint8_t *pool[kKeepPools];
@@ -959,7 +962,12 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int start = a.starts[s], n = a.starts[s + 1] - start, cached = a.lengths[s] - n;
   int kept = a.kept[s];
+  const bool other = a.planned.other();
   if (kept < 1) return;
+  if (other) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.refused) *a.refused = 1;
+    return;
+  }
   const int row = lane < a.max_nodes ? a.path[(size_t)s * a.max_nodes + lane] : -1;
   const int before = __shfl_up(row, 1);
   const bool bad = lane < kept && (lane == 0 ? row != 0 : row <= before || row >= n);
@@ -1121,6 +1129,7 @@ extern "C" int ecf8_draft_keep(const ecf8_paged_batch *b, const ecf8_draft_trees
   Keep a{};
   a.starts = b->starts, a.lengths = b->lengths, a.table = b->table;
   a.kept = t->kept, a.path = t->path, a.refused = b->refused;
+  a.planned = {static_cast<const Counts *>(t->work), step_of(b), schedule_stamp(b, t)};
   a.width = b->width, a.shift = __builtin_ctz((unsigned)b->page_size), a.Hkv = b->Hkv;
   a.max_nodes = t->max_nodes, a.units = fp8 ? kD / 16 : kD / 8, a.pages = (uint32_t)b->pages;
   for (int i0 = 0; i0 < n_pools; i0 += kKeepPools) {

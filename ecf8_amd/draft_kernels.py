@@ -199,8 +199,9 @@ class KeepPlan:
 def draft_keep(plan: KeepPlan):
     """Move the keys and values of the accepted rows together: in all pools the row
     at position cached[s] + path[s, i] goes to cached[s] + i, i < kept[s].  The next
-    step has ``kept`` more tokens in the cache.  Once a step and list of pools: a
-    second call would move what is in its place."""
+    step has ``kept`` more tokens in the cache.  Before ``paged_plan`` plans the next
+    one: the trees are of another step then, which is refused.  Once a step and list of
+    pools: a second call would move what is in its place."""
     trees, batch = plan.trees, plan.trees.batch
     _launch("ecf8_draft_keep", batch.device, batch._ref, trees._ref, plan._ref, len(plan.pools),
             plan.fp8)

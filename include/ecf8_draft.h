@@ -133,8 +133,9 @@ int ecf8_draft_verify(const ecf8_paged_batch *batch, const ecf8_draft_trees *tre
  * or, fp8 != 0, e4m3fn), the row at position cached[s] + path[s][i] goes to
  * cached[s] + i for i < kept[s], as if all were read before any is written.
  * cached: the batch's lengths less the step's rows.  A path that is not ascending
- * from 0 within the sequence's rows sets `refused` and is cut there.  Once a step:
- * a second call would move what is in its place.
+ * from 0 within the sequence's rows sets `refused` and is cut there.  Trees that
+ * were planned, but for another step, set it too, and nothing moves.  Once a step: a
+ * second call would move what is in its place.
  */
 int ecf8_draft_keep(const ecf8_paged_batch *batch, const ecf8_draft_trees *trees,
                     void *const *pools, int n_pools, int fp8, void *stream);

@@ -112,3 +112,35 @@ def test_verification_over_a_plan_of_another_step_is_refused(cuda_device, drawn)
         assert verify(t) == 1 and idle(t)
         draft_plan(t, torch.tensor([-1, 0, 0, -1, 0, -1], dtype=torch.int32).to(dev))
         assert verify(t) == 0 and t.kept.tolist() == [2, 2, new[2]]
+
+
+def test_a_move_of_another_step_is_refused(cuda_device):
+    """The next step's lengths would send the kept rows to other places: after its plan
+    nothing moves.  Paths of a caller's own do, of trees that were never planned."""
+    from ecf8_amd.draft_kernels import DraftTrees, KeepPlan, draft_keep, draft_plan
+    from ecf8_amd.paged_kernels import paged_plan
+
+    dev = cuda_device
+    b, t, parents = _step(dev, [5, 0], [[-1, 0, 1, 0], []], max_nodes=4, kids=2, rows=8)
+    pools = [torch.zeros(b.pages, 1, 16, D, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    page = int(b.table[0, 0])
+
+    def keep(t):
+        for p in pools:
+            p[page, 0] = torch.arange(16, device=dev)[:, None].bfloat16()
+        t.kept.copy_(torch.tensor([2, 0]))
+        t.path.copy_(torch.tensor([[0, 3, -1, -1], [-1] * 4]))
+        draft_keep(KeepPlan(t, [tuple(pools)]))
+        bad = _refused(b)
+        assert torch.equal(*pools)
+        return bad, [int(x) for x in pools[0][page, 0, :, 0]]
+
+    rows = list(range(16))
+    moved = rows[:6] + [8] + rows[7:]
+    assert keep(t) == (0, moved)
+    for cached, new in (([7, 0], [4, 0]), ([5, 0], [4, 3]), ([5, 0], [4, 0])):
+        paged_plan(b, *(torch.tensor(x, dtype=torch.int32).to(dev) for x in (cached, new)))
+        assert keep(t) == (1, rows), (cached, new)
+    draft_plan(t, parents)
+    assert keep(t) == (0, moved)
+    assert keep(DraftTrees(b, 4, 2)) == (0, moved)
