@@ -858,7 +858,9 @@ __global__ __launch_bounds__(256) void pick_kernel(Verify a) {
     const bool whole = !(total > 0.0);
     if (whole) upto = wave_scan(sum_p), total = lane_of(upto, 63), mine = sum_p;
     const double goal = fmax(sample, 0.0) * total;
-    const uint64_t over = __ballot(upto > goal), some = __ballot(mine > 0.0);
+    // (a run of nothing can pass the goal too: lanes add in orders of their own, and
+    // their sums differ by roundings)
+    const uint64_t some = __ballot(mine > 0.0), over = some & __ballot(upto > goal);
     // (a sample of one or more: the last that there is)
     const int run = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
     const double before = lane_of(upto, max(run - 1, 0));

@@ -6,6 +6,7 @@ from __future__ import annotations
 import random
 
 import draft_model as M
+import numpy as np
 import pytest
 import torch
 from test_draft_gpu import D, _check, _filled, _rand, _refused, _seen, _step
@@ -144,3 +145,58 @@ def test_a_move_of_another_step_is_refused(cuda_device):
     draft_plan(t, parents)
     assert keep(t) == (0, moved)
     assert keep(DraftTrees(b, 4, 2)) == (0, moved)
+
+
+def _wave_scan(v):
+    """The inclusive sums of 64 values in the order in which a wave adds them."""
+    for o in (1, 2, 4, 8):
+        v = [x + v[i - o] if i % 16 >= o else x for i, x in enumerate(v)]
+    v = [x + v[i // 16 * 16 - 1] if i // 16 in (1, 3) else x for i, x in enumerate(v)]
+    return [x + v[31] if i >= 32 else x for i, x in enumerate(v)]
+
+
+def _sums_that_differ(seed):
+    """(values, i): half of the sum of 64 fp32 values lies between the wave's sums up to i - 1
+    and up to i, although value i is zero: the two were added in different orders."""
+    rng = random.Random(seed)
+    while True:
+        v = [float(np.float32(rng.random() * 2.0 ** -rng.randrange(60))) if rng.random() < 0.5 else 0.0
+             for _ in range(64)]
+        upto = _wave_scan(v)
+        for i in range(1, 60):
+            if v[i] == 0.0 and upto[i] > upto[i - 1]:
+                # values after i that double the sum before it
+                rest, parts = 2 * upto[i - 1] - upto[i], []
+                for _ in range(3):
+                    parts.append(float(np.float32(rest - sum(parts))))
+                if min(parts) < 0 or sum(parts) != rest:
+                    continue
+                w = v[: i + 1] + [0.0] * (63 - i)
+                for at, x in zip(rng.sample(range(i + 1, 64), 3), parts):
+                    w[at] = x
+                upto = _wave_scan(w)
+                if w[next(k for k in range(64) if upto[k] > 0.5 * upto[63])] == 0.0:
+                    return w, i
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_the_next_token_is_never_of_a_run_of_nothing(cuda_device, drawn):
+    """Probabilities whose partial sums, one a run of the vocabulary, rise by a rounding where
+    nothing is, and a sample that falls between the two: the token before or after is meant."""
+    from ecf8_amd.draft_kernels import draft_verify
+
+    dev, S, V = cuda_device, 24, 256  # 64 runs of four
+    cases = [_sums_that_differ(seed) for seed in range(S)]
+    b, t, _ = _step(dev, [1] * S, [[-1]] * S, max_nodes=1, kids=1)
+    p = torch.zeros(S, V)
+    for s, (w, _) in enumerate(cases):
+        p[s, s % 4:: 4] = torch.tensor(w)
+    p = p.to(dev)
+    half = torch.full((S,), 0.5, device=dev)
+    draft_verify(t, torch.zeros(S, dtype=torch.int64, device=dev), p, half, half,
+                 draft=p.clone() if drawn else None)
+    assert not _refused(b)
+    for s, (w, i) in enumerate(cases):
+        has = [k for k in range(64) if w[k]]
+        near = [max(k for k in has if k < i), min(k for k in has if k > i)]
+        assert int(t.next_token[s]) in [4 * k + s % 4 for k in near], s
