@@ -3,6 +3,7 @@ than it says (include/ecf8_draft.h), beside those of test_draft_gpu.py."""
 
 from __future__ import annotations
 
+import math
 import random
 
 import draft_model as M
@@ -200,3 +201,98 @@ def test_the_next_token_is_never_of_a_run_of_nothing(cuda_device, drawn):
         has = [k for k in range(64) if w[k]]
         near = [max(k for k in has if k < i), min(k for k in has if k > i)]
         assert int(t.next_token[s]) in [4 * k + s % 4 for k in near], s
+
+
+LOG2E = 1.4426950408889634
+
+
+def _scale_error(t):
+    """What rounding log2(e) / t to fp32 changes, relative to it."""
+    return float(np.float32(LOG2E / t)) * t / LOG2E - 1
+
+
+def test_sums_of_probabilities_have_all_of_the_temperature(cuda_device):
+    """One logit of 0 and n of -D, at temperatures of which D log2(e) / T is 12 to within
+    2^-22: as a product with both parts it rounds to 12, the terms are 2^-12 and sums of them
+    exact in fp32, so the first probability is off by 2^-22 ln 2 of the exponent and 2^-23 of
+    the quotient.  With log2(e) / T rounded to fp32 the product is the next value, 2^-20 away,
+    and the sum off by 2^-20 ln 2, four times that."""
+    from ecf8_amd.draft_kernels import token_probabilities
+
+    dev, V = cuda_device, 151_936
+    cases = []
+    for D in np.arange(4.0, 16.0, 0.0625):  # (exact in bf16)
+        t = float(np.float32(D * LOG2E / 12))
+        if (abs(D * LOG2E / t - 12) < 2.0 ** -22
+                and abs(float(np.float32(D) * np.float32(LOG2E / t)) - 12) >= 2.0 ** -21):
+            cases.append((float(D), t))
+    assert len(cases) > 3
+    x = torch.zeros(len(cases), V, device=dev)
+    x[:, :-1] = -torch.tensor([d for d, _ in cases], device=dev)[:, None]
+    for first in (V - 1, 0, 70_001):
+        row = x.roll(first + 1, 1).bfloat16()
+        out = torch.empty(row.shape, device=dev)
+        token_probabilities(row, torch.tensor([t for _, t in cases], device=dev), out)
+        for i, (d, t) in enumerate(cases):
+            want = torch.softmax(row[i].double() / t, -1)
+            error = ((out[i].double() - want).abs() / want).amax()
+            # (and the others' of the same exponent once more, and of a product)
+            assert abs(float(out[i, first]) / float(want[first]) - 1) <= 0.7 * 2 ** -22 + 2 ** -23, (d, t)
+            assert float(error) <= 1.4 * 2 ** -22 + 2 ** -22, (d, t)
+            assert abs(float(out[i].double().sum()) - 1) <= 2 ** -22, (d, t)
+
+
+def test_small_probabilities_have_all_of_the_temperature(cuda_device):
+    """One logit of 0 and others so far below that the sum is 1: a probability e^-|e| has the
+    exponent's one rounding, |e| 2^-24 (the logits' differences are exact), and the
+    exponential's, 2^-22.  Temperatures whose log2(e) / T is off by nearly 2^-24 in fp32."""
+    from ecf8_amd.draft_kernels import token_probabilities
+
+    dev, V, rng = cuda_device, 4096, random.Random(1)
+    temps = []
+    while len(temps) < 8:
+        t = float(np.float32(2.0 ** rng.randrange(-4, 3) * LOG2E * (1 - 0.01 * rng.random())))
+        if abs(_scale_error(t)) > 0.8 * 2 ** -24:
+            temps.append(t)
+    for t in temps:
+        step = 2.0 ** math.floor(math.log2(t / 2))
+        k = torch.arange(V, device=dev) % 256
+        x = (-step * k).bfloat16()
+        keep = (-x.double() / t > 40) & (-x.double() / t < 85)
+        x = torch.where(keep, x, -math.inf)
+        x[17] = 0.0
+        assert int(keep.sum()) > V // 16
+        out = torch.empty(1, V, device=dev)
+        token_probabilities(x[None], t, out)
+        e = x.double() / t
+        bound = e.abs() * 2.0 ** -24 + 2.0 ** -22
+        error = out[0].double() / e.exp() - 1
+        assert bool((error[keep].abs() <= bound[keep]).all()), t
+        assert float(out[0, 17]) == 1.0
+
+
+@pytest.mark.parametrize("N,V", [(1, 1), (3, 9), (5, 4099), (5, 151_936), (70, 50_257), (300, 2048),
+                                 (2, 300_001)])
+@pytest.mark.parametrize("scale", [0.1, 3.0, 60.0])
+def test_probabilities_to_the_last_bits(cuda_device, N, V, scale):
+    """A difference of logits and its product round once each, 2^-24 of the exponent e; the
+    exponential by 2^-23.  Sums are taken in up to 36 additions in a row, 2^-24 each, and
+    rescaled up to 11 times, 2^-22 each, which split an exponent without adding to it; the
+    quotient's two roundings are 2^-23.  In all (|e| + sum p |e| + 45) 2^-23 of p, and of the
+    row's sum twice the weighted part."""
+    from ecf8_amd.draft_kernels import token_probabilities
+
+    dev = cuda_device
+    gen = torch.Generator(device=dev).manual_seed(V)
+    x = _rand(N, V, gen=gen, scale=scale)
+    temps = torch.tensor([[0.7, 1.0, 2.5, 0.05, 0.013][i % 5] for i in range(N)], device=dev)
+    out = torch.empty(N, V, device=dev)
+    token_probabilities(x, temps, out)
+    for i in range(N):
+        e = x[i].double()
+        e = (e - e.max()) / float(temps[i])
+        want = torch.softmax(e, -1)
+        mean = float((want * e.abs()).sum())
+        error = (out[i].double() - want).abs()
+        assert bool((error <= want * (e.abs() + mean + 45) * 2.0 ** -23 + 2.0 ** -126).all()), i
+        assert abs(float(out[i].double().sum()) - 1) <= (2 * mean + 45) * 2.0 ** -23 + V * 2.0 ** -126, i
