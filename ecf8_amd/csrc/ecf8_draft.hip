@@ -44,7 +44,7 @@ constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPer = kMaxSeqs / kPlanThreads;
 constexpr int kLeast = 1;  // units on both sides of a cut
 // What a workgroup's first loads and last sums take, in units.  64 trees after 512
-// keys: of 8 tokens 26.6 us, 29.8 with one; of 32 39 and 47; few long ones alike.
+// keys: of 8 tokens 25 us, 28.5 with one; of 32 42 and 50; few long ones alike.
 constexpr int kBegin = 5;
 
 // The exclusive prefix sums of N values over the workgroup, and their totals.
@@ -229,7 +229,7 @@ __device__ __forceinline__ void plan_schedule(const Plan &a) {
 }
 
 // The first workgroup schedules, the others take 16 sequences' trees each.  Latency of
-// loads, scans and barriers in a row: 6.5 us of one tree, 7.5 of 512.
+// loads, scans and barriers in a row: 6.6 us of 16 trees, 6.7 of 512.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(Plan a) {
   if (blockIdx.x == 0) {
     plan_schedule(a);
@@ -315,7 +315,7 @@ __device__ __forceinline__ void for_run(const Probs &a, int row, Vec, Units unit
 }
 
 // The largest logit of a run of a row and the sum of the exponentials below it;
-// greedy rows: the best key.  Bound by HBM: 416 rows of 151936 (126 MB) 28 us, 4.5
+// greedy rows: the best key.  Bound by HBM: 416 rows of 151936 (126 MB) 28.5 us, 4.4
 // TB/s; the second kernel (253 MB written) 46 us, 5.5 TB/s.
 __global__ __launch_bounds__(256) void probability_stats_kernel(Probs a) {
   __shared__ uint64_t s_k[4];

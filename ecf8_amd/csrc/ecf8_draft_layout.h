@@ -23,17 +23,18 @@ constexpr int kEndedBytes = 1056;  // of where a sequence's walk ended
 
 // Rows (token, head of the group) of a workgroup of the attention: what a sequence
 // has, in as few workgroups as registers allow, since each reads the sequence's pages.
-// One tree of 8 in groups of four after 4096: 12.6 us in 32 rows, 13.2 in 64; 16 trees
-// of 32 after 8192 e4m3 keys 63 in 128, 72 in 256; of 64 after as many bf16 ones 95 in
-// 256, 109 in two of 128.
+// One tree of 8 in groups of four after 4096: 12.5 us in 32 rows, 13.2 in 64; 16 trees
+// of 64 after 8192 bf16 keys 94 in 256, 132 in two of 128.  (Of 32 they take 87 in 128
+// and 74 in 256, since probabilities of 256 rows are rounded once.)
 inline int tile_rows(int max_nodes, int group) {
   const int r = max_nodes * group;
   return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256;
 }
 // Does a workgroup of 64 or 128 rows have a second group of waves, for half of its keys?
 // Where every sequence and head can have a CU of its own: half as many pieces to join.
-// Eight trees of 26 after 8192: 35 us, 40 without; 32 of 32 after 512 29 and 34; 64
-// (two rounds of CUs) of 32 after 512 49 and 39; short e4m3 ones up to 2 us more.
+// Eight trees of 26 after 8192: 38 us, 43 without; 32 of 32 after 512 29.5 and 35; 64
+// (two rounds of CUs) of 32 after 512 49 and 42; some 2 to 3 us more: 16 of 32 after 1024
+// 33 and 30, 32 of 8 with 8 heads a group after 512 19.7 and 17.7.
 inline bool in_halves(int tile, int64_t seqs, int Hkv) {
   return (tile == 64 || tile == 128) && seqs * Hkv <= 256;
 }

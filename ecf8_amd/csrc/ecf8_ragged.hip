@@ -690,7 +690,7 @@ __device__ __forceinline__ void lds_barrier() {
 //
 // kTree: the step's trees (rows read the cached positions and their masks'), up to 32
 // rows.  64 chains of 5 in groups of four after up to 8192 keys, 1.1 GB: 178 us, 6.1
-// TB/s.  T = 1 up to 16 rows: one tree of 4 after 4096 11 us, 12 with T = 2.
+// TB/s.  T = 1 up to 16 rows: one tree of 4 after 4096 10.5 us, 11.5 with T = 2.
 template <Source kSrc, int T, bool kTree = false>
 __global__ __launch_bounds__(256, 2) void few_kernel(Attn a) {
   __shared__ u32x4 s_kv[4][32 * (kKeyRow + kValueRow)];  // a wave's keys and values
@@ -1258,15 +1258,16 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, Joins few, Joins tile
 // registers, two steps ahead, to a ring of LDS stages.  kGroups = 2: eight waves, two
 // groups with a ring each, which take half of the keys and join over LDS.
 //
-// Bound by what of the softmax does not hide behind the products: both together take
-// 0.8 to 1.0 of their sum, whatever their order, and a step's 32 keys cost 16 T rows
-// 17 T products (kFine 25 T) and some 45 T vector instructions.  Eight trees of 64 with
-// 8 heads a group (two tiles of 256) after 32768 e4m3 keys: 175 us with the join, 870
-// TFLOP/s of the 1240 that a large library product reaches beside it.  Smaller trees
-// wait for memory too: 24 of up to 26 after up to 6000 bf16 keys 52 to 56 us by card,
-// 4 TB/s.
+// A step's 32 keys cost 16 T rows 17 T products (kFine 25 T) and some 45 T vector
+// instructions, which in the loop take 0.8 to 1.0 of the sum of their times, whatever
+// their order.  256 rows and long contexts are bound by them: eight trees of 64 with 8
+// heads a group (two tiles of 256) after 32768 e4m3 keys, 175 us with the join, 870
+// TFLOP/s of the 1240 that a large library product reaches beside it; the two units'
+// cycles add up to 71% of the launch.  Of smaller trees, 24 of up to 26 after up to 6000
+// bf16 keys, 57 to 62 us by card, 3.7 TB/s, they are two thirds: the rest is the pieces'
+// first loads and last sums, and a barrier every 32 keys.
 // kOnce, pages past the caches, where a sequence's pages are read by one workgroup:
-// those took 55 us, 63 through the caches; of two tiles (16 trees of 64 with 8
+// those take 61 us, 63 through the caches; of two tiles (16 trees of 64 with 8
 // heads a group, after 8192) 92 us, and 95 past the caches.
 // Not faster: 128 rows in eight waves, 192 in four (registers spill), half of the
 // waves for the staging alone (bf16 5% faster where contexts are long, e4m3 and short
@@ -1283,8 +1284,8 @@ __global__ __launch_bounds__(64 * kGroups * kWaves, 2) void tree_kernel(Attn a) 
   constexpr int kLoads = kHalves ? 1 : 32 / kPass;
   // after the barrier before step j the waves read steps j - 1 to j + 1 and write j + 2
   constexpr int kRing = 4;
-  // steps that two groups share: one tree of 32 after 4096 (pieces of 13 steps) 19.6 us,
-  // 21 from eight on; 32 of 8, 8 heads a group, after up to 512 19.2 and 18.0
+  // steps that two groups share: one tree of 32 after 4096 (pieces of 13 steps) 20.5 us,
+  // 21.5 from eight on; 32 of 8, 8 heads a group, after up to 512 19.7 and 18.8
   constexpr int kBoth = 16;
   __shared__ u32x4 s_rings[kGroups][kRing][32 * (kKeyRow + kValueRow)];
   __shared__ int s_odds[kGroups];
@@ -1796,7 +1797,7 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
   j.n = &counts->joins, j.list = reinterpret_cast<const Join *>(base + w.joins_at);
   j.stats = a.stats, j.sums = a.sums;
   // rows a workgroup: eight, fewer while there are not a thousand workgroups (one tree
-  // of 8 after 4096: 12.6 us, 14.3 with eight; 16 of 32 after 8192: 75, 91 with one)
+  // of 8 after 4096: 12.5 us, 14.2 with eight; 16 of 32 after 8192: 87, 97 with one)
   const int most_rows = trees->max_nodes * a.group < w.tile ? trees->max_nodes * a.group : w.tile;
   const int64_t splits = (tiles < cuts ? tiles : cuts) * a.Hkv;
   int per = 8;
@@ -1822,7 +1823,7 @@ extern "C" int ecf8_draft_attention(const void *q, int64_t q_stride, int64_t row
     case 32:
       ECF8_TREE_FEW(2);
       break;
-    case 64:  // (two parts cost nothing in bf16, a tenth in e4m3)
+    case 64:  // (two parts cost up to 3% in bf16, a tenth in e4m3)
       if (halves) ECF8_TREE(2, 4, 1, true, true);
       else ECF8_TREE(1, 4, 1, true, true);
       break;

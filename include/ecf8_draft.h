@@ -39,7 +39,9 @@ extern "C" {
  *   work       ecf8_draft_work_bytes bytes, 16-byte aligned, its first 256
  *              bytes zeros before the first plan
  * max_nodes: most rows of a sequence, up to 64; max_children: most rows after
- * one row.
+ * one row.  Kernels and launches go by these, not by what a step's trees hold: spare
+ * rows make larger tiles (past 128 a group, of less exact probabilities), and each
+ * child past the first is a launch of every verification of drawn drafts.
  */
 typedef struct ecf8_draft_trees {
   uint64_t *masks;
